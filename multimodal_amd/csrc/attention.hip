@@ -316,7 +316,7 @@ __global__ __launch_bounds__(256, (HD == 64 ? 2 : 1)) void attn_fwd_k(u16* __res
                 rmax = vmax2(lo, hi);
             }
             const float m_new = vmax2(rmax * scale_log2e, m_run);
-            // packed fp32 math (v_pk_fma_f32 / v_pk_add_f32): two scores per VALU issue
+            // two scores at a time (plain fp32: the build has no packed fp32 instructions, see the Makefile)
             const f32x2 sc2 = {scale_log2e, scale_log2e}, mn2 = {m_new, m_new};
             f32x2 lsum2 = {0.f, 0.f};
 #pragma unroll
@@ -574,7 +574,7 @@ __global__ __launch_bounds__(256, (HD == 64 ? 2 : 1)) void attn_bwd_dq_k(u16* __
                         sacc[i] = mk ? 0.f : p * (dpacc[i] - dlt);
                     }
                 } else {
-                    // packed fp32 math, two scores per VALU issue; the causal select is a separate, wave-uniformly
+                    // two scores at a time; the causal select is a separate, wave-uniformly
                     // branched pass that only the tiles on this wave's diagonal execute
                     // scalar fp32 on purpose: v_pk_*_f32 serialise with the partner wave's MFMAs, plain VALU overlaps them
                     // (tools/ubench/coissue.hip)
@@ -755,7 +755,7 @@ __global__ __launch_bounds__(256, (HD == 64 ? 2 : 1)) void attn_bwd_dkv_k(u16* _
                 // wave-uniform: only tiles on this wave's diagonal (or the ragged last tile) pay for the compare/select
                 const bool need_mask = (wave_first + 31 > q0t + 32 * t) || (q0t + 32 * t + 32 > s);
                 if (MODE == 0) {
-                    // packed fp32 math, two scores per VALU issue; the causal select is its own wave-uniformly branched pass
+                    // two scores at a time; the causal select is its own wave-uniformly branched pass
 #pragma unroll
                     for (int g4 = 0; g4 < 4; ++g4) {
                         const int ql = 32 * t + 8 * g4 + 4 * hh;  // local row of register 4*g4
