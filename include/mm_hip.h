@@ -357,6 +357,63 @@ int mm_adam_step(void* const* params, const void* const* grads, float* master, f
                  const void* chunks, int nchunks, float* partial, int* step, float* grad_norm_out, float lr,
                  const float* lr_dev, float beta1, float beta2, float eps, float weight_decay, float max_grad_norm, int bias_correction, int dtype, void* stream);
 
+/* ------------------------------------------------------------------ text generation: the paged key / value cache
+ * The counterpart of use_cache / layer_past (megatron/model/transformer.py:361-365, 602-610, 638-639), which concatenates
+ * [past | new] keys and values for every token: here a layer's keys and values live in pages of page_size token slots that
+ * sequences take as they grow, and a step appends to them in place.
+ *
+ * mm_paged_kv: one layer's pages.  k, v point at page 0, head 0, slot 0; the strides are in elements (a slot's hn elements are
+ * contiguous), each a multiple of 8 and below 2^31, page strides times 2 below 2^32 bytes; k and v 16-byte aligned.  hn in {64, 128}. */
+typedef struct mm_paged_kv {
+    void* k;
+    void* v;
+    int64_t k_page, k_head, k_slot, v_page, v_head, v_slot;
+    int num_pages, page_size, heads, hn, dtype;
+} mm_paged_kv;
+/* mm_paged_step: what one step brings, shared by all layers; every array is in device memory and read at run time, so that a
+ * captured step follows what its caller writes there between replays.
+ *   block_table [seqs, max_pages] (rows table_stride apart): the pages of each sequence, in order;
+ *   cu_new [seqs + 1], ascending: sequence i brings the packed rows cu_new[i] .. cu_new[i + 1] - 1 (none is allowed);
+ *   kv_lens [seqs]: its length INCLUDING the new rows; row j of n has position kv_lens - n + j.
+ * max_new / max_kv: upper bounds of a sequence's new rows / length (they size the launches).
+ * What the arrays hold is checked on the device, never trusted for an address:
+ *   - a row outside every sequence is neither read nor written;
+ *   - a row whose position is negative, behind block_table's last page, behind the cos / sin tables, or in a page outside
+ *     [0, num_pages) leaves the cache alone, and its q_out row is NaN;
+ *   - attention: a key in a page outside [0, num_pages) makes every row that sees it NaN, and a sequence that exceeds max_new,
+ *     max_kv, its block_table row or the packed rows has all its rows NaN (a wrong step never gives a wrong number). */
+typedef struct mm_paged_step {
+    const int32_t* block_table;
+    const int32_t* cu_new;
+    const int32_t* kv_lens;
+    int64_t table_stride;
+    int seqs, max_pages, max_new, max_kv;
+} mm_paged_step;
+/* Append: key / value rows [rows, kv->heads, hn] go to their slots; with cos / sin the first rot_d dims of the keys, and of the
+ * queries on their way to q_out, are rotated by their position: x cos[p] + rotate_half(x) sin[p]
+ * (megatron/model/positional_embeddings.py:69-92), products and sum in fp32, rounded once.  q / q_out [rows, nq, hn] (NULL: keys
+ * and values only); q_out may be q.  cos / sin [table_rows, rot_d] contiguous, fp32 (table_fp32 != 0) or in the cache's dtype;
+ * NULL with rot_d = 0: no rotation.  rot_d even.  Strides in elements, any alignment of the rows (16-byte aligned rows with
+ * strides a multiple of 8 and rot_d a multiple of 16 take the wide path).  Two rows of one call must not share a slot, and
+ * rows must not overlap the cache. */
+int mm_paged_kv_append(const mm_paged_kv* kv, const mm_paged_step* step, const void* k, int64_t k_row, int64_t k_head,
+                       const void* v, int64_t v_row, int64_t v_head, const void* q, int64_t q_row, int64_t q_head, void* q_out,
+                       int64_t qo_row, int64_t qo_head, int nq, int rows, const void* cos, const void* sin, int rot_d,
+                       int table_rows, int table_fp32, void* stream);
+
+/* Attention of the step's new rows over the cache (append first): row j of sequence i sees the keys at positions 0 .. p of its
+ * sequence, p = kv_lens[i] - n + j; query head h reads key head h / (nq / kv->heads), nq a multiple of kv->heads:
+ *   out[row, h] = softmax(softmax_scale q k^T) v in the cache's dtype, lse[row, h] = ln sum exp(softmax_scale q k^T) in fp32
+ * (ParallelSelfAttention.attention with layer_past, megatron/model/transformer.py:315-416).  A row that sees no key gets 0 and
+ * -inf; rows of no sequence are left as they were.  What the cache holds behind a sequence's end, and infinities or NaN in keys
+ * and values that a row does not see, do not reach it.  q, out [rows, nq, hn]: 16-byte aligned, strides a multiple of 8 elements;
+ * lse [rows, nq] with row stride l_row.  workspace: mm_paged_attn_workspace_bytes bytes (0: none; it depends on the shapes and
+ * bounds alone), 16-byte aligned; calls that share one must not overlap.  Deterministic. */
+size_t mm_paged_attn_workspace_bytes(const mm_paged_kv* kv, const mm_paged_step* step, int nq, int rows);
+int mm_paged_attn_fwd(const mm_paged_kv* kv, const mm_paged_step* step, void* out, int64_t o_row, int64_t o_head, float* lse,
+                      int64_t l_row, const void* q, int64_t q_row, int64_t q_head, int nq, int rows, float softmax_scale,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

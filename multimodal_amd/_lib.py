@@ -15,8 +15,19 @@ EPI_NONE, EPI_BIAS, EPI_BIAS_GELU_TANH, EPI_BIAS_GELU_ERF, EPI_BIAS_RELU = 0, 1,
 GEMM_TN_STATIC_MAX_FLOATS = 6 << 20  # MM_GEMM_TN_STATIC_MAX_FLOATS
 EPI_RELU_BWD, EPI_GELU_TANH_BWD, EPI_GELU_ERF_BWD = 5, 6, 7   # backward epilogues: saved forward tensor in the residual slot
 
-c_int, c_float, c_void_p, c_size_t, c_u64 = (
-    ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_uint64)
+c_int, c_float, c_void_p, c_size_t, c_u64, c_i64 = (
+    ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_uint64, ctypes.c_int64)
+
+
+class MmPagedKV(ctypes.Structure):  # mm_paged_kv
+    _fields_ = [("k", c_void_p), ("v", c_void_p)] + [(n, c_i64) for n in ("k_page", "k_head", "k_slot", "v_page", "v_head", "v_slot")] + [
+        (n, c_int) for n in ("num_pages", "page_size", "heads", "hn", "dtype")]
+
+
+class MmPagedStep(ctypes.Structure):  # mm_paged_step
+    _fields_ = [("block_table", c_void_p), ("cu_new", c_void_p), ("kv_lens", c_void_p), ("table_stride", c_i64)] + [
+        (n, c_int) for n in ("seqs", "max_pages", "max_new", "max_kv")]
+
 
 # name -> (restype, argtypes); must list every symbol include/mm_hip.h declares
 # (tests/test_abi.py cross-checks this table against the header).
@@ -80,6 +91,10 @@ PROTOTYPES = {
     "mm_prefix_tail_workspace_bytes": (c_size_t, [c_int, c_int]),
     "mm_prefix_tail_fwd": (c_int, [c_void_p] * 11 + [c_int, c_int, c_int, c_float, c_float, c_int, c_void_p, c_u64, c_int, c_void_p]),
     "mm_dropout_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_size_t, c_float, c_int, c_void_p]),
+    "mm_paged_kv_append": (c_int, [c_void_p] * 2 + [c_void_p, c_i64, c_i64] * 4 + [c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
+    "mm_paged_attn_workspace_bytes": (c_size_t, [c_void_p] * 2 + [c_int] * 2),
+    "mm_paged_attn_fwd": (c_int, [c_void_p] * 2 + [c_void_p, c_i64, c_i64, c_void_p, c_i64, c_void_p, c_i64, c_i64, c_int, c_int, c_float,
+                                                   c_void_p, c_size_t, c_void_p]),
     "mm_adam_chunk_elems": (c_int, []),
     "mm_adam_step": (c_int, [c_void_p] * 6 + [c_int, c_void_p, c_void_p, c_void_p, c_float, c_void_p] + [c_float] * 5 + [c_int, c_int, c_void_p]),
 }

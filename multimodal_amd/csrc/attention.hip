@@ -26,25 +26,11 @@
 //               the eager gpt2_attention_mask_func path).
 #include "common.h"
 #include "mfma32.h"
+#include "attn_common.h"
 
 namespace mm {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kMaskFill = -10000.0f;
-
-__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// Make a register-resident operand "used" here: the compiler must finish its global load before this point instead of
-// sinking the load to the first MFMA inside the tile loop (where its pending vmcnt would serialise every iteration's
-// prefetch behind the MFMAs).
-template <typename V> __device__ __forceinline__ void pin(V& v) {
-    u32x4 t;
-    __builtin_memcpy(&t, &v, 16);
-    asm volatile("" : "+v"(t));
-    __builtin_memcpy(&v, &t, 16);
-}
-__device__ __forceinline__ void pin(float& v) { asm volatile("" : "+v"(v)); }
 
 // Two workgroups share a CU, so every SIMD holds two waves running this same loop.  Left to age-based arbitration the wave in
 // its softmax segment keeps the issue port and the partner's MFMAs trickle in behind it (PMC: matrix pipe and vector port
@@ -66,14 +52,6 @@ __device__ __forceinline__ void mfma_prio_b(int on, bool heavy) {
     }
 }
 
-// Combine a value with the one held by the lane 32 away (the other half of the wave) without the LDS round trip of
-// ds_bpermute: v_permlane32_swap exchanges the upper 32 lanes of its first operand with the lower 32 of its second, so with
-// both operands = x every lane ends up holding (lower-half value, upper-half value) of its lane pair.
-__device__ __forceinline__ void half_pair(float x, float& lo, float& hi) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    lo = __uint_as_float(r[0]);
-    hi = __uint_as_float(r[1]);
-}
 __device__ __forceinline__ float vmax3(float a, float b, float c) {
     float r;
     asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
@@ -84,17 +62,6 @@ __device__ __forceinline__ float vmax2(float a, float b) {
     asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
     return r;
 }
-__device__ __forceinline__ float half_max(float x) {
-    float lo, hi;
-    half_pair(x, lo, hi);
-    return fmaxf(lo, hi);
-}
-__device__ __forceinline__ float half_sum(float x) {
-    float lo, hi;
-    half_pair(x, lo, hi);
-    return lo + hi;
-}
-
 // ---- attention dropout (reference megatron/model/transformer.py:301-302, 383-384: nn.Dropout on the softmax output under the
 // model-parallel rng tracker's fork).  The keep decision of probability element (batch*head, q, key) is a pure function of the
 // tracker's device-resident Philox-style state {seed, base offset}, the launch's position `pos` inside the step and the element's

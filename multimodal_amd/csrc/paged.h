@@ -1,0 +1,61 @@
+// paged.h - what the kernels of the paged key / value cache share: the row -> sequence search, the key -> page arithmetic.
+#pragma once
+#include "common.h"
+
+namespace mm {
+
+// q = n / d for 0 <= n < 2^31 without a division: with l = ceil(log2 d) and m = floor(2^32 (2^l - d) / d) + 1,
+// n / d = (mulhi(m, n) + n) >> l exactly (m / 2^32 + 1 is 2^l / d rounded up by less than 2^l / 2^32).  mulhi(m, n) < n, so the
+// sum stays below 2^32.
+struct FastDiv {
+    uint32_t d, m, l;
+};
+inline FastDiv make_fastdiv(int d) {
+    FastDiv f;
+    f.d = (uint32_t)d;
+    f.l = 0;
+    while ((1ull << f.l) < (uint64_t)d) ++f.l;
+    f.m = (uint32_t)((((1ull << f.l) - (uint64_t)d) << 32) / (uint64_t)d + 1);
+    return f;
+}
+__device__ __forceinline__ uint32_t fdiv(uint32_t n, const FastDiv& f) { return (__umulhi(f.m, n) + n) >> f.l; }
+
+// The sequence of packed row `row` in cu[0 .. n]: the number of i with cu[i + 1] <= row, found by a whole wave, 64 boundaries a
+// step (one step up to 64 sequences, two up to 4096).  n when the row is behind the last sequence; the caller also checks
+// cu[s] <= row.  Whatever cu holds, only cu[1 .. n] is read and the result is in [0, n].
+__device__ __forceinline__ int find_seq(const int32_t* __restrict__ cu, int n, int row, int lane) {
+    int lo = 0;
+    for (;;) {
+        const int step = (n + 63) >> 6;
+        const int i = lane * step + step - 1;  // the last boundary of this lane's group
+        const bool below = i < n && cu[lo + i + 1] <= row;
+        const int g = __popcll(__ballot(below));  // groups that lie wholly before the row
+        lo += g * step;
+        n -= g * step;
+        if (step == 1 || n <= 0) return lo;
+        n = n < step ? n : step;
+    }
+}
+
+inline int check_paged(const char* fn, const mm_paged_kv* kv, const mm_paged_step* st, int rows) {
+    MM_CHECK_ARG(kv && st, "%s: null cache or step", fn);
+    MM_CHECK_ARG(kv->k && kv->v && st->block_table && st->cu_new && st->kv_lens, "%s: null pointer", fn);
+    MM_CHECK_ARG(kv->hn == 64 || kv->hn == 128, "%s: head size %d not supported (64 or 128)", fn, kv->hn);
+    MM_CHECK_ARG(kv->num_pages > 0 && kv->page_size > 0 && kv->heads > 0 && rows >= 0 && st->seqs >= 0 && st->max_pages > 0,
+                 "%s: pages=%d page_size=%d heads=%d rows=%d seqs=%d max_pages=%d out of range", fn, kv->num_pages, kv->page_size,
+                 kv->heads, rows, st->seqs, st->max_pages);
+    MM_CHECK_ARG((int64_t)st->max_pages * kv->page_size < (int64_t)1 << 30, "%s: %d pages of %d slots exceed 2^30 positions", fn,
+                 st->max_pages, kv->page_size);
+    MM_CHECK_ARG(st->max_new >= 0 && st->max_kv >= 0 && st->table_stride >= st->max_pages,
+                 "%s: max_new=%d max_kv=%d table_stride=%lld out of range", fn, st->max_new, st->max_kv, (long long)st->table_stride);
+    MM_CHECK_ARG(aligned16(kv->k) && aligned16(kv->v), "%s: the cache must be 16-byte aligned", fn);
+    const int64_t str[6] = {kv->k_page, kv->k_head, kv->k_slot, kv->v_page, kv->v_head, kv->v_slot};
+    for (int64_t x : str)
+        MM_CHECK_ARG(x >= 0 && x % 8 == 0 && x < (int64_t)1 << 31, "%s: cache stride %lld must be a multiple of 8 in [0, 2^31)", fn,
+                     (long long)x);
+    MM_CHECK_ARG(kv->page_size * kv->k_slot < (int64_t)1 << 31 && kv->page_size * kv->v_slot < (int64_t)1 << 31,
+                 "%s: a page's slots span 2^31 elements or more", fn);
+    return MM_OK;
+}
+
+}  // namespace mm

@@ -1,0 +1,677 @@
+// paged_attention.hip - attention of a step's new tokens over a paged key / value cache, for gfx950.
+//
+// Row j of a sequence that brings n rows and has len tokens afterwards sits at position p = len - n + j and sees keys 0 .. p:
+// out = softmax(scale q k^T) v, lse = ln sum exp(scale q k^T) (reference: ParallelSelfAttention.attention with layer_past,
+// megatron/model/transformer.py:315-416, 602-610).  The group = nq / heads query heads of one key head and the n new tokens
+// together are the "rows" of one (sequence, key head): row r = token r / group, query head kh * group + r % group, so that a
+// key or value tile is read once for all of them.
+//
+// Softmax runs in the exp2 domain with fp32 statistics in one pass over the keys; products accumulate in fp32; the
+// probabilities (in [0, 1]) are rounded to the cache's dtype for the matrix instruction of P V, the row sum takes them unrounded.
+//
+// Masked places never matter: a score behind a row's position is replaced by -inf (not added to), value rows behind the
+// sequence's end are zeroed on their way into LDS, and where a tile holds keys that some of its rows do not see, infinities and
+// NaN in the values are taken out of the matrix product (0 * inf would spread them to those rows) and added afterwards to
+// the rows that do see them: p * v is +-inf or NaN whatever p > 0 is.
+#include "common.h"
+#include "mfma32.h"
+#include "attn_common.h"
+#include "paged.h"
+
+namespace mm {
+
+struct PagedAttnArgs {
+    mm_paged_kv kv;
+    mm_paged_step st;
+    const u16* q;
+    u16* out;
+    float* lse;
+    int64_t q_row, q_head, o_row, o_head, l_row;
+    int nq, group, rows;
+    float scale_log2e;
+    FastDiv page, grp;
+    int chunk, nsplit;  // keys per split (a multiple of the kernels' tiles), splits
+    float *ws_o, *ws_ml;  // nsplit > 1: [nsplit, rows, nq, hn] unnormalised outputs, [nsplit, rows, nq, 2] (max, sum)
+};
+
+// {first row, new rows, length} of a sequence; false: nothing to do
+struct SeqInfo {
+    int beg, n, len;
+};
+// A sequence that breaks the step's bounds has its rows set to NaN (by the workgroups with writer set) and is skipped.
+template <int HD>
+__device__ __forceinline__ bool seq_info(const PagedAttnArgs& a, int seq, int kh, bool writer, SeqInfo& s) {
+    s.beg = a.st.cu_new[seq];
+    const int end = a.st.cu_new[seq + 1];
+    s.len = a.st.kv_lens[seq];
+    if (end <= s.beg) return false;
+    if (s.beg >= 0 && end <= a.rows && end - s.beg <= a.st.max_new && s.len <= a.st.max_kv &&
+        s.len <= a.st.max_pages * (int)a.page.d) {
+        s.n = end - s.beg;
+        return true;
+    }
+    if (writer) {
+        const int b = s.beg < 0 ? 0 : s.beg, e = end < a.rows ? end : a.rows;
+        const float nan = __builtin_nanf("");
+        for (int64_t i = threadIdx.x; i < (int64_t)(e - b) * a.group * HD; i += blockDim.x) {
+            const int row = b + (int)(i / (a.group * HD)), x = (int)(i % (a.group * HD)), h = kh * a.group + x / HD;
+            a.out[(int64_t)row * a.o_row + (int64_t)h * a.o_head + x % HD] = 0x7fff;  // a NaN in both 16-bit types
+            if (x % HD == 0) a.lse[(int64_t)row * a.l_row + h] = nan;
+        }
+    }
+    return false;
+}
+
+__device__ __forceinline__ uint32_t nonfinite2(uint32_t v, uint32_t expm) {  // mask 0xffff per 16-bit value whose exponent is all ones
+    return ((v & expm) == expm ? 0xffffu : 0u) | (((v >> 16) & expm) == expm ? 0xffff0000u : 0u);
+}
+template <typename T> constexpr uint32_t exp_mask();
+template <> constexpr uint32_t exp_mask<BF16>() { return 0x7f80u; }
+template <> constexpr uint32_t exp_mask<F16>() { return 0x7c00u; }
+// takes infinities and NaN out of a 16-byte chunk; true if there were any
+template <typename T> __device__ __forceinline__ bool take_nonfinite(u32x4& v) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t m = nonfinite2(v[i], exp_mask<T>());
+        v[i] &= ~m;
+        any |= m;
+    }
+    return any != 0;
+}
+// the infinity or NaN at p, else 0
+template <typename T> __device__ __forceinline__ float only_nonfinite(const u16* __restrict__ p) {
+    const u16 v = *p;
+    return (v & exp_mask<T>()) == exp_mask<T>() ? to_f32<T>(v) : 0.f;
+}
+
+template <typename T> struct M16;
+template <> struct M16<BF16> {
+    typedef bf16x8 frag;
+    static __device__ __forceinline__ f32x4 run(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct M16<F16> {
+    typedef f16x8 frag;
+    static __device__ __forceinline__ f32x4 run(frag a, frag b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+
+// =====================================================================================  few rows: at most 16 per (sequence, key head)
+// Bound by the cache's bytes.  A wave works alone on 32-key tiles (the NW waves of a workgroup take them in turn, a grid
+// dimension splits long sequences further) and keeps a tile of keys and values in flight in registers:
+//   S^T[key][row] = K Q^T: mfma 16x16x32, the keys straight from global memory as the A operand (lane = key, 16 bytes of dims);
+//   softmax over the keys of a column: 8 registers and the four 16-lane groups;
+//   O^T[dim][row] += V^T P^T: P^T is S^T's registers as they stand - register j of sub-tile t in group g is key 16 t + 4 g + j,
+//   and the V^T operand takes its keys in that order - V through a wave-private LDS tile, read transposed (ds_read_b64_tr_b16).
+// The LDS rows are unpadded; the 32-byte units of a row are XOR-ed with the row so that the transposed reads (16 rows, one unit
+// each) and the writes (16 rows, two units each) spread evenly over the banks.
+template <int HD> __device__ __forceinline__ int v_off(int row, int byte) {
+    const int unit = byte >> 5;
+    const int swz = HD == 128 ? (row & 7) : ((row >> 1) & 3);
+    return row * (HD * 2) + ((unit ^ swz) << 5) + (byte & 31);
+}
+
+template <typename T, int HD, int NW>
+__global__ __launch_bounds__(NW * 64) void paged_attn_few_k(const PagedAttnArgs a) {
+    typedef typename M16<T>::frag frag;
+    constexpr int NC = HD / 32;  // 16-byte chunks of a key per lane = k-steps of Q K^T
+    constexpr int NDB = HD / 16;
+    constexpr int VB = 32 * HD * 2, RS = HD + 4;  // bytes of a wave's V tile; floats per row of the final exchange
+    constexpr int SM = NW * VB > NW * 16 * RS * 4 ? NW * VB : NW * 16 * RS * 4;
+    __shared__ __attribute__((aligned(16))) char smem[SM];
+    __shared__ float sm_m[NW][16], sm_l[NW][16];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, g = lane >> 4;
+    const int nkv = a.kv.heads, seq = blockIdx.x / nkv, kh = blockIdx.x % nkv, split = blockIdx.y;
+    SeqInfo s;
+    if (!seq_info<HD>(a, seq, kh, split == 0, s)) return;
+    const int R = s.n * a.group;
+    const int c0 = split * a.chunk, c1 = min(c0 + a.chunk, s.len);
+    if (split > 0 && c0 >= s.len) return;  // the combining kernel knows
+
+    const int rc = r < R ? r : R - 1;
+    const int tok = (int)fdiv((uint32_t)rc, a.grp), qh = kh * a.group + rc - tok * a.group;
+    const int limit = s.len - s.n + tok, min_limit = s.len - s.n;
+    const u16* qp = a.q + (int64_t)(s.beg + tok) * a.q_row + (int64_t)qh * a.q_head;
+    frag qf[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) qf[i] = *reinterpret_cast<const frag*>(qp + 32 * i + 8 * g);
+
+    const int32_t* bt = a.st.block_table + (int64_t)seq * a.st.table_stride;
+    const u16* kb = (const u16*)a.kv.k + (int64_t)kh * a.kv.k_head + 8 * g;
+    const u16* vb = (const u16*)a.kv.v + (int64_t)kh * a.kv.v_head + 8 * g;
+
+    u32x4 kr[2][NC], vr[2][NC];
+    int pid[2];
+    uint32_t bad = 0;  // bit t: this lane's key of sub-tile t is in a page the cache does not have
+    auto fetch_pid = [&](int kt) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int key = min(kt + 16 * t + r, s.len - 1);
+            pid[t] = bt[fdiv((uint32_t)key, a.page)];
+        }
+    };
+    auto fetch = [&](int kt) {
+        bad = 0;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int key = min(kt + 16 * t + r, s.len - 1);
+            const int off = key - (int)(fdiv((uint32_t)key, a.page) * a.page.d);
+            const bool b = (uint32_t)pid[t] >= (uint32_t)a.kv.num_pages;
+            const uint32_t pg = b ? 0u : (uint32_t)pid[t];
+            bad |= b ? 1u << t : 0u;
+            const u16* kp = kb + (uint64_t)pg * (uint32_t)a.kv.k_page + (uint32_t)off * (uint32_t)a.kv.k_slot;
+            const u16* vp = vb + (uint64_t)pg * (uint32_t)a.kv.v_page + (uint32_t)off * (uint32_t)a.kv.v_slot;
+#pragma unroll
+            for (int i = 0; i < NC; ++i) kr[t][i] = *reinterpret_cast<const u32x4*>(kp + 32 * i);
+#pragma unroll
+            for (int i = 0; i < NC; ++i) vr[t][i] = *reinterpret_cast<const u32x4*>(vp + 32 * i);
+        }
+    };
+
+    f32x4 o[NDB];
+#pragma unroll
+    for (int d = 0; d < NDB; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m_run = -INFINITY, l_run = 0.f;
+    char* vs = smem + wave * VB;
+
+    int kt = c0 + wave * 32;
+    if (kt < c1) {
+        fetch_pid(kt);
+        fetch(kt);
+        fetch_pid(kt + NW * 32);
+    }
+    for (; kt < c1; kt += NW * 32) {
+        // the tile's values into LDS, its keys into the matrix unit; then its registers take the next tile
+        const bool part = kt + 31 > min_limit;  // some row does not see all of it (wave-uniform)
+        uint64_t nf[2] = {0, 0};
+        const uint64_t badk[2] = {__ballot(bad & 1), __ballot(bad & 2)};
+        if (part) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                bool any = false;
+#pragma unroll
+                for (int i = 0; i < NC; ++i) {
+                    if (kt + 16 * t + r >= s.len) vr[t][i] = u32x4{0, 0, 0, 0};
+                    any |= take_nonfinite<T>(vr[t][i]);
+                }
+                const uint64_t bl = __ballot(any);
+                nf[t] = (bl | (bl >> 16) | (bl >> 32) | (bl >> 48)) & 0xffff;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < NC; ++i) *reinterpret_cast<u32x4*>(vs + v_off<HD>(16 * t + r, 64 * i + 16 * g)) = vr[t][i];
+        f32x4 sc[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            sc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < NC; ++i) sc[t] = M16<T>::run(__builtin_bit_cast(frag, kr[t][i]), qf[i], sc[t]);
+        }
+        if (kt + NW * 32 < c1) {
+            fetch(kt + NW * 32);
+            fetch_pid(kt + 2 * NW * 32);
+        }
+        if (badk[0] | badk[1]) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if ((badk[t] >> (4 * g + j)) & 1) sc[t][j] = __builtin_nanf("");
+        }
+        if (part) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (kt + 16 * t + 4 * g + j > limit) sc[t][j] = -INFINITY;
+        }
+        float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])), fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = half_max(mx);
+        const float m_new = fmaxf(m_run, mx * a.scale_log2e);
+        const float m_use = m_new == -INFINITY ? 0.f : m_new;  // no key seen yet: every p is exp2(-inf) = 0
+        if (__any(m_new > m_run)) {
+            const float alpha = fast_exp2(m_run - m_use);
+            l_run *= alpha;
+#pragma unroll
+            for (int d = 0; d < NDB; ++d) o[d] *= alpha;
+        }
+        m_run = m_new;
+        float p[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                p[t][j] = fast_exp2(sc[t][j] * a.scale_log2e - m_use);
+                l_run += p[t][j];
+            }
+        const u32x4 pw = {pack2<T>(p[0][0], p[0][1]), pack2<T>(p[0][2], p[0][3]), pack2<T>(p[1][0], p[1][1]), pack2<T>(p[1][2], p[1][3])};
+        const frag pf = __builtin_bit_cast(frag, pw);
+        // V^T operand: lane (dim r of block d, group g) takes keys 4 g .. 4 g + 3 of both sub-tiles
+#pragma unroll
+        for (int d = 0; d < NDB; ++d) {
+            const int row = 4 * g + (r >> 2), byte = 32 * d + 8 * (r & 3);
+            const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vs + v_off<HD>(row, byte)));
+            const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vs + v_off<HD>(row + 16, byte)));
+            const s16x8 v = s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+            o[d] = M16<T>::run(__builtin_bit_cast(frag, v), pf, o[d]);
+        }
+        if (nf[0] | nf[1]) {
+            for (uint32_t left = (uint32_t)(nf[0] | (nf[1] << 16)); left; left &= left - 1) {
+                const int key = kt + __builtin_ctz(left);
+                const int pi = (int)fdiv((uint32_t)key, a.page), pg = bt[pi];
+                if ((uint32_t)pg >= (uint32_t)a.kv.num_pages || key > limit) continue;
+                const u16* vp = (const u16*)a.kv.v + (int64_t)pg * a.kv.v_page + (int64_t)kh * a.kv.v_head +
+                                (int64_t)(key - pi * (int)a.page.d) * a.kv.v_slot;
+#pragma unroll
+                for (int d = 0; d < NDB; ++d)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[d][j] += only_nonfinite<T>(vp + 16 * d + 4 * g + j);
+            }
+        }
+    }
+
+    // join the waves: rows' maxima and sums, then the weighted outputs
+    l_run += __shfl_xor(l_run, 16, 64);
+    l_run = half_sum(l_run);
+    __syncthreads();  // every wave has read its V tile
+    float* red = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int d = 0; d < NDB; ++d) *reinterpret_cast<f32x4*>(red + (wave * 16 + r) * RS + 16 * d + 4 * g) = o[d];
+    if (g == 0) {
+        sm_m[wave][r] = m_run;
+        sm_l[wave][r] = l_run;
+    }
+    __syncthreads();
+    for (int i = tid; i < R * (HD / 8); i += NW * 64) {
+        const int row = i / (HD / 8), d0 = (i % (HD / 8)) * 8;
+        float M = -INFINITY, L = 0.f, acc[8];
+#pragma unroll
+        for (int w = 0; w < NW; ++w) M = fmaxf(M, sm_m[w][row]);
+        const float mu = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const float m = sm_m[w][row];
+            if (m == -INFINITY && sm_l[w][row] == 0.f) continue;  // a wave without a key
+            const float al = fast_exp2(m - mu);
+            L += al * sm_l[w][row];
+            const float* src = red + (w * 16 + row) * RS + d0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] += al * src[e];
+        }
+        const int t = (int)fdiv((uint32_t)row, a.grp), h = kh * a.group + row - t * a.group, grow = s.beg + t;
+        if (a.nsplit == 1) {
+            const float inv = L == 0.f ? 0.f : 1.0f / L;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] *= inv;
+            *reinterpret_cast<u32x4*>(a.out + (int64_t)grow * a.o_row + (int64_t)h * a.o_head + d0) = pack8<T>(acc);
+            if (d0 == 0) a.lse[(int64_t)grow * a.l_row + h] = (M + __log2f(L)) * kLn2;
+        } else {
+            const int64_t at = ((int64_t)split * a.rows + grow) * a.nq + h;
+            f32x4* dst = reinterpret_cast<f32x4*>(a.ws_o + at * HD + d0);
+            dst[0] = f32x4{acc[0], acc[1], acc[2], acc[3]};
+            dst[1] = f32x4{acc[4], acc[5], acc[6], acc[7]};
+            if (d0 == 0) {
+                a.ws_ml[2 * at] = M;
+                a.ws_ml[2 * at + 1] = L;
+            }
+        }
+    }
+}
+
+// =====================================================================================  many rows
+// Bound by the matrix unit and the softmax's vector work, as the training forward (attention.hip), whose tile walk it shares: a
+// workgroup of 4 waves owns 128 rows, a wave 32 of them on the lane index of mfma 32x32x16 score tiles; keys and values come
+// in 64-key tiles, global -> registers -> double-buffered LDS, one barrier a tile; page ids are fetched a tile further ahead, so
+// that no load waits for another.  Row blocks with the most keys start first.
+template <typename T, int HD>
+__global__ __launch_bounds__(256, (HD == 64 ? 2 : 1)) void paged_attn_many_k(const PagedAttnArgs a) {
+    typedef Tile<HD> TL;
+    typedef typename M32<T>::frag frag;
+    constexpr int NDS = HD / 16, NDB = HD / 32, NCH = TL::NCH;
+    // per ring slot (tile & 3) two 64-bit key masks: pages the cache does not have, values taken out as non-finite.  Head size 128
+    // keeps them in the padding of the first LDS row (two workgroups fill a CU's LDS to the byte).
+    constexpr int FLAGS = HD == 128 ? 2 * HD : 4 * TL::BYTES;
+    __shared__ __attribute__((aligned(16))) char smem[4 * TL::BYTES + (HD == 128 ? 0 : 64)];  // [buf][K | V]
+    unsigned long long* flags = reinterpret_cast<unsigned long long*>(smem + FLAGS);  // [slot][page | value]
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 31, hh = lane >> 5;
+    const int nkv = a.kv.heads, seq = blockIdx.x / nkv, kh = blockIdx.x % nkv, split = blockIdx.z;
+    const int r0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * 128;
+    SeqInfo s;
+    if (!seq_info<HD>(a, seq, kh, blockIdx.y == 0 && split == 0, s)) return;
+    const int R = s.n * a.group;
+    if (r0 >= R) return;
+    const int c0 = split * a.chunk;
+    if (split > 0 && c0 >= s.len) return;  // the combining kernel knows
+
+    const int past = s.len - s.n;
+    const int row = r0 + wave * 32 + r, rc = row < R ? row : R - 1;
+    const int tok = (int)fdiv((uint32_t)rc, a.grp), qh = kh * a.group + rc - tok * a.group;
+    const int limit = past + tok;
+    const u16* qp = a.q + (int64_t)(s.beg + tok) * a.q_row + (int64_t)qh * a.q_head;
+    frag qf[NDS];
+#pragma unroll
+    for (int ds = 0; ds < NDS; ++ds) qf[ds] = *reinterpret_cast<const frag*>(qp + 16 * ds + 8 * hh);
+
+    const int wr0 = r0 + wave * 32;
+    const int blk_first = past + (int)fdiv((uint32_t)r0, a.grp);
+    const int blk_last = past + (int)fdiv((uint32_t)min(r0 + 127, R - 1), a.grp);
+    const int wave_first = past + (int)fdiv((uint32_t)min(wr0, R - 1), a.grp);
+    const int wave_last = wr0 < R ? past + (int)fdiv((uint32_t)min(wr0 + 31, R - 1), a.grp) : -1;
+    const int c1 = min(c0 + a.chunk, blk_last + 1);
+    const int ntiles = c1 > c0 ? (c1 - c0 + 63) >> 6 : 0;
+
+    const int32_t* bt = a.st.block_table + (int64_t)seq * a.st.table_stride;
+    const int trow = tid / TL::CPR, tch = tid % TL::CPR;  // this thread's first row and its 16-byte chunk of a tile
+    constexpr int RSTEP = 256 / TL::CPR;
+    const u16* kb = (const u16*)a.kv.k + (int64_t)kh * a.kv.k_head + tch * 8;
+    const u16* vb = (const u16*)a.kv.v + (int64_t)kh * a.kv.v_head + tch * 8;
+    u32x4 kreg[NCH], vreg[NCH];
+    int pid[NCH];
+    uint32_t bad = 0;
+    auto fetch_pid = [&](int kv0) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) pid[i] = bt[fdiv((uint32_t)min(kv0 + trow + RSTEP * i, s.len - 1), a.page)];
+    };
+    auto fetch = [&](int kv0) {
+        bad = 0;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const int key = min(kv0 + trow + RSTEP * i, s.len - 1);
+            const uint32_t off = (uint32_t)key - fdiv((uint32_t)key, a.page) * a.page.d;
+            const bool b = (uint32_t)pid[i] >= (uint32_t)a.kv.num_pages;
+            const uint32_t pg = b ? 0u : (uint32_t)pid[i];
+            bad |= b ? 1u << i : 0u;
+            kreg[i] = *reinterpret_cast<const u32x4*>(kb + (uint64_t)pg * (uint32_t)a.kv.k_page + off * (uint32_t)a.kv.k_slot);
+            vreg[i] = *reinterpret_cast<const u32x4*>(vb + (uint64_t)pg * (uint32_t)a.kv.v_page + off * (uint32_t)a.kv.v_slot);
+        }
+    };
+    // registers -> LDS stage of tile j; where some row of the block does not see the whole tile, the values behind the end become
+    // zero and the non-finite ones are taken out and noted
+    auto put = [&](char* ks, int j) {
+        const int kv0 = c0 + j * 64;
+        unsigned long long* fl = flags + 2 * (j & 3);
+        if (kv0 + 63 > blk_first) {
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) {
+                const int key = trow + RSTEP * i;
+                if (kv0 + key >= s.len) vreg[i] = u32x4{0, 0, 0, 0};
+                if (take_nonfinite<T>(vreg[i])) atomicOr(fl + 1, 1ull << key);
+            }
+        }
+        if (bad) {
+#pragma unroll
+            for (int i = 0; i < NCH; ++i)
+                if ((bad >> i) & 1) atomicOr(fl, 1ull << (trow + RSTEP * i));
+        }
+        tile_store<HD>(ks, kreg, tid);
+        tile_store<HD>(ks + TL::BYTES, vreg, tid);
+    };
+
+    f32x16 o[NDB];
+#pragma unroll
+    for (int i = 0; i < NDB; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
+    float m_run = -INFINITY, l_run = 0.f;
+
+    if (tid < 8) flags[tid] = 0;
+    __syncthreads();
+    if (ntiles > 0) {
+        fetch_pid(c0);
+        fetch(c0);
+        fetch_pid(c0 + 64);
+        put(smem, 0);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int ds = 0; ds < NDS; ++ds) pin(qf[ds]);
+
+    auto tile_step = [&](const int j, auto parity) {
+        constexpr int cur = decltype(parity)::value;
+        const char* ks = smem + cur * 2 * TL::BYTES;
+        const char* vs = ks + TL::BYTES;
+        const int kv0 = c0 + j * 64;
+        if (j + 1 < ntiles) {
+            fetch(kv0 + 64);
+            fetch_pid(kv0 + 128);
+        }
+        if (tid < 2) flags[2 * ((j + 2) & 3) + tid] = 0;  // read in tile j - 2, written for tile j + 2 behind this tile's barrier
+        const unsigned long long badk = flags[2 * (j & 3)], nonf = flags[2 * (j & 3) + 1];
+        if (kv0 <= wave_last) {
+            f32x16 sacc[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) sacc[t][i] = 0.f;
+#pragma unroll
+                for (int ds = 0; ds < NDS; ++ds) sacc[t] = M32<T>::run(row_frag<T, HD>(ks, 32 * t, ds, lane), qf[ds], sacc[t]);
+            }
+            if (badk) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if ((badk >> (32 * t + acc_row(i, hh))) & 1) sacc[t][i] = __builtin_nanf("");
+            }
+            if (kv0 + 63 > wave_first) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (kv0 + 32 * t + acc_row(i, hh) > limit) sacc[t][i] = -INFINITY;
+            }
+            float rmax = fmaxf(sacc[0][0], sacc[1][0]);
+#pragma unroll
+            for (int i = 1; i < 16; ++i) rmax = fmaxf(fmaxf(rmax, sacc[0][i]), sacc[1][i]);
+            rmax = half_max(rmax);
+            const float m_new = fmaxf(m_run, rmax * a.scale_log2e);
+            const float m_use = m_new == -INFINITY ? 0.f : m_new;  // no key seen yet
+            float lsum = 0.f;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    sacc[t][i] = fast_exp2(sacc[t][i] * a.scale_log2e - m_use);
+                    lsum += sacc[t][i];
+                }
+            if (__any(m_new > m_run)) {
+                const float alpha = fast_exp2(m_run - m_use);
+                l_run *= alpha;
+#pragma unroll
+                for (int d = 0; d < NDB; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+            }
+            l_run += lsum;
+            m_run = m_new;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int s2 = 0; s2 < 2; ++s2) {
+                    const frag pf = M32<T>::cvt8(sacc[t][8 * s2], sacc[t][8 * s2 + 1], sacc[t][8 * s2 + 2], sacc[t][8 * s2 + 3],
+                                                 sacc[t][8 * s2 + 4], sacc[t][8 * s2 + 5], sacc[t][8 * s2 + 6], sacc[t][8 * s2 + 7]);
+#pragma unroll
+                    for (int d = 0; d < NDB; ++d) o[d] = M32<T>::run(tr_frag<T, HD>(vs, 32 * t + 16 * s2, d, lane), pf, o[d]);
+                }
+            if (nonf) {
+                for (unsigned long long left = nonf; left; left &= left - 1) {
+                    const int key = kv0 + __builtin_ctzll(left);
+                    const int pi = (int)fdiv((uint32_t)key, a.page), pg = bt[pi];
+                    if ((uint32_t)pg >= (uint32_t)a.kv.num_pages || key > limit) continue;
+                    const u16* vp = (const u16*)a.kv.v + (int64_t)pg * a.kv.v_page + (int64_t)kh * a.kv.v_head +
+                                    (int64_t)(key - pi * (int)a.page.d) * a.kv.v_slot;
+#pragma unroll
+                    for (int d = 0; d < NDB; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[d][i] += only_nonfinite<T>(vp + 32 * d + acc_row(i, hh));
+                }
+            }
+        }
+        if (j + 1 < ntiles) put(smem + (cur ^ 1) * 2 * TL::BYTES, j + 1);
+        __syncthreads();
+    };
+    for (int j = 0; j < ntiles; j += 2) {
+        tile_step(j, std::integral_constant<int, 0>{});
+        if (j + 1 < ntiles) tile_step(j + 1, std::integral_constant<int, 1>{});
+    }
+
+    const float l_tot = half_sum(l_run);
+    if (row >= R) return;
+    const int grow = s.beg + tok;
+    if (a.nsplit == 1) {
+        const float inv = l_tot == 0.f ? 0.f : 1.0f / l_tot;
+        u16* orow = a.out + (int64_t)grow * a.o_row + (int64_t)qh * a.o_head;
+#pragma unroll
+        for (int d = 0; d < NDB; ++d)
+#pragma unroll
+            for (int g4 = 0; g4 < 4; ++g4)
+                *reinterpret_cast<u32x2*>(orow + 32 * d + 8 * g4 + 4 * hh) =
+                    u32x2{pack2<T>(o[d][4 * g4] * inv, o[d][4 * g4 + 1] * inv), pack2<T>(o[d][4 * g4 + 2] * inv, o[d][4 * g4 + 3] * inv)};
+        if (hh == 0) a.lse[(int64_t)grow * a.l_row + qh] = (m_run + __log2f(l_tot)) * kLn2;
+    } else {
+        const int64_t at = ((int64_t)split * a.rows + grow) * a.nq + qh;
+        float* orow = a.ws_o + at * HD;
+#pragma unroll
+        for (int d = 0; d < NDB; ++d)
+#pragma unroll
+            for (int g4 = 0; g4 < 4; ++g4)
+                *reinterpret_cast<f32x4*>(orow + 32 * d + 8 * g4 + 4 * hh) = f32x4{o[d][4 * g4], o[d][4 * g4 + 1], o[d][4 * g4 + 2], o[d][4 * g4 + 3]};
+        if (hh == 0) {
+            a.ws_ml[2 * at] = m_run;
+            a.ws_ml[2 * at + 1] = l_tot;
+        }
+    }
+}
+
+// =====================================================================================  joining the splits
+// out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s, always in split order.  One wave per row and head.
+template <typename T, int HD> __global__ __launch_bounds__(256) void paged_attn_join_k(const PagedAttnArgs a) {
+    constexpr int E = HD / 64;
+    const int lane = threadIdx.x & 63;
+    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (id >= (int64_t)a.rows * a.nq) return;
+    const int row = (int)(id / a.nq), h = (int)(id % a.nq);
+    const int seq = find_seq(a.st.cu_new, a.st.seqs, row, lane);
+    if (seq >= a.st.seqs) return;
+    const int beg = a.st.cu_new[seq], end = a.st.cu_new[seq + 1], len = a.st.kv_lens[seq];
+    // the rows the main kernel has handled itself (seq_info): nothing to join
+    if (beg > row || beg < 0 || end > a.rows || end - beg > a.st.max_new || len > a.st.max_kv || len > a.st.max_pages * (int)a.page.d) return;
+    const int ns = min(a.nsplit, max(1, (len + a.chunk - 1) / a.chunk));
+    const int64_t step = (int64_t)a.rows * a.nq;
+    float M = -INFINITY, L = 0.f, acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int i = lane; i < ns; i += 64) M = fmaxf(M, a.ws_ml[2 * (id + i * step)]);
+    M = wave_max(M);
+    const float mu = M == -INFINITY ? 0.f : M;
+    for (int i = 0; i < ns; ++i) {
+        const int64_t at = id + i * step;
+        const float m = a.ws_ml[2 * at], l = a.ws_ml[2 * at + 1];
+        if (m == -INFINITY && l == 0.f) continue;
+        const float al = fast_exp2(m - mu);
+        L += al * l;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += al * a.ws_o[at * HD + E * lane + e];
+    }
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+    u16* orow = a.out + (int64_t)row * a.o_row + (int64_t)h * a.o_head + E * lane;
+    if constexpr (E == 2) *reinterpret_cast<uint32_t*>(orow) = pack2<T>(acc[0] * inv, acc[1] * inv);
+    else *orow = from_f32<T>(acc[0] * inv);
+    if (lane == 0) a.lse[(int64_t)row * a.l_row + h] = (M + __log2f(L)) * kLn2;
+}
+
+// ---- launch plan, from the step's bounds alone (a captured step keeps it)
+struct PagedPlan {
+    bool few;
+    int chunk, nsplit, row_blocks;
+};
+constexpr int kFewRows = 16, kFewWaves = 4;
+static PagedPlan plan(const mm_paged_kv& kv, const mm_paged_step& st, int nq) {
+    PagedPlan p;
+    const int group = nq / kv.heads;
+    p.few = (int64_t)st.max_new * group <= kFewRows;
+    p.row_blocks = p.few ? 1 : (int)(((int64_t)st.max_new * group + 127) / 128);
+    // Split the keys while the launch has too few workgroups to fill 256 CUs: few-row workgroups are small (target 4 a CU), and no
+    // split is shorter than 4 tiles per wave; many-row ones take 2 a CU and at least 8 tiles.
+    const int64_t wgs = (int64_t)st.seqs * kv.heads * p.row_blocks;
+    const int target = p.few ? 1024 : 512, gran = p.few ? 32 * kFewWaves : 64, least = p.few ? 512 : 512;
+    int64_t ns = wgs > 0 ? target / wgs : 1;
+    const int64_t cap = (st.max_kv + least - 1) / least;
+    if (ns > cap) ns = cap;
+    if (ns < 1) ns = 1;
+    int64_t chunk = (st.max_kv + ns - 1) / ns;
+    chunk = (chunk + gran - 1) / gran * gran;
+    if (chunk < gran) chunk = gran;
+    p.chunk = (int)chunk;
+    p.nsplit = st.max_kv > 0 ? (int)((st.max_kv + chunk - 1) / chunk) : 1;
+    return p;
+}
+
+template <typename T, int HD> static int launch_paged_attn(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
+    const unsigned bx = (unsigned)(a.st.seqs * a.kv.heads);
+    if (p.few) paged_attn_few_k<T, HD, kFewWaves><<<dim3(bx, p.nsplit), kFewWaves * 64, 0, st>>>(a);
+    else paged_attn_many_k<T, HD><<<dim3(bx, p.row_blocks, p.nsplit), 256, 0, st>>>(a);
+    MM_CHECK_LAUNCH();
+    if (p.nsplit > 1) {
+        paged_attn_join_k<T, HD><<<(unsigned)(((int64_t)a.rows * a.nq + 3) / 4), 256, 0, st>>>(a);
+        MM_CHECK_LAUNCH();
+    }
+    return MM_OK;
+}
+
+static int check_paged_attn(const char* fn, const mm_paged_kv* kv, const mm_paged_step* st, int nq, int rows) {
+    if (int rc = check_paged(fn, kv, st, rows)) return rc;
+    MM_CHECK_ARG(nq > 0 && nq % kv->heads == 0 && nq < 1 << 20, "%s: %d query heads are no multiple of %d key heads", fn, nq, kv->heads);
+    MM_CHECK_ARG((int64_t)st->max_new * (nq / kv->heads) < (int64_t)1 << 30 && (int64_t)st->max_new * (nq / kv->heads) / 128 < 65535,
+                 "%s: max_new=%d rows of %d heads exceed the grid limit", fn, st->max_new, nq);
+    MM_CHECK_ARG((int64_t)st->seqs * kv->heads < (int64_t)1 << 31 && (int64_t)rows * nq < (int64_t)1 << 31,
+                 "%s: %d sequences, %d rows exceed the grid limit", fn, st->seqs, rows);
+    MM_CHECK_ARG(st->max_kv < 1 << 30, "%s: max_kv=%d exceeds 2^30", fn, st->max_kv);
+    return MM_OK;
+}
+
+}  // namespace mm
+
+using namespace mm;
+
+extern "C" size_t mm_paged_attn_workspace_bytes(const mm_paged_kv* kv, const mm_paged_step* step, int nq, int rows) {
+    if (check_paged_attn("mm_paged_attn_workspace_bytes", kv, step, nq, rows) != MM_OK) return 0;
+    const PagedPlan p = plan(*kv, *step, nq);
+    return p.nsplit == 1 ? 0 : (size_t)p.nsplit * rows * nq * (kv->hn + 2) * sizeof(float);
+}
+
+extern "C" int mm_paged_attn_fwd(const mm_paged_kv* kv, const mm_paged_step* step, void* out, int64_t o_row, int64_t o_head, float* lse,
+                                 int64_t l_row, const void* q, int64_t q_row, int64_t q_head, int nq, int rows, float softmax_scale,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+    const char* fn = "mm_paged_attn_fwd";
+    if (int rc = check_paged_attn(fn, kv, step, nq, rows)) return rc;
+    if (rows == 0 || step->seqs == 0 || step->max_new == 0) return MM_OK;
+    MM_CHECK_ARG(out && lse && q, "%s: null pointer", fn);
+    MM_CHECK_ARG(aligned16(q) && aligned16(out) && q_row % 8 == 0 && q_head % 8 == 0 && o_row % 8 == 0 && o_head % 8 == 0,
+                 "%s: q / out must be 16-byte aligned with strides a multiple of 8", fn);
+    MM_CHECK_ARG(softmax_scale > 0.f, "%s: softmax_scale %g must be positive", fn, (double)softmax_scale);
+    const PagedPlan p = plan(*kv, *step, nq);
+    const size_t need = p.nsplit == 1 ? 0 : (size_t)p.nsplit * rows * nq * (kv->hn + 2) * sizeof(float);
+    MM_CHECK_ARG(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need),
+                 "%s: workspace of %zu bytes needed (16-byte aligned), got %zu", fn, need, workspace ? workspace_bytes : (size_t)0);
+    PagedAttnArgs a{};
+    a.kv = *kv;
+    a.st = *step;
+    a.q = (const u16*)q, a.out = (u16*)out, a.lse = lse;
+    a.q_row = q_row, a.q_head = q_head, a.o_row = o_row, a.o_head = o_head, a.l_row = l_row;
+    a.nq = nq, a.group = nq / kv->heads, a.rows = rows;
+    a.scale_log2e = softmax_scale * kLog2e;
+    a.page = make_fastdiv(kv->page_size), a.grp = make_fastdiv(a.group);
+    a.chunk = p.chunk, a.nsplit = p.nsplit;
+    a.ws_o = (float*)workspace;
+    a.ws_ml = need ? a.ws_o + (size_t)p.nsplit * rows * nq * kv->hn : nullptr;
+    hipStream_t st = (hipStream_t)stream;
+    return dispatch_dtype(kv->dtype, [&](auto t) -> int {
+        using T = decltype(t);
+        return kv->hn == 64 ? launch_paged_attn<T, 64>(a, p, st) : launch_paged_attn<T, 128>(a, p, st);
+    });
+}

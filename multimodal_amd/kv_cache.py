@@ -1,0 +1,68 @@
+"""The paged key / value cache of text generation.
+
+The reference keeps `[past | new]` keys and values of every layer in tensors that grow by concatenation (use_cache /
+layer_past, megatron/model/transformer.py:361-365, 602-610).  Here a layer's keys and values live in pages of `page_size`
+token slots; sequences take pages as they grow and give them back when they end, so nothing is copied and sequences of any
+lengths share one batch.  `PagedKV` is one layer's pages, `PagedStep` what one step of a batch brings; `ops.paged_kv_append`
+and `ops.paged_attn_fwd` work on a pair of them.
+"""
+import ctypes
+
+import torch
+
+from ._lib import MmPagedKV, MmPagedStep, dtype_code
+
+
+class PagedKV:
+    """One layer's pages: k and v [num_pages, heads, page_size, hn] in fp16 / bf16, head size 64 or 128.  Any strides that are
+    multiples of 8 elements with the head dim contiguous, so both may be views of one tensor."""
+
+    def __init__(self, k, v):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or not k.is_cuda:
+            raise RuntimeError("PagedKV: k and v must be GPU tensors [num_pages, heads, page_size, hn] of one shape, dtype and device")
+        if k.size(3) not in (64, 128):
+            raise RuntimeError(f"PagedKV: head size {k.size(3)} not supported (64 or 128)")
+        if min(k.shape) < 1:
+            raise RuntimeError(f"PagedKV: empty cache {tuple(k.shape)}")
+        for t in (k, v):
+            if t.stride(3) != 1 or any(s % 8 or s < 0 for s in t.stride()[:3]) or t.data_ptr() % 16:
+                raise RuntimeError("PagedKV: pages must be 16-byte aligned with a contiguous head dim and strides that are multiples of 8")
+        self.k, self.v = k, v
+        self.num_pages, self.heads, self.page_size, self.hn = k.shape
+        self.dtype, self.device = k.dtype, k.device
+        self._c = MmPagedKV(k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], self.num_pages, self.page_size, self.heads,
+                            self.hn, dtype_code(k.dtype))
+        self._ref = ctypes.addressof(self._c)
+
+
+class PagedStep:
+    """What one step of a batch brings, shared by all layers.  block_table int32 [seqs, max_pages]: the pages of each sequence in
+    order; cu_new int32 [seqs + 1], ascending: sequence i brings the packed rows cu_new[i] .. cu_new[i + 1] - 1; kv_lens int32
+    [seqs]: its length including them.  max_new, max_kv: upper bounds of a sequence's new rows and length (defaults: read from
+    the arrays, which waits for the GPU).  The kernels read the arrays when they run, so their contents may be rewritten between
+    the replays of a captured step; a step that breaks the bounds, or names pages the cache does not have, gives NaN rows and
+    leaves the cache alone (include/mm_hip.h, mm_paged_step)."""
+
+    def __init__(self, block_table, cu_new, kv_lens, max_new=None, max_kv=None):
+        if block_table.dim() != 2 or cu_new.dim() != 1 or kv_lens.dim() != 1:
+            raise RuntimeError("PagedStep: block_table [seqs, max_pages], cu_new [seqs + 1] and kv_lens [seqs] expected")
+        for t in (block_table, cu_new, kv_lens):
+            if t.dtype != torch.int32 or not t.is_cuda or t.device != cu_new.device:
+                raise RuntimeError("PagedStep: block_table, cu_new and kv_lens must be int32 tensors on one GPU")
+        self.seqs = kv_lens.numel()
+        if cu_new.numel() != self.seqs + 1 or block_table.size(0) != self.seqs or block_table.size(1) < 1:
+            raise RuntimeError(f"PagedStep: block_table {tuple(block_table.shape)} and cu_new {tuple(cu_new.shape)} do not fit "
+                               f"{self.seqs} sequences")
+        if not (cu_new.is_contiguous() and kv_lens.is_contiguous()) or block_table.stride(1) != 1 or block_table.stride(0) < block_table.size(1):
+            raise RuntimeError("PagedStep: cu_new, kv_lens and the rows of block_table must be contiguous and the rows must not overlap")
+        if max_new is None:
+            max_new = int((cu_new[1:] - cu_new[:-1]).max()) if self.seqs else 0
+        if max_kv is None:
+            max_kv = int(kv_lens.max()) if self.seqs else 0
+        if max_new < 0 or max_kv < 0:
+            raise RuntimeError(f"PagedStep: max_new={max_new}, max_kv={max_kv} must not be negative")
+        self.block_table, self.cu_new, self.kv_lens = block_table, cu_new, kv_lens
+        self.max_new, self.max_kv, self.device = int(max_new), int(max_kv), cu_new.device
+        self._c = MmPagedStep(block_table.data_ptr(), cu_new.data_ptr(), kv_lens.data_ptr(), block_table.stride(0), self.seqs,
+                              block_table.size(1), self.max_new, self.max_kv)
+        self._ref = ctypes.addressof(self._c)

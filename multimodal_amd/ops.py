@@ -700,3 +700,99 @@ def embed_prefix(table, tokens, prefix=None):
     check(get_lib().mm_embed_prefix(out.data_ptr(), table.contiguous().data_ptr(), tokens.contiguous().data_ptr(), _ptr(prefix),
                                     s, b, h, P, V, _stream()), "embed_prefix")
     return out
+
+
+# ---------------------------------------------------------------------------- text generation: paged key / value cache
+def _launch(device, fn, *args):
+    """fn(*args, stream) with the current stream of `device`, which need not be the current device."""
+    if device.index == torch.cuda.current_device():
+        return fn(*args, torch.cuda.current_stream().cuda_stream)
+    with torch.cuda.device(device):
+        return fn(*args, torch.cuda.current_stream().cuda_stream)
+
+
+def _rows(name, t, kv, heads=None):
+    """A [rows, heads, hn] operand in the cache's dtype, on its device, with a contiguous head dim."""
+    if t.dim() != 3 or t.size(2) != kv.hn or (heads is not None and t.size(1) != heads) or t.dtype != kv.dtype or t.device != kv.device:
+        raise RuntimeError(f"{name} must be a [rows, {'heads' if heads is None else heads}, {kv.hn}] {kv.dtype} tensor on {kv.device}, "
+                           f"got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return t if t.stride(2) == 1 else t.contiguous()
+
+
+def _out_rows(name, t, like, dtype):
+    if t.shape != like or t.dtype != dtype or t.stride(-1) != 1:
+        raise RuntimeError(f"{name} must be a {tuple(like)} {dtype} tensor with a contiguous last dim, got {tuple(t.shape)} {t.dtype}")
+
+
+def paged_kv_append(kv, step, k, v, q=None, cos=None, sin=None, q_out=None):
+    """The step's key / value rows [rows, kv.heads, hn] into their slots of the cache; with cos / sin tables [positions, d] (fp32
+    or the cache's dtype) the first d dims of the keys, and of the queries q [rows, nq, hn] on their way to q_out, are rotated by
+    each row's position.  kv: kv_cache.PagedKV, step: kv_cache.PagedStep.  Returns q_out (allocated unless given; it may be q;
+    rows of no sequence are left as they were), or None without q.  k, v and q may be strided views, e.g. the slices of the
+    layer's fused [rows, heads, 3, hn] projection.  No backward: generation only."""
+    if kv.device != step.device:
+        raise RuntimeError(f"paged_kv_append: cache on {kv.device}, step on {step.device}")
+    k, v = _rows("paged_kv_append: k", k, kv, kv.heads), _rows("paged_kv_append: v", v, kv, kv.heads)
+    rows = k.size(0)
+    if v.size(0) != rows:
+        raise RuntimeError(f"paged_kv_append: {rows} key rows but {v.size(0)} value rows")
+    qa = (0, 0, 0, 0, 0, 0, 0)
+    if q is not None:
+        q = _rows("paged_kv_append: q", q, kv)
+        if q.size(0) != rows:
+            raise RuntimeError(f"paged_kv_append: {rows} key rows but {q.size(0)} query rows")
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        else:
+            _out_rows("paged_kv_append: q_out", q_out, q.shape, q.dtype)
+            if q_out.device != q.device:
+                raise RuntimeError(f"paged_kv_append: q_out on {q_out.device}, the cache on {q.device}")
+        qa = (q.data_ptr(), q.stride(0), q.stride(1), q_out.data_ptr(), q_out.stride(0), q_out.stride(1), q.size(1))
+    elif q_out is not None:
+        raise RuntimeError("paged_kv_append: q_out without q")
+    d = table_rows = fp32 = 0
+    cp = sp = 0
+    if cos is not None or sin is not None:
+        if cos is None or sin is None or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.device != kv.device or sin.device != kv.device:
+            raise RuntimeError("paged_kv_append: cos and sin must be two tables of one shape and dtype on the cache's device")
+        d = cos.size(-1)
+        if d % 2 or not 0 < d <= kv.hn or cos.numel() == 0 or cos.dtype not in (torch.float32, kv.dtype):
+            raise RuntimeError(f"paged_kv_append: tables {tuple(cos.shape)} {cos.dtype} must be [positions, d], d even and at most "
+                               f"{kv.hn}, in fp32 or {kv.dtype}")
+        cos, sin = cos.contiguous(), sin.contiguous()
+        cp, sp, table_rows, fp32 = cos.data_ptr(), sin.data_ptr(), cos.numel() // d, int(cos.dtype == torch.float32)
+    check(_launch(kv.device, get_lib().mm_paged_kv_append, kv._ref, step._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
+                  v.stride(0), v.stride(1), *qa, rows, cp, sp, d, table_rows, fp32), "paged_kv_append")
+    return q_out
+
+
+def paged_attn_fwd(kv, step, q, softmax_scale, out=None, lse=None):
+    """Attention of the step's new rows q [rows, nq, hn] over the cache (append their keys and values first): a row at position p
+    sees keys 0 .. p of its sequence, query head h reads key head h // (nq // kv.heads).  Returns (out [rows, nq, hn], lse [rows,
+    nq] fp32), allocated unless given; rows of no sequence are left as they were, a row that sees no key gets 0 and -inf.  No
+    backward: generation only."""
+    if kv.device != step.device:
+        raise RuntimeError(f"paged_attn_fwd: cache on {kv.device}, step on {step.device}")
+    q = _rows("paged_attn_fwd: q", q, kv)
+    if q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
+        q = q.contiguous() if not q.is_contiguous() else q.clone()
+    rows, nq, _ = q.shape
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    else:
+        _out_rows("paged_attn_fwd: out", out, q.shape, q.dtype)
+        if out.device != q.device or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16:
+            raise RuntimeError("paged_attn_fwd: out must be 16-byte aligned with strides a multiple of 8, on the cache's device")
+    if lse is None:
+        lse = torch.empty(rows, nq, dtype=torch.float32, device=q.device)
+    else:
+        _out_rows("paged_attn_fwd: lse", lse, q.shape[:2], torch.float32)
+        if lse.device != q.device:
+            raise RuntimeError(f"paged_attn_fwd: lse on {lse.device}, the cache on {q.device}")
+    lib = get_lib()
+    ws_bytes = lib.mm_paged_attn_workspace_bytes(kv._ref, step._ref, nq, rows)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
+    check(_launch(q.device, lib.mm_paged_attn_fwd, kv._ref, step._ref, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(),
+                  lse.stride(0), q.data_ptr(), q.stride(0), q.stride(1), nq, rows, float(softmax_scale), _ptr(ws), ws_bytes),
+          "paged_attn_fwd")
+    return out, lse
