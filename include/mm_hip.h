@@ -414,6 +414,19 @@ int mm_paged_attn_fwd(const mm_paged_kv* kv, const mm_paged_step* step, void* ou
                       int64_t l_row, const void* q, int64_t q_row, int64_t q_head, int nq, int rows, float softmax_scale,
                       void* workspace, size_t workspace_bytes, void* stream);
 
+/* The next token of each row of logits [rows, vocab] (16-bit, row stride in elements, any alignment) from a given random number
+ * u[row] in [0, 1) (filter_logits and the multinomial draw behind it, megatron/text_generation_utils.py).  The tokens of a row are
+ * ordered by descending logit, ties by ascending index, and weigh w = exp((logit - max) / temperature):
+ *   top_k > 0 keeps the first top_k; 0 < top_p < 1 keeps a token while the weight ahead of it is at most top_p times the weight of
+ *   what top_k kept; min_p > 0 keeps w >= min_p; the first token always stays; other values of the three switch them off;
+ *   tokens[row] = the first token in that order whose running weight exceeds u times the kept weight (u >= 1: the last one kept).
+ * temperature <= 0 takes the first token (the lowest index of the largest logit).  -inf is never drawn, +inf always wins; a row
+ * with a NaN, or of nothing but -inf, gives -1.  Each parameter is the scalar, or per row where its array is not NULL.  Weights and
+ * their sums are in 64 bits and the order of summation is fixed. */
+int mm_sample_tokens(int64_t* tokens, const void* logits, int64_t row_stride, const float* u, int rows, int vocab, float temperature,
+                     const float* temperature_rows, int top_k, const int32_t* top_k_rows, float top_p, const float* top_p_rows,
+                     float min_p, const float* min_p_rows, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -95,6 +95,8 @@ PROTOTYPES = {
     "mm_paged_attn_workspace_bytes": (c_size_t, [c_void_p] * 2 + [c_int] * 2),
     "mm_paged_attn_fwd": (c_int, [c_void_p] * 2 + [c_void_p, c_i64, c_i64, c_void_p, c_i64, c_void_p, c_i64, c_i64, c_int, c_int, c_float,
                                                    c_void_p, c_size_t, c_void_p]),
+    "mm_sample_tokens": (c_int, [c_void_p, c_void_p, c_i64, c_void_p, c_int, c_int, c_float, c_void_p, c_int, c_void_p, c_float, c_void_p,
+                                 c_float, c_void_p, c_int, c_void_p]),
     "mm_adam_chunk_elems": (c_int, []),
     "mm_adam_step": (c_int, [c_void_p] * 6 + [c_int, c_void_p, c_void_p, c_void_p, c_float, c_void_p] + [c_float] * 5 + [c_int, c_int, c_void_p]),
 }

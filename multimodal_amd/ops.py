@@ -796,3 +796,44 @@ def paged_attn_fwd(kv, step, q, softmax_scale, out=None, lse=None):
                   lse.stride(0), q.data_ptr(), q.stride(0), q.stride(1), nq, rows, float(softmax_scale), _ptr(ws), ws_bytes),
           "paged_attn_fwd")
     return out, lse
+
+
+# ---------------------------------------------------------------------------- text generation: the next token
+def _per_row(name, v, dtype, rows, device, lo, hi):
+    """A sampling parameter: (scalar, pointer).  A number, checked; or a [rows] tensor, read on the device."""
+    if isinstance(v, torch.Tensor):
+        if v.dtype != dtype or v.shape != (rows,) or v.device != device:
+            raise RuntimeError(f"sample_tokens: {name} must be a number or a [{rows}] {dtype} tensor on {device}, got {tuple(v.shape)} "
+                               f"{v.dtype} on {v.device}")
+        v = v.contiguous()
+        return 0, v.data_ptr(), v
+    if not lo <= v <= hi:
+        raise RuntimeError(f"sample_tokens: {name}={v} must be in [{lo}, {hi}]")
+    return v, 0, None
+
+
+def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=0.0, min_p=0.0, out=None):
+    """The next token of each row: logits [rows, vocab] fp16 / bf16 (rows may be strided: the unpadded part of a padded vocabulary),
+    u [rows] fp32 random numbers in [0, 1).  temperature 0: the largest logit; top_k 0, top_p 0 or 1, min_p 0: off (the
+    reference's defaults).  Each parameter is a number or a [rows] tensor (fp32; top_k int32).  Returns int64 [rows] (`out` if
+    given); -1 for a row with a NaN or of nothing but -inf.  The order, ties and borders are defined in include/mm_hip.h."""
+    if logits.dim() != 2 or not logits.is_cuda or logits.size(1) < 1:
+        raise RuntimeError(f"sample_tokens: logits must be a GPU tensor [rows, vocab], got {tuple(logits.shape)} on {logits.device}")
+    rows, vocab = logits.shape
+    dev = logits.device
+    if logits.stride(1) != 1 and vocab > 1:
+        logits = logits.contiguous()
+    if u.shape != (rows,) or u.dtype != torch.float32 or u.device != dev:
+        raise RuntimeError(f"sample_tokens: u must be a [{rows}] fp32 tensor on {dev}, got {tuple(u.shape)} {u.dtype} on {u.device}")
+    u = u.contiguous()
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int64, device=dev)
+    elif out.shape != (rows,) or out.dtype != torch.int64 or out.device != dev or not out.is_contiguous():
+        raise RuntimeError(f"sample_tokens: out must be a contiguous [{rows}] int64 tensor on {dev}")
+    t, tv, t_ = _per_row("temperature", temperature, torch.float32, rows, dev, 0.0, float("inf"))
+    k, kv, k_ = _per_row("top_k", top_k, torch.int32, rows, dev, 0, 2 ** 31 - 1)
+    p, pv, p_ = _per_row("top_p", top_p, torch.float32, rows, dev, 0.0, 1.0)
+    m, mv, m_ = _per_row("min_p", min_p, torch.float32, rows, dev, 0.0, 1.0)
+    check(_launch(dev, get_lib().mm_sample_tokens, out.data_ptr(), logits.data_ptr(), logits.stride(0), u.data_ptr(), rows, vocab, t, tv,
+                  k, kv, p, pv, m, mv, dtype_code(logits.dtype)), "sample_tokens")
+    return out
