@@ -9,12 +9,14 @@
 // the j-th by index of one value.  Sums run in a fixed order: the result does not depend on scheduling, and a border of two tokens
 // is off by about 1e-15 of the weight.
 //
-// One workgroup of 16 waves per row.  Its histogram (32768 words: a count of a non-negative value in the low half, of a negative
-// one in the high half; 128 KB) fills most of a CU's LDS.  Steps: (1) the row into registers, each wave a contiguous 16th of it
-// (the search by index needs that), and its largest value; (2) one LDS atomic per logit; (3) per 64 neighbouring values ("chunk")
-// count and weight, one wave a chunk, empty chunks and weights below e^-50 skipped; (4) a scan over the 1024 chunks; (5) one wave
-// finds the borders: 64-way search for the chunk, a scan over its 64 values; (6) the j-th match of the value found.
-// Rows of more than 65535 logits (BIG) could overflow 16-bit counts: they count non-negative and negative values one after the
+// One workgroup of 16 waves per row.  Its histogram (a count of a non-negative value in the low half of a word, of a negative one
+// in the high half; 130 KB) fills most of a CU's LDS.  Steps: (1) the row into registers, each wave a contiguous 16th of it (the
+// search by index needs that), and its largest value; (2) one LDS atomic per logit; (3) count and weight of every 64 neighbouring
+// values ("chunk"), one thread a chunk: the values of a chunk share their exponent and are evenly spaced, so their weights are a
+// geometric sequence and the chunk's weight is a polynomial, sum n_i r^i, by Horner's rule - two exponentials a chunk instead of one
+// a value.  A chunk takes 65 words of LDS, so that 64 lanes walking 64 chunks in step meet 64 banks; (4) a scan over the 1024 chunks;
+// (5) one wave finds the borders: 64-way search for the chunk, a scan over its 64 values; (6) the j-th match of the value found.
+// Rows of more than 65528 logits (BIG) could overflow 16-bit counts: they count non-negative and negative values one after the
 // other in 32 bits, re-read the row instead of keeping it, and recount a chunk when a border falls into it.
 #include "common.h"
 
@@ -57,49 +59,85 @@ template <typename T> struct Weights {
     }
 };
 
-__device__ __forceinline__ double shfl_up_d(double v, int o) {
+// Inclusive scans over a wave by DPP (row shifts inside 16 lanes, then the row broadcasts): no LDS round trips.
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp_u(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ double dpp_d(double v) {
     const unsigned long long b = __double_as_longlong(v);
-    const uint32_t lo = __shfl_up((uint32_t)b, o, 64), hi = __shfl_up((uint32_t)(b >> 32), o, 64);
+    const uint32_t lo = dpp_u<CTRL, ROWS>((uint32_t)b), hi = dpp_u<CTRL, ROWS>((uint32_t)(b >> 32));
     return __longlong_as_double(((unsigned long long)hi << 32) | lo);
 }
-__device__ __forceinline__ double shfl_d(double v, int l) {
+__device__ __forceinline__ uint32_t scan_u(uint32_t v) {
+    v += dpp_u<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+    v += dpp_u<0x112, 0xf>(v);
+    v += dpp_u<0x114, 0xf>(v);
+    v += dpp_u<0x118, 0xf>(v);
+    v += dpp_u<0x142, 0xa>(v);  // row_bcast 15 into rows 1 and 3, row_bcast 31 into rows 2 and 3
+    v += dpp_u<0x143, 0xc>(v);
+    return v;
+}
+__device__ __forceinline__ double scan_d(double v) {
+    v += dpp_d<0x111, 0xf>(v);
+    v += dpp_d<0x112, 0xf>(v);
+    v += dpp_d<0x114, 0xf>(v);
+    v += dpp_d<0x118, 0xf>(v);
+    v += dpp_d<0x142, 0xa>(v);
+    v += dpp_d<0x143, 0xc>(v);
+    return v;
+}
+// minimum over a wave of two 16-bit numbers at once, in the last lane; row_min over each 16 lanes, in the last lane of the row
+typedef __attribute__((ext_vector_type(2))) unsigned short us2;
+__device__ __forceinline__ us2 pk_min(us2 a, us2 b) { return __builtin_elementwise_min(a, b); }
+template <int CTRL, int ROWS> __device__ __forceinline__ us2 dpp_min(us2 v) {
+    const int o = __builtin_amdgcn_update_dpp(-1, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false);
+    return pk_min(v, __builtin_bit_cast(us2, o));
+}
+__device__ __forceinline__ us2 row_min(us2 v) {
+    v = dpp_min<0x111, 0xf>(v);
+    v = dpp_min<0x112, 0xf>(v);
+    v = dpp_min<0x114, 0xf>(v);
+    return dpp_min<0x118, 0xf>(v);
+}
+__device__ __forceinline__ us2 wave_min2(us2 v) { return dpp_min<0x143, 0xc>(dpp_min<0x142, 0xa>(row_min(v))); }
+__device__ __forceinline__ uint32_t row_sum_u(uint32_t v) {
+    v += dpp_u<0x111, 0xf>(v);
+    v += dpp_u<0x112, 0xf>(v);
+    v += dpp_u<0x114, 0xf>(v);
+    return v + dpp_u<0x118, 0xf>(v);
+}
+__device__ __forceinline__ double row_sum_d(double v) {
+    v += dpp_d<0x111, 0xf>(v);
+    v += dpp_d<0x112, 0xf>(v);
+    v += dpp_d<0x114, 0xf>(v);
+    return v + dpp_d<0x118, 0xf>(v);
+}
+__device__ __forceinline__ double lane_d(double v, int l) {
     const unsigned long long b = __double_as_longlong(v);
-    const uint32_t lo = __shfl((uint32_t)b, l, 64), hi = __shfl((uint32_t)(b >> 32), l, 64);
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)b, l), hi = __builtin_amdgcn_readlane((uint32_t)(b >> 32), l);
     return __longlong_as_double(((unsigned long long)hi << 32) | lo);
 }
-__device__ __forceinline__ uint32_t scan_u(uint32_t v, int lane) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t x = __shfl_up(v, o, 64);
-        if (lane >= o) v += x;
-    }
-    return v;
-}
-__device__ __forceinline__ double scan_d(double v, int lane) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double x = shfl_up_d(v, o);
-        if (lane >= o) v += x;
-    }
-    return v;
-}
+__device__ __forceinline__ uint32_t lane_u(uint32_t v, int l) { return __builtin_amdgcn_readlane(v, l); }
 
 struct SampleShared {
-    uint32_t hist[32768];
+    uint32_t hist[512 * 65];  // value dk: word hist_word(dk), low half below 0x8000
     double mass[kChunks];    // then its inclusive scan
     uint32_t count[kChunks];
     double wave_mass[kSampleWaves];
     uint32_t wave_count[kSampleWaves];
-    int wave_min[kSampleWaves], wave_max[kSampleWaves];
+    us2 wave_ends[kSampleWaves];
     int dk, j;
     uint32_t one_chunk[64];  // BIG
 };
 
+__device__ __forceinline__ int hist_word(int dk) { return (dk & 0x7fff) + ((dk >> 6) & 511); }
+
 template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) void sample_tokens_k(const SampleArgs a) {
     __shared__ __attribute__((aligned(16))) SampleShared sm;
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, row = blockIdx.x;
-    // The row as 16-byte aligned chunks: `lead` elements of the first one and the end of the last belong to no token.  (An aligned
-    // chunk that holds one element of the row lies in the allocation's own 16-byte granule.)
+    constexpr uint32_t kNone = (uint32_t)minus_inf<T>() * 0x10001u;  // two -inf, in the order
+    // The row as 16-byte aligned chunks: `lead` elements of the first one and the end of the last belong to no token and become
+    // -inf.  (An aligned chunk that holds one element of the row lies in the allocation's own 16-byte granule.)
     const u16* rp = a.logits + (int64_t)row * a.row_stride;
     const int lead = (int)(((uintptr_t)rp & 15) >> 1);
     const u32x4* base = reinterpret_cast<const u32x4*>(rp - lead);
@@ -108,61 +146,74 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
     const int ch0 = wave * seg, ch1 = min(ch0 + seg, nch);
     const int steps = (seg + 63) >> 6;
 
+    auto ordered = [&](u32x4 v, int ch) -> u32x4 {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = order2(v[i]);
+        if (ch == 0 || ch == nch - 1) {
+            const int e0 = ch * 8 - lead;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (e0 + 2 * i < 0 || e0 + 2 * i >= a.vocab) v[i] = (v[i] & 0xffff0000u) | (kNone & 0xffffu);
+                if (e0 + 2 * i + 1 < 0 || e0 + 2 * i + 1 >= a.vocab) v[i] = (v[i] & 0xffffu) | (kNone & 0xffff0000u);
+            }
+        }
+        return v;
+    };
     u32x4 reg[BIG ? 1 : kSampleSteps];
     if constexpr (!BIG) {
 #pragma unroll
-        for (int s = 0; s < kSampleSteps; ++s)
+        for (int s = 0; s < kSampleSteps; ++s) {
+            reg[s] = u32x4{kNone, kNone, kNone, kNone};
             if (s < steps && ch0 + 64 * s + lane < ch1) reg[s] = base[ch0 + 64 * s + lane];
-    }
-    // f(place in the order, element index) for this thread's elements in ascending index
-    auto each = [&](auto&& f) {
-        auto chunk = [&](u32x4 v, int ch) {
-            const int e0 = ch * 8 - lead;
-            const bool whole = e0 >= 0 && e0 + 8 <= a.vocab;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t o = order2(v[i]);
-                if (whole || (e0 + 2 * i >= 0 && e0 + 2 * i < a.vocab)) f((int)(o & 0xffffu), e0 + 2 * i);
-                if (whole || (e0 + 2 * i + 1 >= 0 && e0 + 2 * i + 1 < a.vocab)) f((int)(o >> 16), e0 + 2 * i + 1);
-            }
-        };
-        if constexpr (BIG) {
-            for (int ch = ch0 + lane; ch < ch1; ch += 64) chunk(base[ch], ch);
-        } else {
-#pragma unroll
-            for (int s = 0; s < kSampleSteps; ++s)
-                if (s < steps && ch0 + 64 * s + lane < ch1) chunk(reg[s], ch0 + 64 * s + lane);
         }
-    };
-
+    }
+    const float u = a.u[row];
     const float temp = a.temperature_v ? a.temperature_v[row] : a.temperature;
+    const float p = a.top_p_v ? a.top_p_v[row] : a.top_p, mp = a.min_p_v ? a.min_p_v[row] : a.min_p;
+    const int k = a.top_k_v ? a.top_k_v[row] : a.top_k;
     const bool greedy = !(temp > 0.f);
     auto clear_hist = [&]() {
         u32x4* h = reinterpret_cast<u32x4*>(sm.hist);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) h[tid + kSampleThreads * i] = u32x4{0, 0, 0, 0};
+        for (int i = tid; i < 512 * 65 / 4; i += kSampleThreads) h[i] = u32x4{0, 0, 0, 0};
     };
     if (!greedy) clear_hist();
-    int lo = 0xffff, hi = 0;
-    each([&](int dk, int) {
-        lo = min(lo, dk);
-        hi = max(hi, dk);
-    });
+    if constexpr (!BIG) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        lo = min(lo, __shfl_xor(lo, o, 64));
-        hi = max(hi, __shfl_xor(hi, o, 64));
+        for (int s = 0; s < kSampleSteps; ++s)
+            if (s < steps && ch0 + 64 * s + lane < ch1) reg[s] = ordered(reg[s], ch0 + 64 * s + lane);
     }
-    if (lane == 0) {
-        sm.wave_min[wave] = lo;
-        sm.wave_max[wave] = hi;
+    // f(two places in the order) over this thread's logits
+    auto each2 = [&](auto&& f) {
+        if constexpr (BIG) {
+            for (int ch = ch0 + lane; ch < ch1; ch += 64) {
+                const u32x4 v = ordered(base[ch], ch);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f(v[i]);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < kSampleSteps; ++s)
+                if (s < steps && ch0 + 64 * s + lane < ch1) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) f(reg[s][i]);
+                }
+        }
+    };
+
+    us2 lo2 = {0xffff, 0xffff}, hi2 = {0xffff, 0xffff};  // smallest place; complement of the largest
+    each2([&](uint32_t o) {
+        lo2 = pk_min(lo2, __builtin_bit_cast(us2, o));
+        hi2 = pk_min(hi2, __builtin_bit_cast(us2, ~o));
+    });
+    const us2 mine2 = pk_min(us2{lo2[0], hi2[0]}, us2{lo2[1], hi2[1]});  // {smallest, complement of the largest} of this thread
+    {
+        const us2 w2 = wave_min2(mine2);
+        if (lane == 63) sm.wave_ends[wave] = w2;
     }
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kSampleWaves; ++w) {
-        lo = min(lo, sm.wave_min[w]);
-        hi = max(hi, sm.wave_max[w]);
-    }
+    const us2 ends = __builtin_bit_cast(us2, lane_u(__builtin_bit_cast(uint32_t, row_min(sm.wave_ends[lane & 15])), 15));
+    int lo = ends[0];
+    const int hi = 0xffff - ends[1];
     if (lo < plus_inf<T>() || hi > minus_inf<T>() || lo >= minus_inf<T>()) {  // a NaN, or nothing but -inf: no token
         if (tid == 0) a.out[row] = -1;
         return;
@@ -179,39 +230,79 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
             const u16 b = from_f32<T>(xlow);
             dlow = min(dlow, ((b & 0x8000) ? (int)b : 0x7fff - (int)b) + 1);
         }
-        const int clo = lo >> 6, chi = dlow >> 6;
+        const int clo = lo >> 6;
         sm.count[tid] = 0;
         sm.mass[tid] = 0.0;
-        auto chunk_sums = [&](int first, int last, auto&& counts) {  // chunks first .. last: one wave each
-            for (int c = first + wave; c <= last; c += kSampleWaves) {
-                const uint32_t n = counts(c);
-                if (__ballot(n != 0) == 0) continue;
-                uint32_t cn = n;
-                double m = n ? (double)n * wt.at(64 * c + lane) : 0.0;
-#pragma unroll
-                for (int o = 32; o > 0; o >>= 1) {
-                    cn += __shfl_xor(cn, o, 64);
-                    const unsigned long long b = __double_as_longlong(m);
-                    const uint32_t l = __shfl_xor((uint32_t)b, o, 64), h = __shfl_xor((uint32_t)(b >> 32), o, 64);
-                    m += __longlong_as_double(((unsigned long long)h << 32) | l);
+        if (!BIG && k > 0 && k <= kSampleThreads / 2) {
+            // The k-th largest of the threads' largest logits bounds the k-th largest logit from below: what lies in a later chunk
+            // is not among the first k, and stays out of the histogram (50304 logits, k = 64: 0.3 % of them come in)
+            __syncthreads();
+            atomicAdd(&sm.count[mine2[0] >> 6], 1u);
+            __syncthreads();
+            const uint32_t n = sm.count[tid], c = scan_u(n);
+            if (lane == 63) sm.wave_count[wave] = c;
+            __syncthreads();
+            const uint32_t w = sm.wave_count[lane & 15];
+            const uint32_t upto = c + lane_u(row_sum_u((lane & 15) < wave ? w : 0u), 15);
+            if (upto >= (uint32_t)k && upto - n < (uint32_t)k) sm.dk = 64 * tid + 63;  // one thread
+            __syncthreads();
+            dlow = min(dlow, __builtin_amdgcn_readfirstlane(sm.dk));
+            sm.count[tid] = 0;
+        }
+        const int chi = dlow >> 6;
+        // count and weight of chunk tid, chunks first .. last being in the histogram (BIG: half a histogram of whole words)
+        auto chunk_sums = [&](int first, int last) {
+            if (64 * wave + 63 < first || 64 * wave > last) return;  // none of this wave's chunks
+            const uint32_t* h = sm.hist + (tid & 511) * 65;
+            const int sh = BIG || tid < 512 ? 0 : 16;
+            const uint32_t mask = BIG ? 0xffffffffu : 0xffffu;
+            // the chunk's values are x0 - i ulp; weights e^((x0 - max) / T) r^i with r = e^(-ulp / T).  The largest value's own chunk
+            // counts from that value, so that no power exceeds 1
+            const bool top = tid == clo;
+            const int i0 = top ? lo & 63 : 0, d0 = 64 * tid + i0;
+            const int bits = d0 < 0x8000 ? 0x7fff - d0 : d0 & 0x7fff;  // magnitude of x0
+            const double x0 = (double)order_value<T>(d0);
+            const int e = max(bits >> (inf_bits<T>() == 0x7f80 ? 7 : 10), 1) - (inf_bits<T>() == 0x7f80 ? 127 + 7 : 15 + 10);
+            const double r = exp(fmax(-ldexp(1.0, e) * wt.inv_t, -800.0));
+            const bool none = x0 == -(double)INFINITY || (wt.xmax == (double)INFINITY && !top);
+            const double first_w = top ? 1.0 : none ? 0.0 : exp(fmax((x0 - wt.xmax) * wt.inv_t, -800.0));
+            double acc = 0.0;
+            uint32_t n = 0;
+            if (clo >> 6 == wave) {  // the wave of the top chunk
+#pragma unroll 16
+                for (int i = 63; i >= 0; --i) {
+                    const uint32_t c = (h[i] >> sh) & mask;
+                    n += c;
+                    acc = i >= i0 ? fma(acc, r, (double)c) : acc;
                 }
-                if (lane == 0) {
-                    sm.count[c] = cn;
-                    sm.mass[c] = m;
+            } else {
+#pragma unroll 16
+                for (int i = 63; i >= 0; --i) {
+                    const uint32_t c = (h[i] >> sh) & mask;
+                    n += c;
+                    acc = fma(acc, r, (double)c);
                 }
+            }
+            if (tid >= first && tid <= last) {
+                sm.count[tid] = n;
+                sm.mass[tid] = acc * first_w;
             }
         };
-        auto resident = [&](int c) -> uint32_t { return (sm.hist[((c & 511) << 6) + lane] >> (c < 512 ? 0 : 16)) & 0xffffu; };
         if constexpr (!BIG) {
-            each([&](int d, int) { atomicAdd(&sm.hist[d & 0x7fff], d < 0x8000 ? 1u : 0x10000u); });
+            const uint32_t last = 64u * chi + 63u;
+            each2([&](uint32_t o) {
+                const uint32_t d0 = o & 0xffffu, d1 = o >> 16;
+                if (d0 <= last) atomicAdd(&sm.hist[hist_word(d0)], d0 < 0x8000 ? 1u : 0x10000u);
+                if (d1 <= last) atomicAdd(&sm.hist[hist_word(d1)], d1 < 0x8000 ? 1u : 0x10000u);
+            });
             __syncthreads();
-            if (tid == 0) {  // -0 is +0: word 0x7fff low half takes word 0 high half
-                const uint32_t z = sm.hist[0] >> 16;
-                sm.hist[0] &= 0xffffu;
-                sm.hist[kPlusZero] += z;
+            if (tid == 0) {  // -0 is +0
+                const uint32_t z = sm.hist[hist_word(kMinusZero)] >> 16;
+                sm.hist[hist_word(kMinusZero)] &= 0xffffu;
+                sm.hist[hist_word(kPlusZero)] += z;
             }
             __syncthreads();
-            chunk_sums(clo, chi, resident);
+            chunk_sums(clo, chi);
         } else {
             for (int half = 0; half < 2; ++half) {
                 if (half == 1) {
@@ -219,44 +310,47 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
                     clear_hist();
                     __syncthreads();
                 }
-                each([&](int d, int) {
+                auto one = [&](int d) {
                     if (d == kMinusZero) d = kPlusZero;
-                    if ((d >> 15) == half) atomicAdd(&sm.hist[d & 0x7fff], 1u);
+                    if ((d >> 15) == half) atomicAdd(&sm.hist[hist_word(d)], 1u);
+                };
+                each2([&](uint32_t o) {
+                    one((int)(o & 0xffffu));
+                    one((int)(o >> 16));
                 });
                 __syncthreads();
-                chunk_sums(max(clo, 512 * half), min(chi, 512 * half + 511), [&](int c) -> uint32_t { return sm.hist[((c & 511) << 6) + lane]; });
+                chunk_sums(max(clo, 512 * half), min(chi, 512 * half + 511));
             }
         }
         __syncthreads();
         {   // inclusive scans over the chunks
-            uint32_t c = scan_u(sm.count[tid], lane);
-            double m = scan_d(sm.mass[tid], lane);
+            const uint32_t c = scan_u(sm.count[tid]);
+            const double m = scan_d(sm.mass[tid]);
             if (lane == 63) {
                 sm.wave_count[wave] = c;
                 sm.wave_mass[wave] = m;
             }
             __syncthreads();
-            double bm = 0.0;
-            uint32_t bc = 0;
-            for (int w = 0; w < wave; ++w) {
-                bc += sm.wave_count[w];
-                bm += sm.wave_mass[w];
-            }
-            sm.count[tid] = c + bc;
-            sm.mass[tid] = m + bm;
+            const bool ahead = (lane & 15) < wave;
+            sm.count[tid] = c + lane_u(row_sum_u(ahead ? sm.wave_count[lane & 15] : 0u), 15);
+            sm.mass[tid] = m + lane_d(row_sum_d(ahead ? sm.wave_mass[lane & 15] : 0.0), 15);
             __syncthreads();
         }
 
         // Borders.  One wave (BIG: every wave alike, because recounting a chunk takes the whole workgroup).
         if (BIG || wave == 0) {
             auto counts = [&](int c) -> uint32_t {
-                if constexpr (!BIG) return resident(c);
+                if constexpr (!BIG) return (sm.hist[(c & 511) * 65 + lane] >> (c < 512 ? 0 : 16)) & 0xffffu;
                 __syncthreads();
                 if (tid < 64) sm.one_chunk[tid] = 0;
                 __syncthreads();
-                each([&](int d, int) {
+                auto one = [&](int d) {
                     if (d == kMinusZero) d = kPlusZero;
                     if ((d >> 6) == c) atomicAdd(&sm.one_chunk[d & 63], 1u);
+                };
+                each2([&](uint32_t o) {
+                    one((int)(o & 0xffffu));
+                    one((int)(o >> 16));
                 });
                 __syncthreads();
                 return sm.one_chunk[lane];
@@ -264,7 +358,7 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
             auto first_chunk = [&](auto&& pred) -> int {  // the first chunk with pred(inclusive scan); pred holds from there on
                 uint64_t b = __ballot(pred(16 * lane + 15));
                 const int blk = b ? __builtin_ctzll(b) : 63;
-                b = __ballot(lane < 16 && pred(16 * blk + lane));
+                b = __ballot(lane < 16 && pred(16 * blk + (lane & 15)));
                 return 16 * blk + (b ? __builtin_ctzll(b) : 15);
             };
             // the first token whose running weight exceeds t: value, how many tokens of that value are ahead of it, and the running
@@ -278,32 +372,27 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
                 const double ahead = c ? sm.mass[c - 1] : 0.0;
                 const uint32_t n = counts(c);
                 const double w = n ? wt.at(64 * c + lane) : 0.0;
-                const double incl = ahead + scan_d((double)n * w, lane);
-                uint64_t any = __ballot(n != 0);
+                const double incl = ahead + scan_d((double)n * w);
+                const uint64_t any = __ballot(n != 0);
                 if (!any) return Found{lo, 0, 1.0};  // rounding put t between two chunks' sums
                 const uint64_t over = __ballot(n != 0 && incl > t);
                 const int l = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any);
-                const double before = incl - (double)n * w;
-                double jj = floor((t - before) / w);
-                jj = fmin(fmax(jj, 0.0), (double)(n ? n - 1 : 0));
-                if (!over) jj = (double)(n ? n - 1 : 0);
+                const double before = incl - (double)n * w, last = (double)(n ? n - 1 : 0);
+                const double jj = over ? fmin(fmax(floor((t - before) / w), 0.0), last) : last;
                 const double up = before + (jj + 1.0) * w;
-                return Found{64 * c + l, __shfl((int)jj, l, 64), shfl_d(up, l)};
+                return Found{64 * c + l, (int)lane_u((uint32_t)(int)jj, l), lane_d(up, l)};
             };
-            const double total = sm.mass[kChunks - 1];
-            double z = total;
-            const int k = a.top_k_v ? a.top_k_v[row] : a.top_k;
+            double z = sm.mass[kChunks - 1];
             if (k > 0 && (uint32_t)k < sm.count[kChunks - 1]) {
                 const int c = first_chunk([&](int i) { return sm.count[i] >= (uint32_t)k; });
                 const uint32_t n = counts(c);
                 const double w = n ? wt.at(64 * c + lane) : 0.0;
-                const uint32_t ci = (c ? sm.count[c - 1] : 0u) + scan_u(n, lane);
-                const double mi = (c ? sm.mass[c - 1] : 0.0) + scan_d((double)n * w, lane);
+                const uint32_t ci = (c ? sm.count[c - 1] : 0u) + scan_u(n);
+                const double mi = (c ? sm.mass[c - 1] : 0.0) + scan_d((double)n * w);
                 const uint64_t over = __ballot(n != 0 && ci >= (uint32_t)k);
                 const int l = over ? __builtin_ctzll(over) : 63;
-                z = fmin(z, shfl_d(mi - (double)(ci - (uint32_t)k) * w, l));
+                z = fmin(z, lane_d(mi - (double)(ci - (uint32_t)k) * w, l));
             }
-            const float p = a.top_p_v ? a.top_p_v[row] : a.top_p, mp = a.min_p_v ? a.min_p_v[row] : a.min_p;
             double zp = z;
             if (p > 0.f && p < 1.f) zp = fmin(zp, find((double)p * z).upto);
             if (mp > 0.f) {
@@ -322,11 +411,11 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
                 const int c = min(from, 65535) >> 6;
                 const uint32_t n = counts(c);
                 const double w = n ? wt.at(64 * c + lane) : 0.0;
-                const double mi = scan_d(64 * c + lane < from ? (double)n * w : 0.0, lane);
-                zp = fmin(zp, (c ? sm.mass[c - 1] : 0.0) + shfl_d(mi, 63));
+                const double mi = scan_d(64 * c + lane < from ? (double)n * w : 0.0);
+                zp = fmin(zp, (c ? sm.mass[c - 1] : 0.0) + lane_d(mi, 63));
             }
             zp = fmax(zp, 1.0);
-            double t = (double)a.u[row] * zp;
+            double t = (double)u * zp;
             if (!(t < zp)) t = __longlong_as_double(__double_as_longlong(zp) - 1);  // u of 1 or more: the last token kept
             const Found f = find(t);
             if (BIG || lane == 0) {
@@ -335,49 +424,64 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
             }
         }
         __syncthreads();
-        dk = sm.dk;
-        j = sm.j;
+        dk = __builtin_amdgcn_readfirstlane(sm.dk);
+        j = __builtin_amdgcn_readfirstlane(sm.j);
     }
 
     // the j-th token with this value, by index: matches per wave, then per 64-lane step, then per lane
-    auto is_match = [&](int d) { return d == dk || (dk == kPlusZero && d == kMinusZero); };
-    uint32_t mine = 0;
-    each([&](int d, int) { mine += is_match(d) ? 1u : 0u; });
-    uint32_t tot = mine;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) tot += __shfl_xor(tot, o, 64);
+    const uint32_t want = (uint32_t)dk * 0x10001u;
+    auto matches = [&](uint32_t o) -> uint32_t {  // bit 0: the first of two matches, bit 1: the second
+        const uint32_t x = o ^ want;
+        uint32_t m = ((x & 0xffffu) == 0 ? 1u : 0u) | ((x >> 16) == 0 ? 2u : 0u);
+        if (dk == kPlusZero) m |= ((o & 0xffffu) == kMinusZero ? 1u : 0u) | ((o >> 16) == kMinusZero ? 2u : 0u);
+        return m;
+    };
+    // (x - 1) & ~x has its top bit set where a half x is zero; it may be set above a half that is, which only costs the count
+    uint32_t some = 0;
+    each2([&](uint32_t o) {
+        const uint32_t x = o ^ want;
+        some |= (x - 0x10001u) & ~x;
+    });
+    uint32_t tot = 0;
+    if (dk == kPlusZero || __ballot((some & 0x80008000u) != 0)) {
+        uint32_t mine = 0;
+        each2([&](uint32_t o) { mine += __popc(matches(o)); });
+        tot = lane_u(scan_u(mine), 63);
+    }
+    if (lane == 0) sm.wave_count[wave] = tot;  // its readers of the scan above have passed a barrier since
     __syncthreads();
-    if (lane == 0) sm.wave_count[wave] = tot;
-    __syncthreads();
-    uint32_t before = 0;
-    for (int w = 0; w < wave; ++w) before += sm.wave_count[w];
+    const uint32_t before = lane_u(row_sum_u((lane & 15) < wave ? sm.wave_count[lane & 15] : 0u), 15);
     if ((uint32_t)j < before || (uint32_t)j >= before + tot) return;  // another wave has it
     uint32_t left = (uint32_t)j - before;
-    for (int s = 0; s < steps; ++s) {
-        const int ch = ch0 + 64 * s + lane;
+    bool done = false;
+    auto locate = [&](u32x4 v, int ch) {  // one 64-lane step; lanes without a chunk hold no match
         uint32_t bits = 0;
-        int e0 = 0;
-        if (ch < ch1) {
-            const u32x4 v = base[ch];
-            e0 = ch * 8 - lead;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const uint32_t o = order2(v[i >> 1]);
-                const int d = (int)((i & 1) ? o >> 16 : o & 0xffffu);
-                if (e0 + i >= 0 && e0 + i < a.vocab && is_match(d)) bits |= 1u << i;
-            }
-        }
-        const uint32_t incl = scan_u(__popc(bits), lane), sum = __shfl(incl, 63, 64);
+        for (int i = 0; i < 4; ++i) bits |= matches(v[i]) << (2 * i);
+        if (done || __ballot(bits != 0) == 0) return;
+        const uint32_t incl = scan_u(__popc(bits)), sum = lane_u(incl, 63);
         if (left >= sum) {
             left -= sum;
-            continue;
+            return;
         }
         uint32_t excl = incl - __popc(bits);
         if (left >= excl && left < incl) {
             for (; excl < left; ++excl) bits &= bits - 1;
-            a.out[row] = e0 + __builtin_ctz(bits);
+            a.out[row] = ch * 8 - lead + __builtin_ctz(bits);
         }
-        return;
+        done = true;
+    };
+    if constexpr (BIG) {
+        for (int s = 0; s < steps && !done; ++s) {
+            const int ch = ch0 + 64 * s + lane;
+            u32x4 v = {kNone, kNone, kNone, kNone};
+            if (ch < ch1) v = ordered(base[ch], ch);
+            locate(v, ch);
+        }
+    } else {
+#pragma unroll
+        for (int s = 0; s < kSampleSteps; ++s)
+            if (s < steps) locate(reg[s], ch0 + 64 * s + lane);
     }
 }
 
