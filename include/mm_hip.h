@@ -362,12 +362,13 @@ int mm_adam_step(void* const* params, const void* const* grads, float* master, f
  * [past | new] keys and values for every token: here a layer's keys and values live in pages of page_size token slots that
  * sequences take as they grow, and a step appends to them in place.
  *
- * mm_paged_kv: one layer's pages.  k, v point at page 0, head 0, slot 0; the strides are in elements (a slot's hn elements are
- * contiguous), each a multiple of 8 and below 2^31, page strides times 2 below 2^32 bytes; k and v 16-byte aligned.  hn in {64, 128}. */
+ * mm_paged_kv: one layer's pages.  k, v point at page 0, head 0, slot 0 of the keys and of the values; the strides, the same for
+ * both, are in elements (a slot's hn elements are contiguous), each a multiple of 8 in (0, 2^31), page_size times slot below 2^30;
+ * k and v 16-byte aligned.  hn in {64, 128}. */
 typedef struct mm_paged_kv {
     void* k;
     void* v;
-    int64_t k_page, k_head, k_slot, v_page, v_head, v_slot;
+    int64_t page, head, slot;
     int num_pages, page_size, heads, hn, dtype;
 } mm_paged_kv;
 /* mm_paged_step: what one step brings, shared by all layers; every array is in device memory and read at run time, so that a

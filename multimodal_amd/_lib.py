@@ -20,7 +20,7 @@ c_int, c_float, c_void_p, c_size_t, c_u64, c_i64 = (
 
 
 class MmPagedKV(ctypes.Structure):  # mm_paged_kv
-    _fields_ = [("k", c_void_p), ("v", c_void_p)] + [(n, c_i64) for n in ("k_page", "k_head", "k_slot", "v_page", "v_head", "v_slot")] + [
+    _fields_ = [("k", c_void_p), ("v", c_void_p)] + [(n, c_i64) for n in ("page", "head", "slot")] + [
         (n, c_int) for n in ("num_pages", "page_size", "heads", "hn", "dtype")]
 
 

@@ -10,7 +10,6 @@
 // rows and rotation allow it, else W = 1.
 #include "common.h"
 #include "paged.h"
-#include <initializer_list>
 
 namespace mm {
 
@@ -74,8 +73,7 @@ __global__ __launch_bounds__(256) void paged_kv_append_k(const AppendArgs a, int
         const int off = pos - pi * a.kv.page_size;
         rot = rot && is_k;
         src = is_k ? a.k + (int64_t)row * a.k_row + (int64_t)h * a.k_head : a.v + (int64_t)row * a.v_row + (int64_t)h * a.v_head;
-        dst = is_k ? (u16*)a.kv.k + (int64_t)page * a.kv.k_page + (int64_t)h * a.kv.k_head + (int64_t)off * a.kv.k_slot
-                   : (u16*)a.kv.v + (int64_t)page * a.kv.v_page + (int64_t)h * a.kv.v_head + (int64_t)off * a.kv.v_slot;
+        dst = (u16*)(is_k ? a.kv.k : a.kv.v) + (int64_t)page * a.kv.page + (int64_t)h * a.kv.head + (int64_t)off * a.kv.slot;
     }
     rot = rot && c < hc;
     // the item's two chunks: partners in the rotated part; behind it (everywhere for an unrotated row) neighbours

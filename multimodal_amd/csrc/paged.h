@@ -1,6 +1,7 @@
 // paged.h - what the kernels of the paged key / value cache share: the row -> sequence search, the key -> page arithmetic.
 #pragma once
 #include "common.h"
+#include <initializer_list>
 
 namespace mm {
 
@@ -19,6 +20,31 @@ inline FastDiv make_fastdiv(int d) {
     return f;
 }
 __device__ __forceinline__ uint32_t fdiv(uint32_t n, const FastDiv& f) { return (__umulhi(f.m, n) + n) >> f.l; }
+
+// A key's place in the cache while a thread walks the keys of a sequence in equal steps: its page's index in the block table and
+// the bytes from the page's start to its slot.  A step of n keys is n / page_size pages and n % page_size slots, so that moving on
+// takes two additions and a conditional carry, and no division or multiplication.
+struct PageStep {
+    uint32_t pages, bytes;  // n / page_size, (n % page_size) slots in bytes
+};
+__device__ __forceinline__ PageStep page_step(uint32_t n, const FastDiv& f, uint32_t slot_bytes) {
+    const uint32_t p = fdiv(n, f);
+    return PageStep{p, (n - p * f.d) * slot_bytes};
+}
+struct PageCursor {
+    uint32_t page, byte;
+    __device__ __forceinline__ void set(uint32_t key, const FastDiv& f, uint32_t slot_bytes) {
+        page = fdiv(key, f);
+        byte = (key - page * f.d) * slot_bytes;
+    }
+    __device__ __forceinline__ void move(const PageStep& s, uint32_t page_bytes) {
+        page += s.pages;
+        byte += s.bytes;
+        const bool c = byte >= page_bytes;
+        byte -= c ? page_bytes : 0u;
+        page += c ? 1u : 0u;
+    }
+};
 
 // The sequence of packed row `row` in cu[0 .. n]: the number of i with cu[i + 1] <= row, found by a whole wave, 64 boundaries a
 // step (one step up to 64 sequences, two up to 4096).  n when the row is behind the last sequence; the caller also checks
@@ -49,12 +75,9 @@ inline int check_paged(const char* fn, const mm_paged_kv* kv, const mm_paged_ste
     MM_CHECK_ARG(st->max_new >= 0 && st->max_kv >= 0 && st->table_stride >= st->max_pages,
                  "%s: max_new=%d max_kv=%d table_stride=%lld out of range", fn, st->max_new, st->max_kv, (long long)st->table_stride);
     MM_CHECK_ARG(aligned16(kv->k) && aligned16(kv->v), "%s: the cache must be 16-byte aligned", fn);
-    const int64_t str[6] = {kv->k_page, kv->k_head, kv->k_slot, kv->v_page, kv->v_head, kv->v_slot};
-    for (int64_t x : str)
-        MM_CHECK_ARG(x >= 0 && x % 8 == 0 && x < (int64_t)1 << 31, "%s: cache stride %lld must be a multiple of 8 in [0, 2^31)", fn,
-                     (long long)x);
-    MM_CHECK_ARG(kv->page_size * kv->k_slot < (int64_t)1 << 31 && kv->page_size * kv->v_slot < (int64_t)1 << 31,
-                 "%s: a page's slots span 2^31 elements or more", fn);
+    for (int64_t x : {kv->page, kv->head, kv->slot})
+        MM_CHECK_ARG(x > 0 && x % 8 == 0 && x < (int64_t)1 << 31, "%s: cache stride %lld must be a multiple of 8 in (0, 2^31)", fn, (long long)x);
+    MM_CHECK_ARG(kv->page_size * kv->slot < (int64_t)1 << 30, "%s: a page's slots span 2^30 elements or more", fn);
     return MM_OK;
 }
 

@@ -34,6 +34,9 @@ struct PagedAttnArgs {
     float *ws_o, *ws_ml;  // nsplit > 1: [nsplit, rows, nq, hn] unnormalised outputs, [nsplit, rows, nq, 2] (max, sum)
 };
 
+// How far a score may exceed the running reference of a row's exponentials (in powers of two) before the row is rescaled
+constexpr float kLag = 8.f;
+
 // {first row, new rows, length} of a sequence; false: nothing to do
 struct SeqInfo {
     int beg, n, len;
@@ -79,6 +82,7 @@ template <typename T> __device__ __forceinline__ bool take_nonfinite(u32x4& v) {
     }
     return any != 0;
 }
+__device__ __forceinline__ uint32_t scalar(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 // the infinity or NaN at p, else 0
 template <typename T> __device__ __forceinline__ float only_nonfinite(const u16* __restrict__ p) {
     const u16 v = *p;
@@ -136,34 +140,37 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_few_k(const PagedAttnArgs 
     for (int i = 0; i < NC; ++i) qf[i] = *reinterpret_cast<const frag*>(qp + 32 * i + 8 * g);
 
     const int32_t* bt = a.st.block_table + (int64_t)seq * a.st.table_stride;
-    const u16* kb = (const u16*)a.kv.k + (int64_t)kh * a.kv.k_head + 8 * g;
-    const u16* vb = (const u16*)a.kv.v + (int64_t)kh * a.kv.v_head + 8 * g;
+    const char* kb = (const char*)((const u16*)a.kv.k + (int64_t)kh * a.kv.head + 8 * g);
+    const int64_t k_to_v = (const char*)a.kv.v - (const char*)a.kv.k;
+    const uint32_t page_stride = 2 * (uint32_t)a.kv.page, slot_bytes = 2 * (uint32_t)a.kv.slot, page_bytes = slot_bytes * a.page.d;
+    const PageStep stride = page_step(NW * 32, a.page, slot_bytes);
+    const uint32_t last_page = s.len > 0 ? fdiv((uint32_t)s.len - 1, a.page) : 0;  // behind it the table is not the sequence's
 
     u32x4 kr[2][NC], vr[2][NC];
+    PageCursor cur[2];
     int pid[2];
-    uint32_t bad = 0;  // bit t: this lane's key of sub-tile t is in a page the cache does not have
-    auto fetch_pid = [&](int kt) {
+    uint32_t at[2];    // bytes from the page's start to this lane's key of sub-tile t
+    uint32_t bad = 0;  // bit t: it is in a page the cache does not have
+    auto fetch_pid = [&]() {  // page ids of the cursor's keys; the cursor moves on to the next tile
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const int key = min(kt + 16 * t + r, s.len - 1);
-            pid[t] = bt[fdiv((uint32_t)key, a.page)];
+            pid[t] = bt[min(cur[t].page, last_page)];
+            at[t] = cur[t].byte;
+            cur[t].move(stride, page_bytes);
         }
     };
-    auto fetch = [&](int kt) {
+    auto fetch = [&]() {  // keys and values of the tile whose page ids are here
         bad = 0;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            const int key = min(kt + 16 * t + r, s.len - 1);
-            const int off = key - (int)(fdiv((uint32_t)key, a.page) * a.page.d);
             const bool b = (uint32_t)pid[t] >= (uint32_t)a.kv.num_pages;
-            const uint32_t pg = b ? 0u : (uint32_t)pid[t];
             bad |= b ? 1u << t : 0u;
-            const u16* kp = kb + (uint64_t)pg * (uint32_t)a.kv.k_page + (uint32_t)off * (uint32_t)a.kv.k_slot;
-            const u16* vp = vb + (uint64_t)pg * (uint32_t)a.kv.v_page + (uint32_t)off * (uint32_t)a.kv.v_slot;
+            const char* kp = kb + (uint64_t)(b ? 0u : (uint32_t)pid[t]) * page_stride + at[t];
+            const char* vp = kp + k_to_v;
 #pragma unroll
-            for (int i = 0; i < NC; ++i) kr[t][i] = *reinterpret_cast<const u32x4*>(kp + 32 * i);
+            for (int i = 0; i < NC; ++i) kr[t][i] = *reinterpret_cast<const u32x4*>(kp + 64 * i);
 #pragma unroll
-            for (int i = 0; i < NC; ++i) vr[t][i] = *reinterpret_cast<const u32x4*>(vp + 32 * i);
+            for (int i = 0; i < NC; ++i) vr[t][i] = *reinterpret_cast<const u32x4*>(vp + 64 * i);
         }
     };
 
@@ -175,9 +182,11 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_few_k(const PagedAttnArgs 
 
     int kt = c0 + wave * 32;
     if (kt < c1) {
-        fetch_pid(kt);
-        fetch(kt);
-        fetch_pid(kt + NW * 32);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) cur[t].set((uint32_t)(kt + 16 * t + r), a.page, slot_bytes);
+        fetch_pid();
+        fetch();
+        fetch_pid();
     }
     for (; kt < c1; kt += NW * 32) {
         // the tile's values into LDS, its keys into the matrix unit; then its registers take the next tile
@@ -209,8 +218,8 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_few_k(const PagedAttnArgs 
             for (int i = 0; i < NC; ++i) sc[t] = M16<T>::run(__builtin_bit_cast(frag, kr[t][i]), qf[i], sc[t]);
         }
         if (kt + NW * 32 < c1) {
-            fetch(kt + NW * 32);
-            fetch_pid(kt + 2 * NW * 32);
+            fetch();
+            fetch_pid();
         }
         if (badk[0] | badk[1]) {
 #pragma unroll
@@ -229,15 +238,16 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_few_k(const PagedAttnArgs 
         float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])), fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
         mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
         mx = half_max(mx);
-        const float m_new = fmaxf(m_run, mx * a.scale_log2e);
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;  // no key seen yet: every p is exp2(-inf) = 0
-        if (__any(m_new > m_run)) {
-            const float alpha = fast_exp2(m_run - m_use);
+        const float m_tile = mx * a.scale_log2e;
+        if (__any(m_tile > m_run + kLag)) {
+            const float m_new = fmaxf(m_run, m_tile);
+            const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
             l_run *= alpha;
 #pragma unroll
             for (int d = 0; d < NDB; ++d) o[d] *= alpha;
+            m_run = m_new;
         }
-        m_run = m_new;
+        const float m_use = m_run == -INFINITY ? 0.f : m_run;  // no key seen yet: every p is exp2(-inf) = 0
         float p[2][4];
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -262,8 +272,8 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_few_k(const PagedAttnArgs 
                 const int key = kt + __builtin_ctz(left);
                 const int pi = (int)fdiv((uint32_t)key, a.page), pg = bt[pi];
                 if ((uint32_t)pg >= (uint32_t)a.kv.num_pages || key > limit) continue;
-                const u16* vp = (const u16*)a.kv.v + (int64_t)pg * a.kv.v_page + (int64_t)kh * a.kv.v_head +
-                                (int64_t)(key - pi * (int)a.page.d) * a.kv.v_slot;
+                const u16* vp = (const u16*)a.kv.v + (int64_t)pg * a.kv.page + (int64_t)kh * a.kv.head +
+                                (int64_t)(key - pi * (int)a.page.d) * a.kv.slot;
 #pragma unroll
                 for (int d = 0; d < NDB; ++d)
 #pragma unroll
@@ -328,7 +338,7 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_few_k(const PagedAttnArgs 
 // in 64-key tiles, global -> registers -> double-buffered LDS, one barrier a tile; page ids are fetched a tile further ahead, so
 // that no load waits for another.  Row blocks with the most keys start first.
 template <typename T, int HD>
-__global__ __launch_bounds__(256, (HD == 64 ? 2 : 1)) void paged_attn_many_k(const PagedAttnArgs a) {
+__global__ __launch_bounds__(256, (HD == 64 ? 3 : 2)) void paged_attn_many_k(const PagedAttnArgs a) {
     typedef Tile<HD> TL;
     typedef typename M32<T>::frag frag;
     constexpr int NDS = HD / 16, NDB = HD / 32, NCH = TL::NCH;
@@ -367,26 +377,33 @@ __global__ __launch_bounds__(256, (HD == 64 ? 2 : 1)) void paged_attn_many_k(con
     const int32_t* bt = a.st.block_table + (int64_t)seq * a.st.table_stride;
     const int trow = tid / TL::CPR, tch = tid % TL::CPR;  // this thread's first row and its 16-byte chunk of a tile
     constexpr int RSTEP = 256 / TL::CPR;
-    const u16* kb = (const u16*)a.kv.k + (int64_t)kh * a.kv.k_head + tch * 8;
-    const u16* vb = (const u16*)a.kv.v + (int64_t)kh * a.kv.v_head + tch * 8;
+    const char* kb = (const char*)((const u16*)a.kv.k + (int64_t)kh * a.kv.head + tch * 8);
+    const int64_t k_to_v = (const char*)a.kv.v - (const char*)a.kv.k;
+    const uint32_t page_stride = 2 * (uint32_t)a.kv.page, slot_bytes = 2 * (uint32_t)a.kv.slot, page_bytes = slot_bytes * a.page.d;
+    const PageStep stride = page_step(64, a.page, slot_bytes);
+    const uint32_t last_page = s.len > 0 ? fdiv((uint32_t)s.len - 1, a.page) : 0;  // behind it the table is not the sequence's
     u32x4 kreg[NCH], vreg[NCH];
+    PageCursor pos[NCH];
     int pid[NCH];
+    uint32_t at[NCH];
     uint32_t bad = 0;
-    auto fetch_pid = [&](int kv0) {
+    auto fetch_pid = [&]() {  // page ids of the cursor's keys; the cursor moves on to the next tile
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) pid[i] = bt[fdiv((uint32_t)min(kv0 + trow + RSTEP * i, s.len - 1), a.page)];
+        for (int i = 0; i < NCH; ++i) {
+            pid[i] = bt[min(pos[i].page, last_page)];
+            at[i] = pos[i].byte;
+            pos[i].move(stride, page_bytes);
+        }
     };
-    auto fetch = [&](int kv0) {
+    auto fetch = [&]() {  // keys and values of the tile whose page ids are here
         bad = 0;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
-            const int key = min(kv0 + trow + RSTEP * i, s.len - 1);
-            const uint32_t off = (uint32_t)key - fdiv((uint32_t)key, a.page) * a.page.d;
             const bool b = (uint32_t)pid[i] >= (uint32_t)a.kv.num_pages;
-            const uint32_t pg = b ? 0u : (uint32_t)pid[i];
             bad |= b ? 1u << i : 0u;
-            kreg[i] = *reinterpret_cast<const u32x4*>(kb + (uint64_t)pg * (uint32_t)a.kv.k_page + off * (uint32_t)a.kv.k_slot);
-            vreg[i] = *reinterpret_cast<const u32x4*>(vb + (uint64_t)pg * (uint32_t)a.kv.v_page + off * (uint32_t)a.kv.v_slot);
+            const char* kp = kb + (uint64_t)(b ? 0u : (uint32_t)pid[i]) * page_stride + at[i];
+            kreg[i] = *reinterpret_cast<const u32x4*>(kp);
+            vreg[i] = *reinterpret_cast<const u32x4*>(kp + k_to_v);
         }
     };
     // registers -> LDS stage of tile j; where some row of the block does not see the whole tile, the values behind the end become
@@ -402,7 +419,7 @@ __global__ __launch_bounds__(256, (HD == 64 ? 2 : 1)) void paged_attn_many_k(con
                 if (take_nonfinite<T>(vreg[i])) atomicOr(fl + 1, 1ull << key);
             }
         }
-        if (bad) {
+        if (__ballot(bad != 0)) {
 #pragma unroll
             for (int i = 0; i < NCH; ++i)
                 if ((bad >> i) & 1) atomicOr(fl, 1ull << (trow + RSTEP * i));
@@ -421,9 +438,11 @@ __global__ __launch_bounds__(256, (HD == 64 ? 2 : 1)) void paged_attn_many_k(con
     if (tid < 8) flags[tid] = 0;
     __syncthreads();
     if (ntiles > 0) {
-        fetch_pid(c0);
-        fetch(c0);
-        fetch_pid(c0 + 64);
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) pos[i].set((uint32_t)(c0 + trow + RSTEP * i), a.page, slot_bytes);
+        fetch_pid();
+        fetch();
+        fetch_pid();
         put(smem, 0);
     }
     __syncthreads();
@@ -436,13 +455,15 @@ __global__ __launch_bounds__(256, (HD == 64 ? 2 : 1)) void paged_attn_many_k(con
         const char* vs = ks + TL::BYTES;
         const int kv0 = c0 + j * 64;
         if (j + 1 < ntiles) {
-            fetch(kv0 + 64);
-            fetch_pid(kv0 + 128);
+            fetch();
+            fetch_pid();
         }
         if (tid < 2) flags[2 * ((j + 2) & 3) + tid] = 0;  // read in tile j - 2, written for tile j + 2 behind this tile's barrier
-        const unsigned long long badk = flags[2 * (j & 3)], nonf = flags[2 * (j & 3) + 1];
+        const u32x4 fl = *reinterpret_cast<const u32x4*>(flags + 2 * (j & 3));
+        const uint32_t badk[2] = {scalar(fl[0]), scalar(fl[1])}, nonf[2] = {scalar(fl[2]), scalar(fl[3])};
         if (kv0 <= wave_last) {
             f32x16 sacc[2];
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
 #pragma unroll
@@ -450,12 +471,15 @@ __global__ __launch_bounds__(256, (HD == 64 ? 2 : 1)) void paged_attn_many_k(con
 #pragma unroll
                 for (int ds = 0; ds < NDS; ++ds) sacc[t] = M32<T>::run(row_frag<T, HD>(ks, 32 * t, ds, lane), qf[ds], sacc[t]);
             }
-            if (badk) {
+            __builtin_amdgcn_s_setprio(0);
+            if (badk[0] | badk[1]) {
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
+                for (int t = 0; t < 2; ++t) {
+                    const uint32_t b = badk[t] >> (4 * hh);
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        if ((badk >> (32 * t + acc_row(i, hh))) & 1) sacc[t][i] = __builtin_nanf("");
+                        if ((b >> acc_row(i, 0)) & 1) sacc[t][i] = __builtin_nanf("");
+                }
             }
             if (kv0 + 63 > wave_first) {
 #pragma unroll
@@ -468,8 +492,20 @@ __global__ __launch_bounds__(256, (HD == 64 ? 2 : 1)) void paged_attn_many_k(con
 #pragma unroll
             for (int i = 1; i < 16; ++i) rmax = fmaxf(fmaxf(rmax, sacc[0][i]), sacc[1][i]);
             rmax = half_max(rmax);
-            const float m_new = fmaxf(m_run, rmax * a.scale_log2e);
-            const float m_use = m_new == -INFINITY ? 0.f : m_new;  // no key seen yet
+            // The reference value of the exponentials only moves when a score exceeds it by more than kLag: probabilities are then
+            // at most 2^kLag, their relative rounding is the same, and most tiles need no rescaling.
+            const float m_tile = rmax * a.scale_log2e;
+            if (__any(m_tile > m_run + kLag)) {
+                const float m_new = fmaxf(m_run, m_tile);
+                const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m_run - m_new);
+                l_run *= alpha;
+#pragma unroll
+                for (int d = 0; d < NDB; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
+                m_run = m_new;
+            }
+            const float m_use = m_run == -INFINITY ? 0.f : m_run;  // no key seen yet: every p is exp2(-inf) = 0
             float lsum = 0.f;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -478,16 +514,8 @@ __global__ __launch_bounds__(256, (HD == 64 ? 2 : 1)) void paged_attn_many_k(con
                     sacc[t][i] = fast_exp2(sacc[t][i] * a.scale_log2e - m_use);
                     lsum += sacc[t][i];
                 }
-            if (__any(m_new > m_run)) {
-                const float alpha = fast_exp2(m_run - m_use);
-                l_run *= alpha;
-#pragma unroll
-                for (int d = 0; d < NDB; ++d)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[d][i] *= alpha;
-            }
             l_run += lsum;
-            m_run = m_new;
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -495,15 +523,17 @@ __global__ __launch_bounds__(256, (HD == 64 ? 2 : 1)) void paged_attn_many_k(con
                     const frag pf = M32<T>::cvt8(sacc[t][8 * s2], sacc[t][8 * s2 + 1], sacc[t][8 * s2 + 2], sacc[t][8 * s2 + 3],
                                                  sacc[t][8 * s2 + 4], sacc[t][8 * s2 + 5], sacc[t][8 * s2 + 6], sacc[t][8 * s2 + 7]);
 #pragma unroll
-                    for (int d = 0; d < NDB; ++d) o[d] = M32<T>::run(tr_frag<T, HD>(vs, 32 * t + 16 * s2, d, lane), pf, o[d]);
+                    for (int d = 0; d < NDB; ++d)
+                        o[d] = M32<T>::run(tr_frag<T, HD>(vs, 32 * t + 16 * s2, d, lane), pf, o[d]);
                 }
-            if (nonf) {
-                for (unsigned long long left = nonf; left; left &= left - 1) {
+            __builtin_amdgcn_s_setprio(0);
+            if (nonf[0] | nonf[1]) {
+                for (unsigned long long left = nonf[0] | (unsigned long long)nonf[1] << 32; left; left &= left - 1) {
                     const int key = kv0 + __builtin_ctzll(left);
                     const int pi = (int)fdiv((uint32_t)key, a.page), pg = bt[pi];
                     if ((uint32_t)pg >= (uint32_t)a.kv.num_pages || key > limit) continue;
-                    const u16* vp = (const u16*)a.kv.v + (int64_t)pg * a.kv.v_page + (int64_t)kh * a.kv.v_head +
-                                    (int64_t)(key - pi * (int)a.page.d) * a.kv.v_slot;
+                    const u16* vp = (const u16*)a.kv.v + (int64_t)pg * a.kv.page + (int64_t)kh * a.kv.head +
+                                    (int64_t)(key - pi * (int)a.page.d) * a.kv.slot;
 #pragma unroll
                     for (int d = 0; d < NDB; ++d)
 #pragma unroll

@@ -14,8 +14,8 @@ from ._lib import MmPagedKV, MmPagedStep, dtype_code
 
 
 class PagedKV:
-    """One layer's pages: k and v [num_pages, heads, page_size, hn] in fp16 / bf16, head size 64 or 128.  Any strides that are
-    multiples of 8 elements with the head dim contiguous, so both may be views of one tensor."""
+    """One layer's pages: k and v [num_pages, heads, page_size, hn] in fp16 / bf16, head size 64 or 128.  Any strides, the same for
+    both, that are multiples of 8 elements with the head dim contiguous: both may be views of one tensor."""
 
     def __init__(self, k, v):
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or not k.is_cuda:
@@ -24,13 +24,13 @@ class PagedKV:
             raise RuntimeError(f"PagedKV: head size {k.size(3)} not supported (64 or 128)")
         if min(k.shape) < 1:
             raise RuntimeError(f"PagedKV: empty cache {tuple(k.shape)}")
-        for t in (k, v):
-            if t.stride(3) != 1 or any(s % 8 or s < 0 for s in t.stride()[:3]) or t.data_ptr() % 16:
-                raise RuntimeError("PagedKV: pages must be 16-byte aligned with a contiguous head dim and strides that are multiples of 8")
+        if k.stride() != v.stride() or k.stride(3) != 1 or any(s % 8 or s <= 0 for s in k.stride()[:3]) or k.data_ptr() % 16 or v.data_ptr() % 16:
+            raise RuntimeError("PagedKV: pages must be 16-byte aligned with a contiguous head dim and positive strides that are multiples "
+                               f"of 8, the same for k and v; got {k.stride()} and {v.stride()}")
         self.k, self.v = k, v
         self.num_pages, self.heads, self.page_size, self.hn = k.shape
         self.dtype, self.device = k.dtype, k.device
-        self._c = MmPagedKV(k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], self.num_pages, self.page_size, self.heads,
+        self._c = MmPagedKV(k.data_ptr(), v.data_ptr(), *k.stride()[:3], self.num_pages, self.page_size, self.heads,
                             self.hn, dtype_code(k.dtype))
         self._ref = ctypes.addressof(self._c)
 

@@ -703,6 +703,7 @@ def embed_prefix(table, tokens, prefix=None):
 
 
 # ---------------------------------------------------------------------------- text generation: paged key / value cache
+# A token step of one sequence is a few microseconds of GPU time a call: these wrappers read each tensor's shape and strides once.
 def _launch(device, fn, *args):
     """fn(*args, stream) with the current stream of `device`, which need not be the current device."""
     if device.index == torch.cuda.current_device():
@@ -711,17 +712,27 @@ def _launch(device, fn, *args):
         return fn(*args, torch.cuda.current_stream().cuda_stream)
 
 
-def _rows(name, t, kv, heads=None):
-    """A [rows, heads, hn] operand in the cache's dtype, on its device, with a contiguous head dim."""
-    if t.dim() != 3 or t.size(2) != kv.hn or (heads is not None and t.size(1) != heads) or t.dtype != kv.dtype or t.device != kv.device:
-        raise RuntimeError(f"{name} must be a [rows, {'heads' if heads is None else heads}, {kv.hn}] {kv.dtype} tensor on {kv.device}, "
-                           f"got {tuple(t.shape)} {t.dtype} on {t.device}")
-    return t if t.stride(2) == 1 else t.contiguous()
+def _rows(name, t, kv, rows=None, heads=None):
+    """(tensor, rows, heads, strides) of a [rows, heads, hn] operand in the cache's dtype, on its device, its head dim contiguous."""
+    shape = t.shape
+    if (len(shape) != 3 or shape[2] != kv.hn or t.dtype != kv.dtype or t.device != kv.device
+            or (heads is not None and shape[1] != heads) or (rows is not None and shape[0] != rows)):
+        raise RuntimeError(f"{name} must be a [{'rows' if rows is None else rows}, {'heads' if heads is None else heads}, {kv.hn}] "
+                           f"{kv.dtype} tensor on {kv.device}, got {tuple(shape)} {t.dtype} on {t.device}")
+    stride = t.stride()
+    if stride[2] != 1:
+        t = t.contiguous()
+        stride = t.stride()
+    return t, shape[0], shape[1], stride
 
 
-def _out_rows(name, t, like, dtype):
-    if t.shape != like or t.dtype != dtype or t.stride(-1) != 1:
-        raise RuntimeError(f"{name} must be a {tuple(like)} {dtype} tensor with a contiguous last dim, got {tuple(t.shape)} {t.dtype}")
+def _out_rows(name, t, shape, dtype, device):
+    """The strides of an output the caller brings."""
+    stride = t.stride()
+    if t.shape != shape or t.dtype != dtype or t.device != device or stride[-1] != 1:
+        raise RuntimeError(f"{name} must be a {tuple(shape)} {dtype} tensor on {device} with a contiguous last dim, got {tuple(t.shape)} "
+                           f"{t.dtype} on {t.device}, strides {stride}")
+    return stride
 
 
 def paged_kv_append(kv, step, k, v, q=None, cos=None, sin=None, q_out=None):
@@ -730,39 +741,35 @@ def paged_kv_append(kv, step, k, v, q=None, cos=None, sin=None, q_out=None):
     each row's position.  kv: kv_cache.PagedKV, step: kv_cache.PagedStep.  Returns q_out (allocated unless given; it may be q;
     rows of no sequence are left as they were), or None without q.  k, v and q may be strided views, e.g. the slices of the
     layer's fused [rows, heads, 3, hn] projection.  No backward: generation only."""
-    if kv.device != step.device:
-        raise RuntimeError(f"paged_kv_append: cache on {kv.device}, step on {step.device}")
-    k, v = _rows("paged_kv_append: k", k, kv, kv.heads), _rows("paged_kv_append: v", v, kv, kv.heads)
-    rows = k.size(0)
-    if v.size(0) != rows:
-        raise RuntimeError(f"paged_kv_append: {rows} key rows but {v.size(0)} value rows")
-    qa = (0, 0, 0, 0, 0, 0, 0)
+    dev = kv.device
+    if dev != step.device:
+        raise RuntimeError(f"paged_kv_append: cache on {dev}, step on {step.device}")
+    k, rows, _, ks = _rows("paged_kv_append: k", k, kv, None, kv.heads)
+    v, _, _, vs = _rows("paged_kv_append: v", v, kv, rows, kv.heads)
+    qp = qo = nq = 0
+    qs = os = (0, 0)
     if q is not None:
-        q = _rows("paged_kv_append: q", q, kv)
-        if q.size(0) != rows:
-            raise RuntimeError(f"paged_kv_append: {rows} key rows but {q.size(0)} query rows")
+        q, _, nq, qs = _rows("paged_kv_append: q", q, kv, rows)
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            q_out = torch.empty(rows, nq, kv.hn, dtype=kv.dtype, device=dev)
+            os = (nq * kv.hn, kv.hn)
         else:
-            _out_rows("paged_kv_append: q_out", q_out, q.shape, q.dtype)
-            if q_out.device != q.device:
-                raise RuntimeError(f"paged_kv_append: q_out on {q_out.device}, the cache on {q.device}")
-        qa = (q.data_ptr(), q.stride(0), q.stride(1), q_out.data_ptr(), q_out.stride(0), q_out.stride(1), q.size(1))
+            os = _out_rows("paged_kv_append: q_out", q_out, q.shape, kv.dtype, dev)
+        qp, qo = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise RuntimeError("paged_kv_append: q_out without q")
-    d = table_rows = fp32 = 0
-    cp = sp = 0
+    d = table_rows = fp32 = cp = sp = 0
     if cos is not None or sin is not None:
-        if cos is None or sin is None or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.device != kv.device or sin.device != kv.device:
+        if cos is None or sin is None or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.device != dev or sin.device != dev:
             raise RuntimeError("paged_kv_append: cos and sin must be two tables of one shape and dtype on the cache's device")
-        d = cos.size(-1)
-        if d % 2 or not 0 < d <= kv.hn or cos.numel() == 0 or cos.dtype not in (torch.float32, kv.dtype):
-            raise RuntimeError(f"paged_kv_append: tables {tuple(cos.shape)} {cos.dtype} must be [positions, d], d even and at most "
+        d, n, dt = cos.shape[-1], cos.numel(), cos.dtype
+        if d % 2 or not 0 < d <= kv.hn or n == 0 or (dt != torch.float32 and dt != kv.dtype):
+            raise RuntimeError(f"paged_kv_append: tables {tuple(cos.shape)} {dt} must be [positions, d], d even and at most "
                                f"{kv.hn}, in fp32 or {kv.dtype}")
         cos, sin = cos.contiguous(), sin.contiguous()
-        cp, sp, table_rows, fp32 = cos.data_ptr(), sin.data_ptr(), cos.numel() // d, int(cos.dtype == torch.float32)
-    check(_launch(kv.device, get_lib().mm_paged_kv_append, kv._ref, step._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                  v.stride(0), v.stride(1), *qa, rows, cp, sp, d, table_rows, fp32), "paged_kv_append")
+        cp, sp, table_rows, fp32 = cos.data_ptr(), sin.data_ptr(), n // d, dt == torch.float32
+    check(_launch(dev, get_lib().mm_paged_kv_append, kv._ref, step._ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], qp,
+                  qs[0], qs[1], qo, os[0], os[1], nq, rows, cp, sp, d, table_rows, fp32), "paged_kv_append")
     return q_out
 
 
@@ -771,36 +778,37 @@ def paged_attn_fwd(kv, step, q, softmax_scale, out=None, lse=None):
     sees keys 0 .. p of its sequence, query head h reads key head h // (nq // kv.heads).  Returns (out [rows, nq, hn], lse [rows,
     nq] fp32), allocated unless given; rows of no sequence are left as they were, a row that sees no key gets 0 and -inf.  No
     backward: generation only."""
-    if kv.device != step.device:
-        raise RuntimeError(f"paged_attn_fwd: cache on {kv.device}, step on {step.device}")
-    q = _rows("paged_attn_fwd: q", q, kv)
-    if q.stride(0) % 8 or q.stride(1) % 8 or q.data_ptr() % 16:
-        q = q.contiguous() if not q.is_contiguous() else q.clone()
-    rows, nq, _ = q.shape
+    dev = kv.device
+    if dev != step.device:
+        raise RuntimeError(f"paged_attn_fwd: cache on {dev}, step on {step.device}")
+    q, rows, nq, qs = _rows("paged_attn_fwd: q", q, kv)
+    qp = q.data_ptr()
+    if qs[0] % 8 or qs[1] % 8 or qp % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+        qs, qp = q.stride(), q.data_ptr()
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty(rows, nq, kv.hn, dtype=kv.dtype, device=dev)
+        os = (nq * kv.hn, kv.hn)
     else:
-        _out_rows("paged_attn_fwd: out", out, q.shape, q.dtype)
-        if out.device != q.device or out.stride(0) % 8 or out.stride(1) % 8 or out.data_ptr() % 16:
-            raise RuntimeError("paged_attn_fwd: out must be 16-byte aligned with strides a multiple of 8, on the cache's device")
+        os = _out_rows("paged_attn_fwd: out", out, q.shape, kv.dtype, dev)
+        if os[0] % 8 or os[1] % 8 or out.data_ptr() % 16:
+            raise RuntimeError("paged_attn_fwd: out must be 16-byte aligned with strides a multiple of 8")
     if lse is None:
-        lse = torch.empty(rows, nq, dtype=torch.float32, device=q.device)
+        lse = torch.empty(rows, nq, dtype=torch.float32, device=dev)
+        ls = nq
     else:
-        _out_rows("paged_attn_fwd: lse", lse, q.shape[:2], torch.float32)
-        if lse.device != q.device:
-            raise RuntimeError(f"paged_attn_fwd: lse on {lse.device}, the cache on {q.device}")
+        ls = _out_rows("paged_attn_fwd: lse", lse, (rows, nq), torch.float32, dev)[0]
     lib = get_lib()
     ws_bytes = lib.mm_paged_attn_workspace_bytes(kv._ref, step._ref, nq, rows)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-    check(_launch(q.device, lib.mm_paged_attn_fwd, kv._ref, step._ref, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(),
-                  lse.stride(0), q.data_ptr(), q.stride(0), q.stride(1), nq, rows, float(softmax_scale), _ptr(ws), ws_bytes),
-          "paged_attn_fwd")
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    check(_launch(dev, lib.mm_paged_attn_fwd, kv._ref, step._ref, out.data_ptr(), os[0], os[1], lse.data_ptr(), ls, qp, qs[0], qs[1],
+                  nq, rows, softmax_scale, ws.data_ptr() if ws_bytes else 0, ws_bytes), "paged_attn_fwd")
     return out, lse
 
 
 # ---------------------------------------------------------------------------- text generation: the next token
 def _per_row(name, v, dtype, rows, device, lo, hi):
-    """A sampling parameter: (scalar, pointer).  A number, checked; or a [rows] tensor, read on the device."""
+    """A sampling parameter: (scalar, pointer, the tensor to keep).  A number, checked; or a [rows] tensor, read on the device."""
     if isinstance(v, torch.Tensor):
         if v.dtype != dtype or v.shape != (rows,) or v.device != device:
             raise RuntimeError(f"sample_tokens: {name} must be a number or a [{rows}] {dtype} tensor on {device}, got {tuple(v.shape)} "
@@ -817,12 +825,14 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=0.0, min_p=0.0, out
     u [rows] fp32 random numbers in [0, 1).  temperature 0: the largest logit; top_k 0, top_p 0 or 1, min_p 0: off (the
     reference's defaults).  Each parameter is a number or a [rows] tensor (fp32; top_k int32).  Returns int64 [rows] (`out` if
     given); -1 for a row with a NaN or of nothing but -inf.  The order, ties and borders are defined in include/mm_hip.h."""
-    if logits.dim() != 2 or not logits.is_cuda or logits.size(1) < 1:
-        raise RuntimeError(f"sample_tokens: logits must be a GPU tensor [rows, vocab], got {tuple(logits.shape)} on {logits.device}")
-    rows, vocab = logits.shape
-    dev = logits.device
-    if logits.stride(1) != 1 and vocab > 1:
+    shape, dev = logits.shape, logits.device
+    if len(shape) != 2 or not logits.is_cuda or shape[1] < 1:
+        raise RuntimeError(f"sample_tokens: logits must be a GPU tensor [rows, vocab], got {tuple(shape)} on {dev}")
+    rows, vocab = shape
+    stride = logits.stride()
+    if stride[1] != 1:
         logits = logits.contiguous()
+        stride = logits.stride()
     if u.shape != (rows,) or u.dtype != torch.float32 or u.device != dev:
         raise RuntimeError(f"sample_tokens: u must be a [{rows}] fp32 tensor on {dev}, got {tuple(u.shape)} {u.dtype} on {u.device}")
     u = u.contiguous()
@@ -834,6 +844,6 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=0.0, min_p=0.0, out
     k, kv, k_ = _per_row("top_k", top_k, torch.int32, rows, dev, 0, 2 ** 31 - 1)
     p, pv, p_ = _per_row("top_p", top_p, torch.float32, rows, dev, 0.0, 1.0)
     m, mv, m_ = _per_row("min_p", min_p, torch.float32, rows, dev, 0.0, 1.0)
-    check(_launch(dev, get_lib().mm_sample_tokens, out.data_ptr(), logits.data_ptr(), logits.stride(0), u.data_ptr(), rows, vocab, t, tv,
-                  k, kv, p, pv, m, mv, dtype_code(logits.dtype)), "sample_tokens")
+    check(_launch(dev, get_lib().mm_sample_tokens, out.data_ptr(), logits.data_ptr(), stride[0], u.data_ptr(), rows, vocab, t, tv, k, kv, p,
+                  pv, m, mv, dtype_code(logits.dtype)), "sample_tokens")
     return out
