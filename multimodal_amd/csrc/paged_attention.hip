@@ -151,7 +151,7 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_few_k(const PagedAttnArgs 
     int pid[2];
     uint32_t at[2];    // bytes from the page's start to this lane's key of sub-tile t
     uint32_t bad = 0;  // bit t: it is in a page the cache does not have
-    auto fetch_pid = [&]() {  // page ids of the cursor's keys; the cursor moves on to the next tile
+    auto fetch_pid = [&]() __attribute__((always_inline)) {  // page ids of the cursor's keys; the cursor moves on to the next tile
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             pid[t] = bt[min(cur[t].page, last_page)];
@@ -159,7 +159,7 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_few_k(const PagedAttnArgs 
             cur[t].move(stride, page_bytes);
         }
     };
-    auto fetch = [&]() {  // keys and values of the tile whose page ids are here
+    auto fetch = [&]() __attribute__((always_inline)) {  // keys and values of the tile whose page ids are here
         bad = 0;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -334,22 +334,31 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_few_k(const PagedAttnArgs 
 
 // =====================================================================================  many rows
 // Bound by the matrix unit and the softmax's vector work, as the training forward (attention.hip), whose tile walk it shares: a
-// workgroup of 4 waves owns 128 rows, a wave 32 of them on the lane index of mfma 32x32x16 score tiles; keys and values come
-// in 64-key tiles, global -> registers -> double-buffered LDS, one barrier a tile; page ids are fetched a tile further ahead, so
-// that no load waits for another.  Row blocks with the most keys start first.
-template <typename T, int HD>
-__global__ __launch_bounds__(256, (HD == 64 ? 3 : 2)) void paged_attn_many_k(const PagedAttnArgs a) {
-    typedef Tile<HD> TL;
+// wave owns 32 rows on the lane index of mfma 32x32x16 score tiles; keys and values come in 64-key tiles, global -> registers ->
+// double-buffered LDS, one barrier a tile; page ids are fetched a tile further ahead, so that no load waits for another.  Row
+// blocks with the most keys start first.
+// LDS rows are unpadded; the 16-byte chunks of a row are XOR-ed with the row so that the row reads (16 rows, one chunk) and the
+// transposed reads (4 rows, 4 chunks) both meet all banks once.
+template <int HD> struct KvTile {
+    static constexpr int ROWB = HD * 2, BYTES = 64 * ROWB, CPR = HD / 8;
+    static __device__ __forceinline__ int swz(int row) {
+        if constexpr (HD == 64) return (((row >> 1) & 1) << 2) | ((row >> 1) & 2) | ((row >> 3) & 1);
+        else return ((row & 3) << 2) | ((row >> 2) & 3);
+    }
+    static __device__ __forceinline__ int off(int row, int chunk) { return row * ROWB + ((chunk ^ swz(row)) << 4); }
+};
+
+template <typename T, int HD, int NWV>
+__global__ __launch_bounds__(64 * NWV, (HD == 64 ? 3 : 2)) void paged_attn_many_k(const PagedAttnArgs a) {
+    typedef KvTile<HD> TL;
     typedef typename M32<T>::frag frag;
-    constexpr int NDS = HD / 16, NDB = HD / 32, NCH = TL::NCH;
-    // per ring slot (tile & 3) two 64-bit key masks: pages the cache does not have, values taken out as non-finite.  Head size 128
-    // keeps them in the padding of the first LDS row (two workgroups fill a CU's LDS to the byte).
-    constexpr int FLAGS = HD == 128 ? 2 * HD : 4 * TL::BYTES;
-    __shared__ __attribute__((aligned(16))) char smem[4 * TL::BYTES + (HD == 128 ? 0 : 64)];  // [buf][K | V]
-    unsigned long long* flags = reinterpret_cast<unsigned long long*>(smem + FLAGS);  // [slot][page | value]
+    constexpr int NDS = HD / 16, NDB = HD / 32, NT = 64 * NWV, NCH = 64 * TL::CPR / NT, ROWS = 32 * NWV;
+    // two stages of K | V, then per ring slot (tile & 3) two 64-bit key masks: pages the cache does not have, values taken out
+    __shared__ __attribute__((aligned(16))) char smem[4 * TL::BYTES + 64];
+    unsigned long long* flags = reinterpret_cast<unsigned long long*>(smem + 4 * TL::BYTES);  // [slot][page | value]
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 31, hh = lane >> 5;
     const int nkv = a.kv.heads, seq = blockIdx.x / nkv, kh = blockIdx.x % nkv, split = blockIdx.z;
-    const int r0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * 128;
+    const int r0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * ROWS;
     SeqInfo s;
     if (!seq_info<HD>(a, seq, kh, blockIdx.y == 0 && split == 0, s)) return;
     const int R = s.n * a.group;
@@ -368,7 +377,7 @@ __global__ __launch_bounds__(256, (HD == 64 ? 3 : 2)) void paged_attn_many_k(con
 
     const int wr0 = r0 + wave * 32;
     const int blk_first = past + (int)fdiv((uint32_t)r0, a.grp);
-    const int blk_last = past + (int)fdiv((uint32_t)min(r0 + 127, R - 1), a.grp);
+    const int blk_last = past + (int)fdiv((uint32_t)min(r0 + ROWS - 1, R - 1), a.grp);
     const int wave_first = past + (int)fdiv((uint32_t)min(wr0, R - 1), a.grp);
     const int wave_last = wr0 < R ? past + (int)fdiv((uint32_t)min(wr0 + 31, R - 1), a.grp) : -1;
     const int c1 = min(c0 + a.chunk, blk_last + 1);
@@ -376,7 +385,8 @@ __global__ __launch_bounds__(256, (HD == 64 ? 3 : 2)) void paged_attn_many_k(con
 
     const int32_t* bt = a.st.block_table + (int64_t)seq * a.st.table_stride;
     const int trow = tid / TL::CPR, tch = tid % TL::CPR;  // this thread's first row and its 16-byte chunk of a tile
-    constexpr int RSTEP = 256 / TL::CPR;
+    constexpr int RSTEP = NT / TL::CPR;
+    const int st0 = TL::off(trow, tch);  // RSTEP is a multiple of 16 rows: the swizzle of all the thread's rows is the same
     const char* kb = (const char*)((const u16*)a.kv.k + (int64_t)kh * a.kv.head + tch * 8);
     const int64_t k_to_v = (const char*)a.kv.v - (const char*)a.kv.k;
     const uint32_t page_stride = 2 * (uint32_t)a.kv.page, slot_bytes = 2 * (uint32_t)a.kv.slot, page_bytes = slot_bytes * a.page.d;
@@ -387,7 +397,7 @@ __global__ __launch_bounds__(256, (HD == 64 ? 3 : 2)) void paged_attn_many_k(con
     int pid[NCH];
     uint32_t at[NCH];
     uint32_t bad = 0;
-    auto fetch_pid = [&]() {  // page ids of the cursor's keys; the cursor moves on to the next tile
+    auto fetch_pid = [&]() __attribute__((always_inline)) {  // page ids of the cursor's keys; the cursor moves on to the next tile
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             pid[i] = bt[min(pos[i].page, last_page)];
@@ -395,7 +405,7 @@ __global__ __launch_bounds__(256, (HD == 64 ? 3 : 2)) void paged_attn_many_k(con
             pos[i].move(stride, page_bytes);
         }
     };
-    auto fetch = [&]() {  // keys and values of the tile whose page ids are here
+    auto fetch = [&]() __attribute__((always_inline)) {  // keys and values of the tile whose page ids are here
         bad = 0;
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
@@ -408,7 +418,7 @@ __global__ __launch_bounds__(256, (HD == 64 ? 3 : 2)) void paged_attn_many_k(con
     };
     // registers -> LDS stage of tile j; where some row of the block does not see the whole tile, the values behind the end become
     // zero and the non-finite ones are taken out and noted
-    auto put = [&](char* ks, int j) {
+    auto put = [&](char* ks, int j) __attribute__((always_inline)) {
         const int kv0 = c0 + j * 64;
         unsigned long long* fl = flags + 2 * (j & 3);
         if (kv0 + 63 > blk_first) {
@@ -424,8 +434,11 @@ __global__ __launch_bounds__(256, (HD == 64 ? 3 : 2)) void paged_attn_many_k(con
             for (int i = 0; i < NCH; ++i)
                 if ((bad >> i) & 1) atomicOr(fl, 1ull << (trow + RSTEP * i));
         }
-        tile_store<HD>(ks, kreg, tid);
-        tile_store<HD>(ks + TL::BYTES, vreg, tid);
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            *reinterpret_cast<u32x4*>(ks + st0 + i * RSTEP * TL::ROWB) = kreg[i];
+            *reinterpret_cast<u32x4*>(ks + TL::BYTES + st0 + i * RSTEP * TL::ROWB) = vreg[i];
+        }
     };
 
     f32x16 o[NDB];
@@ -449,7 +462,21 @@ __global__ __launch_bounds__(256, (HD == 64 ? 3 : 2)) void paged_attn_many_k(con
 #pragma unroll
     for (int ds = 0; ds < NDS; ++ds) pin(qf[ds]);
 
-    auto tile_step = [&](const int j, auto parity) {
+    // this lane's fragments: row reads of K (chunk 2 ds + hh of row r), transposed reads of V (as tr_frag in mfma32.h)
+    const int ka0 = TL::off(r, hh);
+    const int tg = lane >> 4, tq = (lane & 15) >> 2, tp = lane & 3;
+    const int va0 = TL::off(4 * hh + tq, 2 * (tg & 1) + (tp >> 1)) + (tp & 1) * 8;
+    auto k_frag = [&](const char* ks, int t, int ds) __attribute__((always_inline)) -> frag { return *reinterpret_cast<const frag*>(ks + ((ka0 ^ (ds << 5)) + t * 32 * TL::ROWB)); };
+    auto v_frag = [&](const char* vs, int kb16, int d) __attribute__((always_inline)) -> frag {  // keys kb16 .. kb16 + 15 (a multiple of 16), dims 32 d .. 32 d + 31
+        // rows 8 further on flip one bit of the swizzle (row bit 3): bit 1 of the chunk at head size 128, bit 0 at 64
+        const char* pa = vs + ((va0 ^ (d << 6)) + kb16 * TL::ROWB);
+        const char* pb = vs + ((va0 ^ (d << 6) ^ (HD == 64 ? 16 : 32)) + (kb16 + 8) * TL::ROWB);
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)pa);
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)pb);
+        const s16x8 v = s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        return __builtin_bit_cast(frag, v);
+    };
+    auto tile_step = [&](const int j, auto parity) __attribute__((always_inline)) {
         constexpr int cur = decltype(parity)::value;
         const char* ks = smem + cur * 2 * TL::BYTES;
         const char* vs = ks + TL::BYTES;
@@ -469,7 +496,7 @@ __global__ __launch_bounds__(256, (HD == 64 ? 3 : 2)) void paged_attn_many_k(con
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sacc[t][i] = 0.f;
 #pragma unroll
-                for (int ds = 0; ds < NDS; ++ds) sacc[t] = M32<T>::run(row_frag<T, HD>(ks, 32 * t, ds, lane), qf[ds], sacc[t]);
+                for (int ds = 0; ds < NDS; ++ds) sacc[t] = M32<T>::run(k_frag(ks, t, ds), qf[ds], sacc[t]);
             }
             __builtin_amdgcn_s_setprio(0);
             if (badk[0] | badk[1]) {
@@ -524,7 +551,7 @@ __global__ __launch_bounds__(256, (HD == 64 ? 3 : 2)) void paged_attn_many_k(con
                                                  sacc[t][8 * s2 + 4], sacc[t][8 * s2 + 5], sacc[t][8 * s2 + 6], sacc[t][8 * s2 + 7]);
 #pragma unroll
                     for (int d = 0; d < NDB; ++d)
-                        o[d] = M32<T>::run(tr_frag<T, HD>(vs, 32 * t + 16 * s2, d, lane), pf, o[d]);
+                        o[d] = M32<T>::run(v_frag(vs, 32 * t + 16 * s2, d), pf, o[d]);
                 }
             __builtin_amdgcn_s_setprio(0);
             if (nonf[0] | nonf[1]) {
@@ -617,18 +644,23 @@ template <typename T, int HD> __global__ __launch_bounds__(256) void paged_attn_
 // ---- launch plan, from the step's bounds alone (a captured step keeps it)
 struct PagedPlan {
     bool few;
-    int chunk, nsplit, row_blocks;
+    int waves, chunk, nsplit, row_blocks;
 };
 constexpr int kFewRows = 16, kFewWaves = 4;
 static PagedPlan plan(const mm_paged_kv& kv, const mm_paged_step& st, int nq) {
     PagedPlan p;
     const int group = nq / kv.heads;
-    p.few = (int64_t)st.max_new * group <= kFewRows;
-    p.row_blocks = p.few ? 1 : (int)(((int64_t)st.max_new * group + 127) / 128);
-    // Split the keys while the launch has too few workgroups to fill 256 CUs: few-row workgroups are small (target 4 a CU), and no
-    // split is shorter than 4 tiles per wave; many-row ones take 2 a CU and at least 8 tiles.
+    const int64_t rows = (int64_t)st.max_new * group;
+    p.few = rows <= kFewRows;
+    // Many rows: 128 a workgroup.  At head size 128 the registers hold two waves a SIMD whatever the workgroup's size, and one of 8
+    // waves fetches each tile once for 256 rows: 1024 tokens over 17k, 32 / 8 heads: 337 -> 314 us.  At 64 three waves a SIMD fit,
+    // which 8-wave workgroups cannot use: 59 us against 70 (4 x 2048 tokens, 16 heads).
+    p.waves = p.few ? kFewWaves : kv.hn == 128 && rows > 128 ? 8 : 4;
+    p.row_blocks = p.few ? 1 : (int)((rows + 32 * p.waves - 1) / (32 * p.waves));
+    // Split the keys while the launch has too few workgroups to fill 256 CUs: few-row workgroups are small (target 4 a CU, at least 4
+    // tiles per wave), many-row ones take 8 waves a CU and at least 8 tiles.
     const int64_t wgs = (int64_t)st.seqs * kv.heads * p.row_blocks;
-    const int target = p.few ? 1024 : 512, gran = p.few ? 32 * kFewWaves : 64, least = p.few ? 512 : 512;
+    const int target = p.few ? 1024 : 2048 / p.waves, gran = p.few ? 32 * kFewWaves : 64, least = 512;
     int64_t ns = wgs > 0 ? target / wgs : 1;
     const int64_t cap = (st.max_kv + least - 1) / least;
     if (ns > cap) ns = cap;
@@ -644,7 +676,8 @@ static PagedPlan plan(const mm_paged_kv& kv, const mm_paged_step& st, int nq) {
 template <typename T, int HD> static int launch_paged_attn(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
     const unsigned bx = (unsigned)(a.st.seqs * a.kv.heads);
     if (p.few) paged_attn_few_k<T, HD, kFewWaves><<<dim3(bx, p.nsplit), kFewWaves * 64, 0, st>>>(a);
-    else paged_attn_many_k<T, HD><<<dim3(bx, p.row_blocks, p.nsplit), 256, 0, st>>>(a);
+    else if (HD == 128 && p.waves == 8) paged_attn_many_k<T, 128, 8><<<dim3(bx, p.row_blocks, p.nsplit), 512, 0, st>>>(a);
+    else paged_attn_many_k<T, HD, 4><<<dim3(bx, p.row_blocks, p.nsplit), 256, 0, st>>>(a);
     MM_CHECK_LAUNCH();
     if (p.nsplit > 1) {
         paged_attn_join_k<T, HD><<<(unsigned)(((int64_t)a.rows * a.nq + 3) / 4), 256, 0, st>>>(a);
