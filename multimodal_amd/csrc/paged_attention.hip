@@ -30,12 +30,14 @@ struct PagedAttnArgs {
     int nq, group, rows;
     float scale_log2e;
     FastDiv page, grp;
-    int chunk, nsplit;  // keys per split (a multiple of the kernels' tiles), splits
-    float *ws_o, *ws_ml;  // nsplit > 1: [nsplit, rows, nq, hn] unnormalised outputs, [nsplit, rows, nq, 2] (max, sum)
+    int few_chunk, few_splits, many_chunk, many_splits;  // keys per split (a multiple of the tiles) and splits, by kind of sequence
+    float *ws_o, *ws_ml;  // more than one split: [splits, rows, nq, hn] unnormalised outputs, [splits, rows, nq, 2] (max, sum)
 };
 
 // How far a score may exceed the running reference of a row's exponentials (in powers of two) before the row is rescaled
 constexpr float kLag = 8.f;
+
+constexpr int kFewRows = 16;  // sequences with at most so many rows per key head take the few-row form
 
 // {first row, new rows, length} of a sequence; false: nothing to do
 struct SeqInfo {
@@ -114,22 +116,37 @@ template <int HD> __device__ __forceinline__ int v_off(int row, int byte) {
     return row * (HD * 2) + ((unit ^ swz) << 5) + (byte & 31);
 }
 
+template <int HD, int NW> constexpr int few_lds() {  // V tiles; then floats of the final exchange; rows' maxima and sums
+    return (NW * 32 * HD * 2 > NW * 16 * (HD + 4) * 4 ? NW * 32 * HD * 2 : NW * 16 * (HD + 4) * 4) + 2 * NW * 16 * 4;
+}
+// The page ids of a wave's first tile: they need nothing but the block table, so their load goes out with those of the sequence's
+// rows and length.
+template <int NW> struct FewStart {
+    PageCursor cur[2];
+    int pid[2];
+    __device__ __forceinline__ FewStart(const PagedAttnArgs& a, int seq, int split) {
+        const int32_t* bt = a.st.block_table + (int64_t)seq * a.st.table_stride;
+        const int key = split * a.few_chunk + (int)scalar(threadIdx.x >> 6) * 32 + (threadIdx.x & 15);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            cur[t].set((uint32_t)(key + 16 * t), a.page, 2 * (uint32_t)a.kv.slot);
+            pid[t] = bt[min(cur[t].page, (uint32_t)a.st.max_pages - 1)];
+        }
+    }
+};
 template <typename T, int HD, int NW>
-__global__ __launch_bounds__(NW * 64) void paged_attn_few_k(const PagedAttnArgs a) {
+__device__ __forceinline__ void paged_attn_few(const PagedAttnArgs& a, char* smem, const SeqInfo& s, int seq, int kh, int split,
+                                               FewStart<NW>& start) {
     typedef typename M16<T>::frag frag;
     constexpr int NC = HD / 32;  // 16-byte chunks of a key per lane = k-steps of Q K^T
     constexpr int NDB = HD / 16;
     constexpr int VB = 32 * HD * 2, RS = HD + 4;  // bytes of a wave's V tile; floats per row of the final exchange
-    constexpr int SM = NW * VB > NW * 16 * RS * 4 ? NW * VB : NW * 16 * RS * 4;
-    __shared__ __attribute__((aligned(16))) char smem[SM];
-    __shared__ float sm_m[NW][16], sm_l[NW][16];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 15, g = lane >> 4;
-    const int nkv = a.kv.heads, seq = blockIdx.x / nkv, kh = blockIdx.x % nkv, split = blockIdx.y;
-    SeqInfo s;
-    if (!seq_info<HD>(a, seq, kh, split == 0, s)) return;
+    float (*sm_m)[16] = reinterpret_cast<float (*)[16]>(smem + few_lds<HD, NW>() - 2 * NW * 16 * 4);
+    float (*sm_l)[16] = sm_m + NW;
+    const int tid = threadIdx.x, wave = (int)scalar(tid >> 6), lane = tid & 63, r = lane & 15, g = lane >> 4;
     const int R = s.n * a.group;
-    const int c0 = split * a.chunk, c1 = min(c0 + a.chunk, s.len);
-    if (split > 0 && c0 >= s.len) return;  // the combining kernel knows
+    const int c0 = split * a.few_chunk, c1 = min(c0 + a.few_chunk, s.len);
+    if (split > 0 && c0 >= s.len) return;  // the joining kernel knows
 
     const int rc = r < R ? r : R - 1;
     const int tok = (int)fdiv((uint32_t)rc, a.grp), qh = kh * a.group + rc - tok * a.group;
@@ -144,20 +161,25 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_few_k(const PagedAttnArgs 
     const int64_t k_to_v = (const char*)a.kv.v - (const char*)a.kv.k;
     const uint32_t page_stride = 2 * (uint32_t)a.kv.page, slot_bytes = 2 * (uint32_t)a.kv.slot, page_bytes = slot_bytes * a.page.d;
     const PageStep stride = page_step(NW * 32, a.page, slot_bytes);
-    const uint32_t last_page = s.len > 0 ? fdiv((uint32_t)s.len - 1, a.page) : 0;  // behind it the table is not the sequence's
+    // Behind a sequence's end its table may hold anything: the keys there are fetched from a page that exists and masked.
+    const uint32_t last_page = (uint32_t)a.st.max_pages - 1;
 
     u32x4 kr[2][NC], vr[2][NC];
-    PageCursor cur[2];
-    int pid[2];
+    PageCursor (&cur)[2] = start.cur;
+    int (&pid)[2] = start.pid;
     uint32_t at[2];    // bytes from the page's start to this lane's key of sub-tile t
     uint32_t bad = 0;  // bit t: it is in a page the cache does not have
-    auto fetch_pid = [&]() __attribute__((always_inline)) {  // page ids of the cursor's keys; the cursor moves on to the next tile
+    auto move_on = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            pid[t] = bt[min(cur[t].page, last_page)];
             at[t] = cur[t].byte;
             cur[t].move(stride, page_bytes);
         }
+    };
+    auto fetch_pid = [&]() __attribute__((always_inline)) {  // page ids of the cursor's keys; the cursor moves on to the next tile
+#pragma unroll
+        for (int t = 0; t < 2; ++t) pid[t] = bt[min(cur[t].page, last_page)];
+        move_on();
     };
     auto fetch = [&]() __attribute__((always_inline)) {  // keys and values of the tile whose page ids are here
         bad = 0;
@@ -182,9 +204,7 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_few_k(const PagedAttnArgs 
 
     int kt = c0 + wave * 32;
     if (kt < c1) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) cur[t].set((uint32_t)(kt + 16 * t + r), a.page, slot_bytes);
-        fetch_pid();
+        move_on();
         fetch();
         fetch_pid();
     }
@@ -313,7 +333,7 @@ __global__ __launch_bounds__(NW * 64) void paged_attn_few_k(const PagedAttnArgs 
             for (int e = 0; e < 8; ++e) acc[e] += al * src[e];
         }
         const int t = (int)fdiv((uint32_t)row, a.grp), h = kh * a.group + row - t * a.group, grow = s.beg + t;
-        if (a.nsplit == 1) {
+        if (a.few_splits == 1) {
             const float inv = L == 0.f ? 0.f : 1.0f / L;
 #pragma unroll
             for (int e = 0; e < 8; ++e) acc[e] *= inv;
@@ -348,23 +368,20 @@ template <int HD> struct KvTile {
     static __device__ __forceinline__ int off(int row, int chunk) { return row * ROWB + ((chunk ^ swz(row)) << 4); }
 };
 
+template <int HD> constexpr int many_lds() { return 4 * KvTile<HD>::BYTES + 64; }
 template <typename T, int HD, int NWV>
-__global__ __launch_bounds__(64 * NWV, (HD == 64 ? 3 : 2)) void paged_attn_many_k(const PagedAttnArgs a) {
+__device__ __forceinline__ void paged_attn_many(const PagedAttnArgs& a, char* smem, const SeqInfo& s, int seq, int kh, int row_block, int split) {
     typedef KvTile<HD> TL;
     typedef typename M32<T>::frag frag;
     constexpr int NDS = HD / 16, NDB = HD / 32, NT = 64 * NWV, NCH = 64 * TL::CPR / NT, ROWS = 32 * NWV;
     // two stages of K | V, then per ring slot (tile & 3) two 64-bit key masks: pages the cache does not have, values taken out
-    __shared__ __attribute__((aligned(16))) char smem[4 * TL::BYTES + 64];
     unsigned long long* flags = reinterpret_cast<unsigned long long*>(smem + 4 * TL::BYTES);  // [slot][page | value]
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, r = lane & 31, hh = lane >> 5;
-    const int nkv = a.kv.heads, seq = blockIdx.x / nkv, kh = blockIdx.x % nkv, split = blockIdx.z;
-    const int r0 = ((int)gridDim.y - 1 - (int)blockIdx.y) * ROWS;
-    SeqInfo s;
-    if (!seq_info<HD>(a, seq, kh, blockIdx.y == 0 && split == 0, s)) return;
+    const int tid = threadIdx.x, wave = (int)scalar(tid >> 6), lane = tid & 63, r = lane & 31, hh = lane >> 5;
+    const int r0 = row_block * ROWS;
     const int R = s.n * a.group;
     if (r0 >= R) return;
-    const int c0 = split * a.chunk;
-    if (split > 0 && c0 >= s.len) return;  // the combining kernel knows
+    const int c0 = split * a.many_chunk;
+    if (split > 0 && c0 >= s.len) return;  // the joining kernel knows
 
     const int past = s.len - s.n;
     const int row = r0 + wave * 32 + r, rc = row < R ? row : R - 1;
@@ -380,7 +397,7 @@ __global__ __launch_bounds__(64 * NWV, (HD == 64 ? 3 : 2)) void paged_attn_many_
     const int blk_last = past + (int)fdiv((uint32_t)min(r0 + ROWS - 1, R - 1), a.grp);
     const int wave_first = past + (int)fdiv((uint32_t)min(wr0, R - 1), a.grp);
     const int wave_last = wr0 < R ? past + (int)fdiv((uint32_t)min(wr0 + 31, R - 1), a.grp) : -1;
-    const int c1 = min(c0 + a.chunk, blk_last + 1);
+    const int c1 = min(c0 + a.many_chunk, blk_last + 1);
     const int ntiles = c1 > c0 ? (c1 - c0 + 63) >> 6 : 0;
 
     const int32_t* bt = a.st.block_table + (int64_t)seq * a.st.table_stride;
@@ -579,7 +596,7 @@ __global__ __launch_bounds__(64 * NWV, (HD == 64 ? 3 : 2)) void paged_attn_many_
     const float l_tot = half_sum(l_run);
     if (row >= R) return;
     const int grow = s.beg + tok;
-    if (a.nsplit == 1) {
+    if (a.many_splits == 1) {
         const float inv = l_tot == 0.f ? 0.f : 1.0f / l_tot;
         u16* orow = a.out + (int64_t)grow * a.o_row + (int64_t)qh * a.o_head;
 #pragma unroll
@@ -604,6 +621,34 @@ __global__ __launch_bounds__(64 * NWV, (HD == 64 ? 3 : 2)) void paged_attn_many_
     }
 }
 
+// =====================================================================================  the kernels
+// Every sequence has at most kFewRows rows (token steps).  Grid: (sequence, key head), split.
+template <typename T, int HD, int NW> __global__ __launch_bounds__(NW * 64) void paged_attn_few_k(const PagedAttnArgs a) {
+    __shared__ __attribute__((aligned(16))) char smem[few_lds<HD, NW>()];
+    const int seq = blockIdx.x / a.kv.heads, kh = blockIdx.x % a.kv.heads;
+    FewStart<NW> start(a, seq, blockIdx.y);
+    SeqInfo s;
+    if (seq_info<HD>(a, seq, kh, blockIdx.y == 0, s)) paged_attn_few<T, HD, NW>(a, smem, s, seq, kh, blockIdx.y, start);
+}
+// Any step: each sequence in the form its rows call for, so that single tokens next to a chunk of a prompt run at the cache's
+// bandwidth beside it.  Grid: (sequence, key head), then row blocks times splits - the row blocks with the most keys first.
+template <typename T, int HD, int NW>
+__global__ __launch_bounds__(NW * 64, (HD == 64 ? 3 : 2)) void paged_attn_any_k(const PagedAttnArgs a, int row_blocks) {
+    constexpr int LDS = few_lds<HD, NW>() > many_lds<HD>() ? few_lds<HD, NW>() : many_lds<HD>();
+    __shared__ __attribute__((aligned(16))) char smem[LDS];
+    const int seq = blockIdx.x / a.kv.heads, kh = blockIdx.x % a.kv.heads;
+    SeqInfo s;
+    if (!seq_info<HD>(a, seq, kh, blockIdx.y == 0, s)) return;
+    if (s.n * a.group <= kFewRows) {
+        if ((int)blockIdx.y >= a.few_splits) return;
+        FewStart<NW> start(a, seq, blockIdx.y);
+        paged_attn_few<T, HD, NW>(a, smem, s, seq, kh, blockIdx.y, start);
+    } else {
+        const int split = blockIdx.y / row_blocks, rb = blockIdx.y % row_blocks;
+        if (split < a.many_splits) paged_attn_many<T, HD, NW>(a, smem, s, seq, kh, row_blocks - 1 - rb, split);
+    }
+}
+
 // =====================================================================================  joining the splits
 // out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s, always in split order.  One wave per row and head.
 template <typename T, int HD> __global__ __launch_bounds__(256) void paged_attn_join_k(const PagedAttnArgs a) {
@@ -617,7 +662,10 @@ template <typename T, int HD> __global__ __launch_bounds__(256) void paged_attn_
     const int beg = a.st.cu_new[seq], end = a.st.cu_new[seq + 1], len = a.st.kv_lens[seq];
     // the rows the main kernel has handled itself (seq_info): nothing to join
     if (beg > row || beg < 0 || end > a.rows || end - beg > a.st.max_new || len > a.st.max_kv || len > a.st.max_pages * (int)a.page.d) return;
-    const int ns = min(a.nsplit, max(1, (len + a.chunk - 1) / a.chunk));
+    const bool few = (end - beg) * a.group <= kFewRows;
+    const int chunk = few ? a.few_chunk : a.many_chunk, splits = few ? a.few_splits : a.many_splits;
+    if (splits == 1) return;  // written by the main kernel
+    const int ns = min(splits, max(1, (len + chunk - 1) / chunk));
     const int64_t step = (int64_t)a.rows * a.nq;
     float M = -INFINITY, L = 0.f, acc[E];
 #pragma unroll
@@ -625,15 +673,30 @@ template <typename T, int HD> __global__ __launch_bounds__(256) void paged_attn_
     for (int i = lane; i < ns; i += 64) M = fmaxf(M, a.ws_ml[2 * (id + i * step)]);
     M = wave_max(M);
     const float mu = M == -INFINITY ? 0.f : M;
-    for (int i = 0; i < ns; ++i) {
-        const int64_t at = id + i * step;
-        const float m = a.ws_ml[2 * at], l = a.ws_ml[2 * at + 1];
-        if (m == -INFINITY && l == 0.f) continue;
-        const float al = fast_exp2(m - mu);
-        L += al * l;
+    for (int i0 = 0; i0 < ns; i0 += 64) {  // a lane has the factor of one split; the outputs of 8 splits are in flight
+        const int n = min(ns - i0, 64);
+        float w = 0.f;
+        if (lane < n) {
+            const float m = a.ws_ml[2 * (id + (i0 + lane) * step)], l = a.ws_ml[2 * (id + (i0 + lane) * step) + 1];
+            w = m == -INFINITY && l == 0.f ? 0.f : fast_exp2(m - mu);
+            L += w == 0.f && l == l ? 0.f : w * l;
+        }
+        for (int i = 0; i < n; i += 8) {
+            float v[8][E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += al * a.ws_o[at * HD + E * lane + e];
+            for (int u = 0; u < 8; ++u)
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[u][e] = a.ws_o[(id + min(i0 + i + u, ns - 1) * step) * HD + E * lane + e];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float f = __shfl(w, min(i + u, 63), 64);
+                if (i + u < n && f != 0.f)
+#pragma unroll
+                    for (int e = 0; e < E; ++e) acc[e] += f * v[u][e];
+            }
+        }
     }
+    L = wave_sum(L);
     const float inv = L == 0.f ? 0.f : 1.0f / L;
     u16* orow = a.out + (int64_t)row * a.o_row + (int64_t)h * a.o_head + E * lane;
     if constexpr (E == 2) *reinterpret_cast<uint32_t*>(orow) = pack2<T>(acc[0] * inv, acc[1] * inv);
@@ -644,42 +707,54 @@ template <typename T, int HD> __global__ __launch_bounds__(256) void paged_attn_
 // ---- launch plan, from the step's bounds alone (a captured step keeps it)
 struct PagedPlan {
     bool few;
-    int waves, chunk, nsplit, row_blocks;
+    int waves, row_blocks, few_chunk, few_splits, many_chunk, many_splits;
+    int splits() const { return few_splits > many_splits ? few_splits : many_splits; }
 };
-constexpr int kFewRows = 16, kFewWaves = 4;
+// Splits while a launch has too few workgroups: as many as keep one resident set (`target`), none shorter than `least` keys
+static void split_keys(int64_t wgs, int64_t target, int64_t least, int64_t gran, int max_kv, int& chunk, int& splits) {
+    int64_t ns = wgs > 0 ? target / wgs : 1;
+    const int64_t cap = (max_kv + least - 1) / least;
+    if (ns > cap) ns = cap;
+    if (ns < 1) ns = 1;
+    int64_t c = (max_kv + ns - 1) / ns;
+    c = (c + gran - 1) / gran * gran;
+    if (c < gran) c = gran;
+    chunk = (int)c;
+    splits = max_kv > 0 ? (int)((max_kv + c - 1) / c) : 1;
+}
 static PagedPlan plan(const mm_paged_kv& kv, const mm_paged_step& st, int nq) {
     PagedPlan p;
     const int group = nq / kv.heads;
-    const int64_t rows = (int64_t)st.max_new * group;
+    const int64_t rows = (int64_t)st.max_new * group, pairs = (int64_t)st.seqs * kv.heads;
     p.few = rows <= kFewRows;
+    // Few rows: one workgroup of 8 waves a CU.  With more, smaller ones the same bytes are in flight in more places at once: 2 x 131071
+    // keys of 4 heads of 128: 162 us with 1024 workgroups of 4 waves, 133 with 512, 112 with 256 of 8.
     // Many rows: 128 a workgroup.  At head size 128 the registers hold two waves a SIMD whatever the workgroup's size, and one of 8
     // waves fetches each tile once for 256 rows: 1024 tokens over 17k, 32 / 8 heads: 337 -> 314 us.  At 64 three waves a SIMD fit,
     // which 8-wave workgroups cannot use: 59 us against 70 (4 x 2048 tokens, 16 heads).
-    p.waves = p.few ? kFewWaves : kv.hn == 128 && rows > 128 ? 8 : 4;
+    p.waves = p.few || (kv.hn == 128 && rows > 128) ? 8 : 4;
     p.row_blocks = p.few ? 1 : (int)((rows + 32 * p.waves - 1) / (32 * p.waves));
-    // Split the keys while the launch has too few workgroups to fill 256 CUs: few-row workgroups are small (target 4 a CU, at least 4
-    // tiles per wave), many-row ones take 8 waves a CU and at least 8 tiles.
-    const int64_t wgs = (int64_t)st.seqs * kv.heads * p.row_blocks;
-    const int target = p.few ? 1024 : 2048 / p.waves, gran = p.few ? 32 * kFewWaves : 64, least = 512;
-    int64_t ns = wgs > 0 ? target / wgs : 1;
-    const int64_t cap = (st.max_kv + least - 1) / least;
-    if (ns > cap) ns = cap;
-    if (ns < 1) ns = 1;
-    int64_t chunk = (st.max_kv + ns - 1) / ns;
-    chunk = (chunk + gran - 1) / gran * gran;
-    if (chunk < gran) chunk = gran;
-    p.chunk = (int)chunk;
-    p.nsplit = st.max_kv > 0 ? (int)((st.max_kv + chunk - 1) / chunk) : 1;
+    // A token step's split pays for its second launch (about 2 us) once a workgroup's keys and values exceed 256 KB (one CU takes in
+    // some 130 GB/s): 700 keys of 64 in one piece 9.7 us, in two 11.2; 1023 of 128 in one 19, in two 15; 2047 of 64 in two 15, in
+    // four 11.7.  Beside chunks of prompts, whose rows the joining launch passes over too, from four times that.
+    p.few_chunk = (st.max_kv + 32 * p.waves - 1) / (32 * p.waves) * (32 * p.waves), p.few_splits = 1;
+    if ((int64_t)st.max_kv * kv.hn > (p.few ? 65536 : 262144)) split_keys(pairs, 2048 / p.waves, 512, 32 * p.waves, st.max_kv, p.few_chunk, p.few_splits);
+    p.many_chunk = 64, p.many_splits = 1;
+    if (!p.few) split_keys(pairs * p.row_blocks, 2048 / p.waves, 512, 64, st.max_kv, p.many_chunk, p.many_splits);
     return p;
 }
 
 template <typename T, int HD> static int launch_paged_attn(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
     const unsigned bx = (unsigned)(a.st.seqs * a.kv.heads);
-    if (p.few) paged_attn_few_k<T, HD, kFewWaves><<<dim3(bx, p.nsplit), kFewWaves * 64, 0, st>>>(a);
-    else if (HD == 128 && p.waves == 8) paged_attn_many_k<T, 128, 8><<<dim3(bx, p.row_blocks, p.nsplit), 512, 0, st>>>(a);
-    else paged_attn_many_k<T, HD, 4><<<dim3(bx, p.row_blocks, p.nsplit), 256, 0, st>>>(a);
+    const int many = p.row_blocks * p.many_splits;
+    const dim3 grid(bx, p.few ? p.few_splits : (p.few_splits > many ? p.few_splits : many));
+    if (p.few) paged_attn_few_k<T, HD, 8><<<grid, 512, 0, st>>>(a);
+    else if constexpr (HD == 128) {
+        if (p.waves == 8) paged_attn_any_k<T, 128, 8><<<grid, 512, 0, st>>>(a, p.row_blocks);
+        else paged_attn_any_k<T, 128, 4><<<grid, 256, 0, st>>>(a, p.row_blocks);
+    } else paged_attn_any_k<T, 64, 4><<<grid, 256, 0, st>>>(a, p.row_blocks);
     MM_CHECK_LAUNCH();
-    if (p.nsplit > 1) {
+    if (p.splits() > 1) {
         paged_attn_join_k<T, HD><<<(unsigned)(((int64_t)a.rows * a.nq + 3) / 4), 256, 0, st>>>(a);
         MM_CHECK_LAUNCH();
     }
@@ -689,7 +764,7 @@ template <typename T, int HD> static int launch_paged_attn(const PagedAttnArgs& 
 static int check_paged_attn(const char* fn, const mm_paged_kv* kv, const mm_paged_step* st, int nq, int rows) {
     if (int rc = check_paged(fn, kv, st, rows)) return rc;
     MM_CHECK_ARG(nq > 0 && nq % kv->heads == 0 && nq < 1 << 20, "%s: %d query heads are no multiple of %d key heads", fn, nq, kv->heads);
-    MM_CHECK_ARG((int64_t)st->max_new * (nq / kv->heads) < (int64_t)1 << 30 && (int64_t)st->max_new * (nq / kv->heads) / 128 < 65535,
+    MM_CHECK_ARG((int64_t)st->max_new * (nq / kv->heads) < (int64_t)1 << 30 && (int64_t)st->max_new * (nq / kv->heads) / 128 < 16000,
                  "%s: max_new=%d rows of %d heads exceed the grid limit", fn, st->max_new, nq);
     MM_CHECK_ARG((int64_t)st->seqs * kv->heads < (int64_t)1 << 31 && (int64_t)rows * nq < (int64_t)1 << 31,
                  "%s: %d sequences, %d rows exceed the grid limit", fn, st->seqs, rows);
@@ -704,7 +779,7 @@ using namespace mm;
 extern "C" size_t mm_paged_attn_workspace_bytes(const mm_paged_kv* kv, const mm_paged_step* step, int nq, int rows) {
     if (check_paged_attn("mm_paged_attn_workspace_bytes", kv, step, nq, rows) != MM_OK) return 0;
     const PagedPlan p = plan(*kv, *step, nq);
-    return p.nsplit == 1 ? 0 : (size_t)p.nsplit * rows * nq * (kv->hn + 2) * sizeof(float);
+    return p.splits() == 1 ? 0 : (size_t)p.splits() * rows * nq * (kv->hn + 2) * sizeof(float);
 }
 
 extern "C" int mm_paged_attn_fwd(const mm_paged_kv* kv, const mm_paged_step* step, void* out, int64_t o_row, int64_t o_head, float* lse,
@@ -718,7 +793,7 @@ extern "C" int mm_paged_attn_fwd(const mm_paged_kv* kv, const mm_paged_step* ste
                  "%s: q / out must be 16-byte aligned with strides a multiple of 8", fn);
     MM_CHECK_ARG(softmax_scale > 0.f, "%s: softmax_scale %g must be positive", fn, (double)softmax_scale);
     const PagedPlan p = plan(*kv, *step, nq);
-    const size_t need = p.nsplit == 1 ? 0 : (size_t)p.nsplit * rows * nq * (kv->hn + 2) * sizeof(float);
+    const size_t need = p.splits() == 1 ? 0 : (size_t)p.splits() * rows * nq * (kv->hn + 2) * sizeof(float);
     MM_CHECK_ARG(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need),
                  "%s: workspace of %zu bytes needed (16-byte aligned), got %zu", fn, need, workspace ? workspace_bytes : (size_t)0);
     PagedAttnArgs a{};
@@ -729,9 +804,9 @@ extern "C" int mm_paged_attn_fwd(const mm_paged_kv* kv, const mm_paged_step* ste
     a.nq = nq, a.group = nq / kv->heads, a.rows = rows;
     a.scale_log2e = softmax_scale * kLog2e;
     a.page = make_fastdiv(kv->page_size), a.grp = make_fastdiv(a.group);
-    a.chunk = p.chunk, a.nsplit = p.nsplit;
+    a.few_chunk = p.few_chunk, a.few_splits = p.few_splits, a.many_chunk = p.many_chunk, a.many_splits = p.many_splits;
     a.ws_o = (float*)workspace;
-    a.ws_ml = need ? a.ws_o + (size_t)p.nsplit * rows * nq * kv->hn : nullptr;
+    a.ws_ml = need ? a.ws_o + (size_t)p.splits() * rows * nq * kv->hn : nullptr;
     hipStream_t st = (hipStream_t)stream;
     return dispatch_dtype(kv->dtype, [&](auto t) -> int {
         using T = decltype(t);
