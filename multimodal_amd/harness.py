@@ -204,6 +204,12 @@ class MagmaStack(nn.Module):
         return Fn.masked_cross_entropy(logits, labels, loss_mask)
 
 
+    def generate(self, prompts, **kw):
+        """Continue token prompts (and images) over a paged key / value cache: generation.generate."""
+        from .generation import generate
+        return generate(self, prompts, **kw)
+
+
 def end_of_step():
     """Call once per training step after the backward: moves the device-resident dropout counters past this step's draws
     (one capturable launch), so that the next step - or the next replay of a captured step - draws fresh masks."""

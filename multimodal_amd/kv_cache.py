@@ -4,7 +4,8 @@ The reference keeps `[past | new]` keys and values of every layer in tensors tha
 layer_past, megatron/model/transformer.py:361-365, 602-610).  Here a layer's keys and values live in pages of `page_size`
 token slots; sequences take pages as they grow and give them back when they end, so nothing is copied and sequences of any
 lengths share one batch.  `PagedKV` is one layer's pages, `PagedStep` what one step of a batch brings; `ops.paged_kv_append`
-and `ops.paged_attn_fwd` work on a pair of them.
+and `ops.paged_attn_fwd` work on a pair of them.  `PagedKVCache` holds the pages of all layers and hands them out; a
+`PagedPast` of one of its layers is what `ParallelTransformerLayer.forward` takes as `layer_past`.
 """
 import ctypes
 
@@ -66,3 +67,72 @@ class PagedStep:
         self._c = MmPagedStep(block_table.data_ptr(), cu_new.data_ptr(), kv_lens.data_ptr(), block_table.stride(0), self.seqs,
                               block_table.size(1), self.max_new, self.max_kv)
         self._ref = ctypes.addressof(self._c)
+
+
+class PagedPast:
+    """`layer_past` of a layer in generation: its pages, the step, and how many positions a sequence can have (the length of the
+    rotary tables)."""
+
+    def __init__(self, kv, step, max_positions):
+        self.kv, self.step, self.max_positions = kv, step, int(max_positions)
+
+
+class PagedKVCache:
+    """Pages for all layers of a model, and the host side of handing them out.  num_heads: this tensor-parallel rank's."""
+
+    def __init__(self, num_layers, num_heads, head_size, num_pages, page_size=16, dtype=torch.bfloat16, device="cuda"):
+        if min(num_layers, num_heads, num_pages, page_size) < 1:
+            raise RuntimeError("PagedKVCache: layers, heads, pages and page_size must be positive")
+        pages = torch.empty(num_layers, 2, num_pages, num_heads, page_size, head_size, dtype=dtype, device=device)
+        self.layers = [PagedKV(pages[i, 0], pages[i, 1]) for i in range(num_layers)]
+        self.page_size, self.device = page_size, pages.device
+        self._free = list(range(num_pages - 1, -1, -1))
+        self._pages = {}   # sequence -> its pages, in order
+        self._next = 0
+
+    @property
+    def free_pages(self):
+        return len(self._free)
+
+    def add(self, tokens):
+        """A new sequence with room for `tokens` tokens; returns its handle."""
+        seq, self._next = self._next, self._next + 1
+        self._pages[seq] = []
+        try:
+            self.reserve(seq, tokens)
+        except RuntimeError:
+            del self._pages[seq]
+            raise
+        return seq
+
+    def reserve(self, seq, tokens):
+        """Room for `tokens` tokens in all; raises, and takes nothing, when the free pages do not suffice."""
+        pages = self._pages[seq]
+        need = -(-int(tokens) // self.page_size) - len(pages)
+        if need > len(self._free):
+            raise RuntimeError(f"PagedKVCache: {need} pages needed, {len(self._free)} free")
+        for _ in range(need):
+            pages.append(self._free.pop())
+
+    def release(self, seq):
+        """Give a sequence's pages back.  Work on the GPU that still reads them must have been enqueued on the stream of the work
+        that will write them next."""
+        self._free.extend(reversed(self._pages.pop(seq)))
+
+    def block_table(self, seqs):
+        """int32 [len(seqs), pages of the longest] on the device; entries behind a sequence's last page are -1."""
+        width = max([len(self._pages[s]) for s in seqs] + [1])
+        rows = [self._pages[s] + [-1] * (width - len(self._pages[s])) for s in seqs]
+        return torch.tensor(rows, dtype=torch.int32).view(len(seqs), width).to(self.device)
+
+    def step(self, seqs, new, lens):
+        """The step that brings new[i] rows to sequence seqs[i], whose length is lens[i] afterwards (host numbers)."""
+        for s, n, l in zip(seqs, new, lens):
+            if not 0 <= n <= l or l > len(self._pages[s]) * self.page_size:
+                raise RuntimeError(f"PagedKVCache: sequence {s} has room for {len(self._pages[s]) * self.page_size} tokens, not for "
+                                   f"{n} new ones up to {l}")
+        cu = [0]
+        for n in new:
+            cu.append(cu[-1] + int(n))
+        meta = torch.tensor(cu + [int(l) for l in lens], dtype=torch.int32).to(self.device)
+        return PagedStep(self.block_table(seqs), meta[:len(cu)], meta[len(cu):], max_new=max(list(new) + [0]), max_kv=max(list(lens) + [0]))

@@ -18,7 +18,8 @@ import torch
 import torch.nn as nn
 
 from .. import functional as Fn
-from .. import mpu
+from .. import mpu, ops
+from ..kv_cache import PagedPast
 from .fused_bias_dropout import (bias_dropout_add_fused_inference, bias_dropout_add_fused_train,
                                  get_bias_dropout_add)
 from .norms import LayerNorm, get_norm
@@ -74,7 +75,8 @@ class ParallelMLP(nn.Module):
 
 
 class ParallelSelfAttention(nn.Module):
-    """megatron/model/transformer.py:179-641 for pos_emb in {rotary, none}, global attention, no kv-cache."""
+    """megatron/model/transformer.py:179-641 for pos_emb in {rotary, none}, global attention.  Generation: a
+    kv_cache.PagedPast as `layer_past` takes the place of the reference's use_cache tensors."""
 
     def __init__(self, neox_args, attention_mask_func, init_method, output_layer_init_method, layer_number,
                  rpe=None, rotary=False, use_cache=False, parallel_output=False):
@@ -124,8 +126,10 @@ class ParallelSelfAttention(nn.Module):
             parallel_output=parallel_output)
 
     def forward(self, hidden_states, attention_mask, layer_past=None):
+        if isinstance(layer_past, PagedPast):
+            return self._forward_paged(hidden_states, attention_mask, layer_past)
         if self.use_cache or (exists(layer_past) and layer_past.numel() > 0):
-            raise NotImplementedError("kv-cache inference is outside this path's scope (training hot path only)")
+            raise NotImplementedError("a kv-cache is taken as layer_past=kv_cache.PagedPast, not as tensors grown by concatenation")
         s, b = hidden_states.size(0), hidden_states.size(1)
         np_, hn = self.num_attention_heads_per_partition, self.hidden_size_per_attention_head
         cos = sin = None
@@ -148,6 +152,27 @@ class ParallelSelfAttention(nn.Module):
         context = Fn.qkv_attention(x, qkv_lin.weight, qkv_lin.bias, cos, sin, mask, np_, hn, d,
                                    1.0 / self.norm_factor, dropout)  # [s, b, np*hn]
         return self.dense(context)
+
+    def _forward_paged(self, hidden_states, attention_mask, past):
+        """The step's packed rows [rows, 1, h] against the cache: QKV, append with rotation (the queries rotate in place),
+        attention, dense.  Always causal; no backward."""
+        if attention_mask is not None:
+            raise RuntimeError("attention over a paged cache is causal: pass attention_mask=None")
+        if torch.is_grad_enabled() and (hidden_states.requires_grad or self.query_key_value.weight.requires_grad):
+            raise RuntimeError("attention over a paged cache has no backward: run generation under torch.no_grad()")
+        if self.dropout_p > 0.0 and self.training:
+            raise RuntimeError("attention over a paged cache has no dropout: put the model in eval mode")
+        if hidden_states.size(1) != 1:
+            raise RuntimeError(f"attention over a paged cache takes packed rows [rows, 1, h], got {tuple(hidden_states.shape)}")
+        rows, np_, hn = hidden_states.size(0), self.num_attention_heads_per_partition, self.hidden_size_per_attention_head
+        mixed, _ = self.query_key_value(hidden_states)
+        q, k, v = mixed.view(rows, np_, 3, hn).unbind(2)
+        cos = sin = None
+        if exists(self.rotary_emb):
+            cos, sin = self.rotary_emb.tables(hidden_states, past.max_positions)
+        ops.paged_kv_append(past.kv, past.step, k, v, q=q, cos=cos, sin=sin, q_out=q)
+        context, _ = ops.paged_attn_fwd(past.kv, past.step, q, 1.0 / self.norm_factor)
+        return self.dense(context.view(rows, 1, np_ * hn))
 
 
 _SIDE_STREAMS = {}
@@ -214,7 +239,6 @@ class ParallelTransformerLayer(nn.Module):
         """(adapter Linear 0, Linear 2) when `.mlp` is an AdapterWrapper of a shape the fused adapter kernel takes
         (training.py:421-432 wraps `.mlp` / `.attention`), else None."""
         from .adapter import AdapterWrapper
-        from .. import ops
         m = self.mlp
         if type(m) is not AdapterWrapper:
             return None
@@ -248,14 +272,14 @@ class ParallelTransformerLayer(nn.Module):
             if tail is not None:
                 # MAGMA layer: the MLP's adapter is the last kernel, so the residual tail rides on its output store
                 a0, a2 = tail
-                if _branch_streams() and x2.is_cuda:
+                # (a generation step's few rows leave nothing to overlap)
+                if _branch_streams() and x2.is_cuda and layer_past is None:
                     # GPT-J parallel residual: the MLP GEMMs and the attention branch only meet in the tail, so they go to two
                     # HIP streams (the attention kernels are vector-bound, the GEMMs matrix-bound: they share a CU well)
                     main, side = torch.cuda.current_stream(), _side_stream(x2.device)
                     side.wait_stream(main)
                     # each branch's big GEMMs take half the CUs, so that the pair runs side by side instead of one persistent
                     # launch after the other (ops.cu_share; step 20.34 -> 19.40 ms on one box)
-                    from .. import ops
                     share_attn, share_mlp = _branch_shares(x2.device)
                     with ops.cu_share(share_mlp), torch.cuda.stream(side):
                         mlp_raw, mlp_bias = self.mlp.attn_block(x2)

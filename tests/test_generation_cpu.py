@@ -1,0 +1,120 @@
+"""Refusals of the generation entry points, before any device work: safe without a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+from multimodal_amd import _lib, ops
+from multimodal_amd._lib import MmPagedKV, MmPagedStep
+
+KV = dict(k=4096, v=8192, page=4 * 16 * 64, head=16 * 64, slot=64, num_pages=10, page_size=16, heads=4, hn=64, dtype=0)
+STEP = dict(block_table=4096, cu_new=4096, kv_lens=4096, table_stride=8, seqs=2, max_pages=8, max_new=1, max_kv=100)
+
+
+def refs(kv=(), step=()):
+    a, b = MmPagedKV(**{**KV, **dict(kv)}), MmPagedStep(**{**STEP, **dict(step)})
+    return a, b, ctypes.addressof(a), ctypes.addressof(b)
+
+
+def append(kv=(), step=(), k=4096, v=4096, q=4096, q_out=4096, nq=4, rows=2, cos=4096, sin=4096, d=16, positions=100):
+    a, b, pa, pb = refs(kv, step)
+    lib = _lib.get_lib()
+    return lib.mm_paged_kv_append(pa, pb, k, 256, 64, v, 256, 64, q, 256, 64, q_out, 256, 64, nq, rows, cos, sin, d, positions, 1, None), \
+        lib.mm_last_error().decode()
+
+
+def attend(kv=(), step=(), out=4096, lse=4096, q=4096, q_row=256, nq=4, rows=2, scale=0.125, ws=0, ws_bytes=0):
+    a, b, pa, pb = refs(kv, step)
+    lib = _lib.get_lib()
+    return lib.mm_paged_attn_fwd(pa, pb, out, 256, 64, lse, nq, q, q_row, 64, nq, rows, scale, ws, ws_bytes, None), \
+        lib.mm_last_error().decode()
+
+
+BAD_CACHE = [(dict(k=0), "null"), (dict(hn=96), "head size"), (dict(num_pages=0), "out of range"), (dict(page_size=0), "out of range"),
+             (dict(heads=-1), "out of range"), (dict(k=4100), "16-byte"), (dict(page=1 << 31), "stride"), (dict(head=12), "stride"),
+             (dict(slot=0), "stride"), (dict(slot=-64), "stride"), (dict(page_size=1 << 20, slot=4096), "slots span")]
+BAD_STEP = [(dict(block_table=0), "null"), (dict(cu_new=0), "null"), (dict(kv_lens=0), "null"), (dict(seqs=-1), "out of range"),
+            (dict(max_pages=0), "out of range"), (dict(max_pages=1 << 27, table_stride=1 << 27), "2^30"), (dict(max_new=-1), "out of range"),
+            (dict(max_kv=-1), "out of range"), (dict(table_stride=7), "out of range")]
+
+
+@pytest.mark.parametrize("call", [append, attend])
+def test_bad_caches_and_steps(call):
+    for bad, text in BAD_CACHE:
+        rc, msg = call(kv=bad)
+        assert rc == -1 and text in msg, (bad, rc, msg)
+    for bad, text in BAD_STEP:
+        rc, msg = call(step=bad)
+        assert rc == -1 and text in msg, (bad, rc, msg)
+
+
+def test_bad_append_arguments():
+    for bad, text in [(dict(k=0), "null"), (dict(v=0), "null"), (dict(q_out=0), "q_out"), (dict(nq=0), "head count"), (dict(d=15), "rotary"),
+                      (dict(d=66), "rotary"), (dict(d=-2), "rotary"), (dict(cos=0), "tables"), (dict(positions=0), "tables"), (dict(rows=-1), "out of range")]:
+        rc, msg = append(**bad)
+        assert rc == -1 and text in msg, (bad, rc, msg)
+    rc, msg = append(kv=dict(dtype=7))
+    assert rc == -2 and "dtype" in msg
+    assert append(rows=0)[0] == 0 and append(step=dict(seqs=0))[0] == 0  # nothing to do is no error
+
+
+def test_bad_attention_arguments():
+    for bad, text in [(dict(out=0), "null"), (dict(lse=0), "null"), (dict(q=0), "null"), (dict(nq=6), "multiple"), (dict(nq=0), "multiple"),
+                      (dict(q=4104), "aligned"), (dict(q_row=252), "aligned"), (dict(scale=0.0), "softmax_scale"), (dict(scale=float("nan")), "softmax_scale"),
+                      (dict(step=dict(max_kv=1 << 30)), "2^30"), (dict(step=dict(max_new=1 << 30)), "grid")]:
+        rc, msg = attend(**bad)
+        assert rc == -1 and text in msg, (bad, rc, msg)
+    assert attend(kv=dict(dtype=7))[0] == -2
+    assert attend(rows=0)[0] == 0 and attend(step=dict(max_new=0))[0] == 0
+
+
+def test_workspace_is_asked_for_and_checked():
+    a, b, pa, pb = refs(step=dict(max_kv=5000, max_pages=512, table_stride=512))
+    lib = _lib.get_lib()
+    need = lib.mm_paged_attn_workspace_bytes(pa, pb, 4, 2)
+    assert need > 0 and need % (2 * 4 * 66 * 4) == 0
+    for ws, n in ((0, need), (4096, need - 1), (4100, need)):
+        rc, msg = attend(step=dict(max_kv=5000, max_pages=512, table_stride=512), ws=ws, ws_bytes=n)
+        assert rc == -1 and "workspace" in msg
+    a, b, pa, pb = refs()
+    assert lib.mm_paged_attn_workspace_bytes(pa, pb, 4, 2) == 0          # short: in one piece
+    assert lib.mm_paged_attn_workspace_bytes(pa, pb, 5, 2) == 0          # not a call attention would take
+
+
+def test_bad_sampling_arguments():
+    lib = _lib.get_lib()
+
+    def call(tokens=4096, logits=4096, u=4096, rows=2, vocab=100, dtype=0):
+        return lib.mm_sample_tokens(tokens, logits, 128, u, rows, vocab, 1.0, None, 0, None, 0.0, None, 0.0, None, dtype, None), \
+            lib.mm_last_error().decode()
+    for bad, text in [(dict(tokens=0), "null"), (dict(logits=0), "null"), (dict(u=0), "null"), (dict(rows=-1), "out of range"),
+                      (dict(vocab=0), "out of range"), (dict(vocab=1 << 30), "out of range"), (dict(logits=4097), "aligned")]:
+        rc, msg = call(**bad)
+        assert rc == -1 and text in msg, (bad, rc, msg)
+    assert call(dtype=3)[0] == -2 and call(rows=0)[0] == 0
+
+
+def test_wrappers_refuse_cpu_tensors():
+    from multimodal_amd.kv_cache import PagedKV, PagedStep
+    k = torch.zeros(4, 2, 16, 64, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="GPU"):
+        PagedKV(k, k.clone())
+    i = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="one GPU"):
+        PagedStep(torch.zeros(1, 4, dtype=torch.int32), i, i[:1])
+    with pytest.raises(RuntimeError, match="GPU"):
+        ops.sample_tokens(torch.zeros(2, 100, dtype=torch.bfloat16), torch.zeros(2))
+
+
+@pytest.mark.parametrize("d", [1, 2, 3, 7, 8, 16, 24, 48, 63, 64, 100, 128, 1000, 65536, (1 << 20) + 1])
+def test_division_by_multiplication(d):
+    """The kernels' n / page_size: (mulhi(m, n) + n) >> l with l = ceil(log2 d), m = floor(2^32 (2^l - d) / d) + 1, exact below 2^31."""
+    l = (d - 1).bit_length()
+    m = (((1 << l) - d) << 32) // d + 1
+    assert m < 1 << 32
+    ns = {0, 1, d - 1, d, d + 1, (1 << 31) - 1, (1 << 30) - 1}
+    ns |= {k * d + e for k in (1, 2, 1000, ((1 << 31) - 1) // d) for e in (-1, 0, 1)}
+    for n in ns:
+        if 0 <= n < 1 << 31:
+            q = ((m * n) >> 32) + n
+            assert q < 1 << 32 and q >> l == n // d, (n, d)

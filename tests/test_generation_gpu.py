@@ -1,0 +1,151 @@
+"""Generation as it is used: append -> attention -> sampling through the layer and the stack, against the same model without a
+cache."""
+import pytest
+import torch
+
+from multimodal_amd import harness
+
+pytestmark = pytest.mark.gpu
+
+# Both sides round to bf16 at every stage (a rounding is off by at most 2^-8 of the value).  They differ in the rotation (three
+# roundings against one), the probabilities, the order of the sums and what follows from those: query, key, probability, context,
+# dense, adapters and the residual sums, some 13 roundings of values no larger than the row's largest.
+LAYER_TOL = 16 * 2.0 ** -8
+
+
+def build(name, seed=1, **over):
+    from multimodal_amd import mpu
+    mpu.destroy_model_parallel()
+    mpu.initialize_model_parallel(1)
+    mpu.model_parallel_cuda_manual_seed(seed)
+    torch.manual_seed(seed)
+    cfg = dict(harness.CONFIGS[name], **over)
+    stack = harness.MagmaStack(cfg).eval()
+    with torch.no_grad():  # adapters that do something
+        for n, p in stack.named_parameters():
+            if "adapter" in n:
+                p.normal_(0.0, 0.05)
+    return cfg, stack
+
+
+@pytest.mark.parametrize("name", ["tiny_magma", "tiny_1_3B", "tiny"])
+@pytest.mark.parametrize("chunks", [[70], [1] * 9, [33, 1, 1, 20, 1], [64, 64]])
+def test_layer_over_the_cache_equals_the_layer(name, chunks):
+    from multimodal_amd.kv_cache import PagedKVCache, PagedPast
+    cfg, stack = build(name)
+    layer, h, s = stack.layers[1], cfg["hidden_size"], sum(chunks)
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(s, 2, h, generator=g).bfloat16().cuda()
+    with torch.no_grad():
+        want = layer(x, stack.attention_mask(s, x.device))
+        heads = cfg["num_attention_heads"]
+        cache = PagedKVCache(1, heads, h // heads, 40, page_size=16)
+        seqs = [cache.add(s), cache.add(s)]
+        done, got = 0, []
+        for n in chunks:
+            step = cache.step(seqs, [n, n], [done + n] * 2)
+            rows = x[done:done + n].transpose(0, 1).reshape(2 * n, 1, h)  # packed: sequence 0's rows, then sequence 1's
+            y = layer(rows, None, layer_past=PagedPast(cache.layers[0], step, s))
+            got.append(y.view(2, n, h).transpose(0, 1))
+            done += n
+        got = torch.cat(got)
+    err = (got.float() - want.float()).abs().max() / want.float().abs().max()
+    assert err <= LAYER_TOL, f"{err}"
+
+
+def full_logits(stack, seq, enc=None):
+    """Logits of every position of one sequence, without a cache."""
+    with torch.no_grad():
+        pre = stack.image_prefix(enc).view(1, -1, stack.word_embeddings.weight.size(1)) if enc is not None else None
+        p = 0 if pre is None else pre.size(1)
+        from multimodal_amd import ops
+        tok = torch.cat((seq, torch.zeros(p, dtype=torch.int64))).view(1, -1).cuda()
+        x = ops.embed_prefix(stack.word_embeddings.weight, tok, pre)
+        mask = stack.attention_mask(x.size(0), x.device)
+        for layer in stack.layers:
+            x = layer(x, mask)
+        logits, _ = stack.final_linear(stack.final_norm(x))
+        return logits[:, 0].float().cpu(), p
+
+
+@pytest.mark.parametrize("name", ["tiny_magma", "tiny_1_3B"])
+@pytest.mark.parametrize("image", [False, True])
+def test_greedy_tokens_are_the_largest_logits_of_the_model_without_a_cache(name, image):
+    """Every token generated has, given the tokens before it, a logit within the two sides' rounding of the largest."""
+    cfg, stack = build(name)
+    g = torch.Generator().manual_seed(5)
+    prompts = [torch.randint(0, 1000, (n,), generator=g) for n in (7, 1, 30)]
+    enc = torch.randn(3, 1, cfg["encoder_out_dim"], generator=g).bfloat16().cuda() if image else None
+    out = stack.generate(prompts, enc_out=enc, maximum_tokens=20)
+    for i, (p, o) in enumerate(zip(prompts, out)):
+        assert o.shape == (20,)
+        logits, pl = full_logits(stack, torch.cat((p, o)), None if enc is None else enc[i:i + 1])
+        first = pl + len(p) - 1
+        for t in range(20):
+            row = logits[first + t]
+            # two layers' difference, then the head: hidden rows of unit variance within LAYER_TOL a layer
+            assert row[o[t]] >= row.max() - 2 * LAYER_TOL * row.abs().max(), (i, t)
+
+
+def test_generation_is_the_same_eagerly_replayed_and_for_any_paging():
+    cfg, stack = build("tiny_magma")
+    g = torch.Generator().manual_seed(6)
+    prompts = [torch.randint(0, 1000, (n,), generator=g) for n in (5, 17, 2, 40)]
+    enc = torch.randn(4, 1, cfg["encoder_out_dim"], generator=g).bfloat16().cuda()
+    run = lambda **kw: stack.generate(prompts, enc_out=enc, maximum_tokens=25, temperature=0.9, top_k=50, top_p=0.95, min_p=0.001,
+                                      vocab_size=1000, generator=torch.Generator("cuda").manual_seed(9), **kw)
+    ref = run(graph=False)
+    assert all(int(o.max()) < 1000 and int(o.min()) >= 0 for o in ref)
+    for kw in (dict(graph=True), dict(graph=True), dict(graph=False, page_size=24), dict(graph=True, page_size=64)):
+        got = run(**kw)
+        assert all(torch.equal(a, b) for a, b in zip(got, ref)), kw
+    # per-row parameters
+    t = torch.tensor([0.0, 0.9, 0.9, 0.0], device="cuda")
+    got = stack.generate(prompts, enc_out=enc, maximum_tokens=25, temperature=t, top_k=50, top_p=0.95, min_p=0.001, vocab_size=1000,
+                         generator=torch.Generator("cuda").manual_seed(9))
+    assert torch.equal(got[1], ref[1]) and torch.equal(got[2], ref[2])
+
+
+def test_end_of_text_and_the_pages_come_back():
+    from multimodal_amd.generation import make_cache
+    cfg, stack = build("tiny")
+    g = torch.Generator().manual_seed(7)
+    prompts = [torch.randint(0, 1000, (n,), generator=g) for n in (3, 9)]
+    free = stack.generate(prompts, maximum_tokens=40)
+    eos = int(free[0][5])
+    cut = stack.generate(prompts, maximum_tokens=40, eos_token_id=eos)
+    for f, c in zip(free, cut):
+        n = int((f == eos).nonzero()[0]) + 1 if bool((f == eos).any()) else 40
+        assert torch.equal(c, f[:n])
+    cache = make_cache(stack, 2, 64)
+    pages = cache.free_pages
+    a = stack.generate(prompts, maximum_tokens=10, cache=cache)
+    b = stack.generate(prompts, maximum_tokens=10, cache=cache)
+    assert cache.free_pages == pages and all(torch.equal(x, y) and torch.equal(x, f[:10]) for x, y, f in zip(a, b, free))
+    with pytest.raises(RuntimeError, match="pages needed"):
+        stack.generate(prompts, maximum_tokens=500, cache=cache)
+    assert cache.free_pages == pages
+    assert [len(x) for x in stack.generate(prompts, maximum_tokens=1)] == [1, 1]
+    assert [len(x) for x in stack.generate([], maximum_tokens=5)] == []
+
+
+def test_refusals_of_the_layer():
+    from multimodal_amd.kv_cache import PagedKVCache, PagedPast
+    cfg, stack = build("tiny")
+    layer, h = stack.layers[0], cfg["hidden_size"]
+    cache = PagedKVCache(1, 4, 64, 8)
+    step = cache.step([cache.add(10)], [10], [10])
+    past = PagedPast(cache.layers[0], step, 10)
+    x = torch.zeros(10, 1, h, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="no backward"):
+        layer(x, None, layer_past=past)
+    with torch.no_grad():
+        with pytest.raises(RuntimeError, match="attention_mask=None"):
+            layer(x, stack.attention_mask(10, x.device), layer_past=past)
+        with pytest.raises(RuntimeError, match="packed rows"):
+            layer(x.view(5, 2, h), None, layer_past=past)
+        with pytest.raises(NotImplementedError, match="PagedPast"):
+            layer(x, None, layer_past=torch.zeros(2, 3, device="cuda"))
+    stack.train()
+    with pytest.raises(RuntimeError, match="eval"):
+        stack.generate([[1, 2]], maximum_tokens=3)
