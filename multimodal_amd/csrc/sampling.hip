@@ -16,6 +16,7 @@
 // geometric sequence and the chunk's weight is a polynomial, sum n_i r^i, by Horner's rule - two exponentials a chunk instead of one
 // a value.  A chunk takes 65 words of LDS, so that 64 lanes walking 64 chunks in step meet 64 banks; (4) a scan over the 1024 chunks;
 // (5) one wave finds the borders: 64-way search for the chunk, a scan over its 64 values; (6) the j-th match of the value found.
+// With a top-k of at most 512, what can be among the first k is listed and ranked instead of (2) to (6).
 // Rows of more than 65528 logits (BIG) could overflow 16-bit counts: they count non-negative and negative values one after the
 // other in 32 bits, re-read the row instead of keeping it, and recount a chunk when a border falls into it.
 #include "common.h"
@@ -34,11 +35,15 @@ struct SampleArgs {
     const int32_t* top_k_v;
 };
 
-constexpr int kSampleThreads = 1024, kSampleWaves = 16, kChunks = 1024, kSampleSteps = 8;
+constexpr int kSampleThreads = 1024, kSampleWaves = 16, kChunks = 1024, kSampleSteps = 8, kListed = 1024;
 
 // A 16-bit logit's place in descending order: non-negative b -> 0x7fff - b, negative b (sign bit set) -> b.  Two at a time.
 // -0 (0x8000) becomes a value of its own next to +0 (0x7fff); they are merged where it matters.
-__device__ __forceinline__ uint32_t order2(uint32_t v) { return v ^ 0x7fff7fffu ^ (((v >> 15) & 0x00010001u) * 0x7fffu); }
+__device__ __forceinline__ uint32_t order2(uint32_t v) {
+    typedef __attribute__((ext_vector_type(2))) short ss2;
+    const uint32_t negative = __builtin_bit_cast(uint32_t, __builtin_bit_cast(ss2, v) >> 15);
+    return v ^ (0x7fff7fffu & ~negative);
+}
 constexpr int kPlusZero = 0x7fff, kMinusZero = 0x8000;
 template <typename T> constexpr int inf_bits();
 template <> constexpr int inf_bits<BF16>() { return 0x7f80; }
@@ -127,10 +132,23 @@ struct SampleShared {
     uint32_t wave_count[kSampleWaves];
     us2 wave_ends[kSampleWaves];
     int dk, j;
-    uint32_t one_chunk[64];  // BIG
+    uint32_t one_chunk[64];
+    uint32_t listed;
+    // the list of a top-k's candidates and its ranking take the histogram's place
+    __device__ __forceinline__ uint64_t* list() { return reinterpret_cast<uint64_t*>(hist); }
+    __device__ __forceinline__ uint64_t* sorted() { return reinterpret_cast<uint64_t*>(hist) + kListed; }
 };
 
 __device__ __forceinline__ int hist_word(int dk) { return (dk & 0x7fff) + ((dk >> 6) & 511); }
+
+// the first of 1024 entries with pred(entry), which holds from there on (the last one if it never does); a whole wave calls it
+template <typename F> __device__ __forceinline__ int first_of(F&& pred) {
+    const int lane = threadIdx.x & 63;
+    uint64_t b = __ballot(pred(16 * lane + 15));
+    const int blk = b ? __builtin_ctzll(b) : 63;
+    b = __ballot(lane < 16 && pred(16 * blk + (lane & 15)));
+    return 16 * blk + (b ? __builtin_ctzll(b) : 15);
+}
 
 template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) void sample_tokens_k(const SampleArgs a) {
     __shared__ __attribute__((aligned(16))) SampleShared sm;
@@ -176,7 +194,7 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
         u32x4* h = reinterpret_cast<u32x4*>(sm.hist);
         for (int i = tid; i < 512 * 65 / 4; i += kSampleThreads) h[i] = u32x4{0, 0, 0, 0};
     };
-    if (!greedy) clear_hist();
+    if (!greedy && (BIG || k <= 0 || k > kSampleThreads / 2)) clear_hist();
     if constexpr (!BIG) {
 #pragma unroll
         for (int s = 0; s < kSampleSteps; ++s)
@@ -200,12 +218,13 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
         }
     };
 
-    us2 lo2 = {0xffff, 0xffff}, hi2 = {0xffff, 0xffff};  // smallest place; complement of the largest
+    us2 lo2 = {0xffff, 0xffff}, hi2 = {0, 0};
     each2([&](uint32_t o) {
         lo2 = pk_min(lo2, __builtin_bit_cast(us2, o));
-        hi2 = pk_min(hi2, __builtin_bit_cast(us2, ~o));
+        hi2 = __builtin_elementwise_max(hi2, __builtin_bit_cast(us2, o));
     });
-    const us2 mine2 = pk_min(us2{lo2[0], hi2[0]}, us2{lo2[1], hi2[1]});  // {smallest, complement of the largest} of this thread
+    hi2 = ~hi2;
+    const us2 mine2 = pk_min(us2{lo2[0], hi2[0]}, us2{lo2[1], hi2[1]});  // {smallest, complement of the largest} place of this thread
     {
         const us2 w2 = wave_min2(mine2);
         if (lane == 63) sm.wave_ends[wave] = w2;
@@ -233,21 +252,89 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
         const int clo = lo >> 6;
         sm.count[tid] = 0;
         sm.mass[tid] = 0.0;
+        bool listed = false;
         if (!BIG && k > 0 && k <= kSampleThreads / 2) {
             // The k-th largest of the threads' largest logits bounds the k-th largest logit from below: what lies in a later chunk
-            // is not among the first k, and stays out of the histogram (50304 logits, k = 64: 0.3 % of them come in)
+            // is not among the first k (50304 logits, k = 64: some 0.3 % are left).
             __syncthreads();
             atomicAdd(&sm.count[mine2[0] >> 6], 1u);
             __syncthreads();
             const uint32_t n = sm.count[tid], c = scan_u(n);
             if (lane == 63) sm.wave_count[wave] = c;
+            if (tid == 0) sm.listed = 0;
             __syncthreads();
             const uint32_t w = sm.wave_count[lane & 15];
             const uint32_t upto = c + lane_u(row_sum_u((lane & 15) < wave ? w : 0u), 15);
-            if (upto >= (uint32_t)k && upto - n < (uint32_t)k) sm.dk = 64 * tid + 63;  // one thread
+            if (upto >= (uint32_t)k && upto - n < (uint32_t)k) {  // one thread
+                sm.dk = tid;
+                sm.j = (int)((uint32_t)k - (upto - n));  // the how manieth of this chunk's maxima
+            }
+            if (tid < 64) sm.one_chunk[tid] = 0;
             __syncthreads();
-            dlow = min(dlow, __builtin_amdgcn_readfirstlane(sm.dk));
+            const int bc = __builtin_amdgcn_readfirstlane(sm.dk);
+            if ((int)(mine2[0] >> 6) == bc) atomicAdd(&sm.one_chunk[mine2[0] & 63], 1u);
+            __syncthreads();
+            const uint64_t at_k = __ballot(scan_u(sm.one_chunk[lane]) >= (uint32_t)sm.j);
+            dlow = min(dlow, 64 * bc + (int)__builtin_ctzll(at_k));
+            if (dlow == kPlusZero) dlow = kMinusZero;  // the two zeros tie
             sm.count[tid] = 0;
+            // What is left is listed (in no order) and, if the list holds it, ranked: place and index make one number
+            const us2 beyond = {(unsigned short)(dlow + 1), (unsigned short)(dlow + 1)};
+            auto list = [&](uint32_t o, int e) {
+                const us2 in = __builtin_elementwise_sub_sat(beyond, __builtin_bit_cast(us2, o));  // not 0: at or before dlow
+                if (__builtin_bit_cast(uint32_t, in) != 0) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        if (in[i] == 0) continue;
+                        uint32_t d = i ? o >> 16 : o & 0xffffu;
+                        if (d == (uint32_t)kMinusZero) d = kPlusZero;
+                        const uint32_t at = atomicAdd(&sm.listed, 1u);
+                        if (at < kListed) sm.list()[at] = ((uint64_t)d << 32) | (uint32_t)(e + i);
+                    }
+                }
+            };
+#pragma unroll
+            for (int s = 0; s < kSampleSteps; ++s)
+                if (s < steps && ch0 + 64 * s + lane < ch1) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) list(reg[s < (BIG ? 1 : kSampleSteps) ? s : 0][i], (ch0 + 64 * s + lane) * 8 - lead + 2 * i);
+                }
+            __syncthreads();
+            const int m = __builtin_amdgcn_readfirstlane((int)sm.listed);
+            listed = m <= kListed;
+            if (listed) {
+                if (64 * wave < m) {
+                    const uint64_t key = sm.list()[min(tid, m - 1)];
+                    int rank = 0;
+#pragma unroll 8
+                    for (int i = 0; i < m; ++i) rank += sm.list()[i] < key ? 1 : 0;
+                    if (tid < m) sm.sorted()[rank] = key;
+                }
+                __syncthreads();
+                // weights in order; their running sum
+                double wgt = 0.0;
+                if (tid < m && tid < k) wgt = wt.at((int)(sm.sorted()[tid] >> 32));
+                const double c2 = scan_d(wgt);
+                const uint64_t heavy = __ballot(wgt >= fmin((double)mp, 1.0));
+                if (lane == 63) {
+                    sm.wave_mass[wave] = c2;
+                    sm.wave_count[wave] = __popcll(heavy);
+                }
+                __syncthreads();
+                sm.mass[tid] = c2 + lane_d(row_sum_d((lane & 15) < wave ? sm.wave_mass[lane & 15] : 0.0), 15);
+                __syncthreads();
+                if (wave == 0) {
+                    double z = sm.mass[kChunks - 1], zp = z;
+                    if (p > 0.f && p < 1.f) zp = fmin(zp, sm.mass[first_of([&](int i) { return sm.mass[i] > (double)p * z; })]);
+                    if (mp > 0.f) zp = fmin(zp, sm.mass[max((int)lane_u(row_sum_u(sm.wave_count[lane & 15]), 15), 1) - 1]);
+                    zp = fmax(zp, 1.0);
+                    double t = (double)u * zp;
+                    if (!(t < zp)) t = __longlong_as_double(__double_as_longlong(zp) - 1);  // u of 1 or more: the last token kept
+                    const int f = first_of([&](int i) { return sm.mass[i] > t; });
+                    if (lane == 0) a.out[row] = (int64_t)(uint32_t)sm.sorted()[f];
+                }
+                return;
+            }
         }
         const int chi = dlow >> 6;
         // count and weight of chunk tid, chunks first .. last being in the histogram (BIG: half a histogram of whole words)
@@ -289,11 +376,17 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
             }
         };
         if constexpr (!BIG) {
-            const uint32_t last = 64u * chi + 63u;
-            each2([&](uint32_t o) {
-                const uint32_t d0 = o & 0xffffu, d1 = o >> 16;
-                if (d0 <= last) atomicAdd(&sm.hist[hist_word(d0)], d0 < 0x8000 ? 1u : 0x10000u);
-                if (d1 <= last) atomicAdd(&sm.hist[hist_word(d1)], d1 < 0x8000 ? 1u : 0x10000u);
+            if (k > 0 && k <= kSampleThreads / 2) {  // the list has been where the counts go
+                __syncthreads();
+                clear_hist();
+                __syncthreads();
+            }
+            each2([&](uint32_t o) {  // hist_word of both halves at once
+                const uint32_t w = (o & 0x7fff7fffu) + ((o >> 6) & 0x01ff01ffu);
+                uint32_t s0 = __builtin_amdgcn_ubfe(o, 15, 1), s1 = o >> 31;
+                asm("" : "+v"(s0), "+v"(s1));  // keep the signs numbers: a compare and a select each cost more
+                atomicAdd(&sm.hist[w & 0xffffu], __umul24(s0, 0xffffu) + 1u);
+                atomicAdd(&sm.hist[w >> 16], __umul24(s1, 0xffffu) + 1u);
             });
             __syncthreads();
             if (tid == 0) {  // -0 is +0
@@ -355,12 +448,6 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
                 __syncthreads();
                 return sm.one_chunk[lane];
             };
-            auto first_chunk = [&](auto&& pred) -> int {  // the first chunk with pred(inclusive scan); pred holds from there on
-                uint64_t b = __ballot(pred(16 * lane + 15));
-                const int blk = b ? __builtin_ctzll(b) : 63;
-                b = __ballot(lane < 16 && pred(16 * blk + (lane & 15)));
-                return 16 * blk + (b ? __builtin_ctzll(b) : 15);
-            };
             // the first token whose running weight exceeds t: value, how many tokens of that value are ahead of it, and the running
             // weight up to and with it
             struct Found {
@@ -368,7 +455,7 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
                 double upto;
             };
             auto find = [&](double t) -> Found {
-                const int c = first_chunk([&](int i) { return sm.mass[i] > t; });
+                const int c = first_of([&](int i) { return sm.mass[i] > t; });
                 const double ahead = c ? sm.mass[c - 1] : 0.0;
                 const uint32_t n = counts(c);
                 const double w = n ? wt.at(64 * c + lane) : 0.0;
@@ -384,7 +471,7 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
             };
             double z = sm.mass[kChunks - 1];
             if (k > 0 && (uint32_t)k < sm.count[kChunks - 1]) {
-                const int c = first_chunk([&](int i) { return sm.count[i] >= (uint32_t)k; });
+                const int c = first_of([&](int i) { return sm.count[i] >= (uint32_t)k; });
                 const uint32_t n = counts(c);
                 const double w = n ? wt.at(64 * c + lane) : 0.0;
                 const uint32_t ci = (c ? sm.count[c - 1] : 0u) + scan_u(n);
@@ -436,14 +523,10 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
         if (dk == kPlusZero) m |= ((o & 0xffffu) == kMinusZero ? 1u : 0u) | ((o >> 16) == kMinusZero ? 2u : 0u);
         return m;
     };
-    // (x - 1) & ~x has its top bit set where a half x is zero; it may be set above a half that is, which only costs the count
-    uint32_t some = 0;
-    each2([&](uint32_t o) {
-        const uint32_t x = o ^ want;
-        some |= (x - 0x10001u) & ~x;
-    });
+    us2 some = {1, 1};  // 0 where a half has been equal
+    each2([&](uint32_t o) { some = pk_min(some, __builtin_bit_cast(us2, o ^ want)); });
     uint32_t tot = 0;
-    if (dk == kPlusZero || __ballot((some & 0x80008000u) != 0)) {
+    if (dk == kPlusZero || __ballot(some[0] == 0 || some[1] == 0)) {
         uint32_t mine = 0;
         each2([&](uint32_t o) { mine += __popc(matches(o)); });
         tot = lane_u(scan_u(mine), 63);
