@@ -13,6 +13,7 @@ __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_ex
 // sinking the load to the first MFMA inside the tile loop (where its pending vmcnt would serialise every iteration's
 // prefetch behind the MFMAs).
 template <typename V> __device__ __forceinline__ void pin(V& v) {
+    static_assert(sizeof(V) == 16, "a 16-byte operand");
     u32x4 t;
     __builtin_memcpy(&t, &v, 16);
     asm volatile("" : "+v"(t));

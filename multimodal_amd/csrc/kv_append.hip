@@ -109,7 +109,7 @@ __global__ __launch_bounds__(256) void paged_kv_append_k(const AppendArgs a, int
 template <typename T, typename TT, int W> static int launch_append(const AppendArgs& a, hipStream_t st) {
     const int items = (a.nq + 2 * a.kv.heads) * (a.kv.hn / (2 * W));
     const int parts = (items + 255) / 256;
-    MM_CHECK_ARG((int64_t)parts * a.rows < (int64_t)1 << 31, "mm_paged_kv_append: %d rows of %d items exceed the grid limit", a.rows, items);
+    MM_CHECK_ARG((int64_t)parts * a.rows < (int64_t)1 << 24, "mm_paged_kv_append: %d rows of %d items exceed the grid limit", a.rows, items);
     if (a.kv.hn == 64) paged_kv_append_k<T, TT, W, 64><<<parts * a.rows, 256, 0, st>>>(a, parts);
     else paged_kv_append_k<T, TT, W, 128><<<parts * a.rows, 256, 0, st>>>(a, parts);
     MM_CHECK_LAUNCH();
@@ -126,7 +126,7 @@ extern "C" int mm_paged_kv_append(const mm_paged_kv* kv, const mm_paged_step* st
                                   int rot_d, int table_rows, int table_fp32, void* stream) {
     const char* fn = "mm_paged_kv_append";
     if (int rc = check_paged(fn, kv, step, rows)) return rc;
-    MM_CHECK_ARG(k && v, "%s: null pointer", fn);
+    MM_CHECK_ARG(rows == 0 || (k && v), "%s: null pointer", fn);
     if (!q) nq = 0;
     MM_CHECK_ARG(!q || (q_out && nq > 0 && nq < 1 << 20), "%s: queries need q_out and a head count, got %d", fn, nq);
     MM_CHECK_ARG(rot_d >= 0 && rot_d <= kv->hn && rot_d % 2 == 0, "%s: rotary dims %d must be even and at most %d", fn, rot_d, kv->hn);

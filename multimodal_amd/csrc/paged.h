@@ -65,7 +65,7 @@ __device__ __forceinline__ int find_seq(const int32_t* __restrict__ cu, int n, i
 
 inline int check_paged(const char* fn, const mm_paged_kv* kv, const mm_paged_step* st, int rows) {
     MM_CHECK_ARG(kv && st, "%s: null cache or step", fn);
-    MM_CHECK_ARG(kv->k && kv->v && st->block_table && st->cu_new && st->kv_lens, "%s: null pointer", fn);
+    MM_CHECK_ARG(kv->k && kv->v && (st->seqs == 0 || (st->block_table && st->cu_new && st->kv_lens)), "%s: null pointer", fn);
     MM_CHECK_ARG(kv->hn == 64 || kv->hn == 128, "%s: head size %d not supported (64 or 128)", fn, kv->hn);
     MM_CHECK_ARG(kv->num_pages > 0 && kv->page_size > 0 && kv->heads > 0 && rows >= 0 && st->seqs >= 0 && st->max_pages > 0,
                  "%s: pages=%d page_size=%d heads=%d rows=%d seqs=%d max_pages=%d out of range", fn, kv->num_pages, kv->page_size,

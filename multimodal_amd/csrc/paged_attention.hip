@@ -11,8 +11,9 @@
 //
 // Masked places never matter: a score behind a row's position is replaced by -inf (not added to), value rows behind the
 // sequence's end are zeroed on their way into LDS, and where a tile holds keys that some of its rows do not see, infinities and
-// NaN in the values are taken out of the matrix product (0 * inf would spread them to those rows) and added afterwards to
-// the rows that do see them: p * v is +-inf or NaN whatever p > 0 is.
+// NaN in the values are taken out of the matrix product (0 * inf would spread them to those rows) and added at the end to
+// the rows that do see them: p * v is +-inf or NaN whatever p > 0 is.  Tiles that all rows see go unchecked; if an output is not
+// finite at the end, the keys are gone through once more with every tile checked, because there p may have rounded to 0.
 #include "common.h"
 #include "mfma32.h"
 #include "attn_common.h"
@@ -48,7 +49,7 @@ template <int HD>
 __device__ __forceinline__ bool seq_info(const PagedAttnArgs& a, int seq, int kh, bool writer, SeqInfo& s) {
     s.beg = a.st.cu_new[seq];
     const int end = a.st.cu_new[seq + 1];
-    s.len = a.st.kv_lens[seq];
+    s.len = max(a.st.kv_lens[seq], 0);
     if (end <= s.beg) return false;
     if (s.beg >= 0 && end <= a.rows && end - s.beg <= a.st.max_new && s.len <= a.st.max_kv &&
         s.len <= a.st.max_pages * (int)a.page.d) {
@@ -90,6 +91,33 @@ template <typename T> __device__ __forceinline__ float only_nonfinite(const u16*
     const u16 v = *p;
     return (v & exp_mask<T>()) == exp_mask<T>() ? to_f32<T>(v) : 0.f;
 }
+__device__ __forceinline__ bool nonfinite(float x) { return !(x - x == 0.f); }
+// w * x where w stands for a positive weight that may have become 0
+__device__ __forceinline__ float weigh(float w, float x) { return w != 0.f ? w * x : nonfinite(x) ? x : 0.f; }
+// add(key, its value row) for the keys of [k0, k1) whose value rows hold infinities or NaN; a whole wave calls it
+template <typename T, int HD, typename F>
+__device__ __forceinline__ void each_nonfinite(const PagedAttnArgs& a, const int32_t* __restrict__ bt, int kh, int k0, int k1, F&& add) {
+    constexpr int CPR = HD / 8, KEYS = 64 / CPR;  // lanes a key, keys a step
+    const int lane = threadIdx.x & 63;
+    auto row_of = [&](int key) -> const u16* {  // NULL: its page does not exist
+        const int pi = (int)fdiv((uint32_t)key, a.page), pg = bt[pi];
+        if ((uint32_t)pg >= (uint32_t)a.kv.num_pages) return nullptr;
+        return (const u16*)a.kv.v + (int64_t)pg * a.kv.page + (int64_t)kh * a.kv.head + (int64_t)(key - pi * (int)a.page.d) * a.kv.slot;
+    };
+    for (int base = k0; base < k1; base += KEYS) {
+        bool any = false;
+        if (base + lane / CPR < k1) {
+            const u16* vp = row_of(base + lane / CPR);
+            if (vp) {
+                u32x4 v = *reinterpret_cast<const u32x4*>(vp + 8 * (lane % CPR));
+                any = take_nonfinite<T>(v);
+            }
+        }
+        const uint64_t b = __ballot(any);
+        for (int i = 0; i < KEYS && b; ++i)
+            if ((b >> (CPR * i)) & ((1ull << CPR) - 1)) add(base + i, row_of(base + i));
+    }
+}
 
 template <typename T> struct M16;
 template <> struct M16<BF16> {
@@ -126,12 +154,14 @@ template <int NW> struct FewStart {
     int pid[2];
     __device__ __forceinline__ FewStart(const PagedAttnArgs& a, int seq, int split) {
         const int32_t* bt = a.st.block_table + (int64_t)seq * a.st.table_stride;
+        set(a, split);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) pid[t] = bt[min(cur[t].page, (uint32_t)a.st.max_pages - 1)];
+    }
+    __device__ __forceinline__ void set(const PagedAttnArgs& a, int split) {
         const int key = split * a.few_chunk + (int)scalar(threadIdx.x >> 6) * 32 + (threadIdx.x & 15);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            cur[t].set((uint32_t)(key + 16 * t), a.page, 2 * (uint32_t)a.kv.slot);
-            pid[t] = bt[min(cur[t].page, (uint32_t)a.st.max_pages - 1)];
-        }
+        for (int t = 0; t < 2; ++t) cur[t].set((uint32_t)(key + 16 * t), a.page, 2 * (uint32_t)a.kv.slot);
     }
 };
 template <typename T, int HD, int NW>
@@ -197,34 +227,33 @@ __device__ __forceinline__ void paged_attn_few(const PagedAttnArgs& a, char* sme
     };
 
     f32x4 o[NDB];
+    float m_run, l_run;
+    char* vs = smem + wave * VB;
+    const int kt0 = c0 + wave * 32;
+    bool taken = false;  // values that are not finite have been taken out of the products
+    for (bool check_all = false;; check_all = true) {
 #pragma unroll
     for (int d = 0; d < NDB; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m_run = -INFINITY, l_run = 0.f;
-    char* vs = smem + wave * VB;
-
-    int kt = c0 + wave * 32;
-    if (kt < c1) {
+    m_run = -INFINITY, l_run = 0.f;
+    if (kt0 < c1) {
         move_on();
         fetch();
         fetch_pid();
     }
-    for (; kt < c1; kt += NW * 32) {
+    for (int kt = kt0; kt < c1; kt += NW * 32) {
         // the tile's values into LDS, its keys into the matrix unit; then its registers take the next tile
-        const bool part = kt + 31 > min_limit;  // some row does not see all of it (wave-uniform)
-        uint64_t nf[2] = {0, 0};
+        const bool part = check_all || kt + 31 > min_limit;  // some row does not see all of it (wave-uniform)
         const uint64_t badk[2] = {__ballot(bad & 1), __ballot(bad & 2)};
         if (part) {
+            bool any = false;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                bool any = false;
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < NC; ++i) {
                     if (kt + 16 * t + r >= s.len) vr[t][i] = u32x4{0, 0, 0, 0};
                     any |= take_nonfinite<T>(vr[t][i]);
                 }
-                const uint64_t bl = __ballot(any);
-                nf[t] = (bl | (bl >> 16) | (bl >> 32) | (bl >> 48)) & 0xffff;
-            }
+            taken |= __any(any);
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t)
@@ -295,19 +324,26 @@ __device__ __forceinline__ void paged_attn_few(const PagedAttnArgs& a, char* sme
             const s16x8 v = s16x8{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
             o[d] = M16<T>::run(__builtin_bit_cast(frag, v), pfr, M16<T>::run(__builtin_bit_cast(frag, v), pf, o[d]));
         }
-        if (nf[0] | nf[1]) {
-            for (uint32_t left = (uint32_t)(nf[0] | (nf[1] << 16)); left; left &= left - 1) {
-                const int key = kt + __builtin_ctz(left);
-                const int pi = (int)fdiv((uint32_t)key, a.page), pg = bt[pi];
-                if ((uint32_t)pg >= (uint32_t)a.kv.num_pages || key > limit) continue;
-                const u16* vp = (const u16*)a.kv.v + (int64_t)pg * a.kv.page + (int64_t)kh * a.kv.head +
-                                (int64_t)(key - pi * (int)a.page.d) * a.kv.slot;
+    }
+    float bad_out = 0.f;  // NaN if an output is not finite
+#pragma unroll
+    for (int d = 0; d < NDB; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bad_out = fmaf(o[d][j], 0.f, bad_out);
+    if (check_all || !__any(bad_out != bad_out)) break;
+    start.set(a, split);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) pid[t] = bt[min(cur[t].page, last_page)];
+    }
+    if (taken) {
+        for (int kt = kt0; kt < c1; kt += NW * 32)
+            each_nonfinite<T, HD>(a, bt, kh, kt, min(kt + 32, c1), [&](int key, const u16* vp) {
+                if (key > limit) return;
 #pragma unroll
                 for (int d = 0; d < NDB; ++d)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) o[d][j] += only_nonfinite<T>(vp + 16 * d + 4 * g + j);
-            }
-        }
+            });
     }
 
     // join the waves: rows' maxima and sums, then the weighted outputs
@@ -338,7 +374,7 @@ __device__ __forceinline__ void paged_attn_few(const PagedAttnArgs& a, char* sme
             L += al * sm_l[w][row];
             const float* src = red + (w * 16 + row) * RS + d0;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] += al * src[e];
+            for (int e = 0; e < 8; ++e) acc[e] += weigh(al, src[e]);
         }
         const int t = (int)fdiv((uint32_t)row, a.grp), h = kh * a.group + row - t * a.group, grow = s.beg + t;
         if (a.few_splits == 1) {
@@ -376,14 +412,17 @@ template <int HD> struct KvTile {
     static __device__ __forceinline__ int off(int row, int chunk) { return row * ROWB + ((chunk ^ swz(row)) << 4); }
 };
 
-template <int HD> constexpr int many_lds() { return 4 * KvTile<HD>::BYTES + 64; }
+template <int HD> constexpr int many_lds() { return 4 * KvTile<HD>::BYTES + 48; }
 template <typename T, int HD, int NWV>
 __device__ __forceinline__ void paged_attn_many(const PagedAttnArgs& a, char* smem, const SeqInfo& s, int seq, int kh, int row_block, int split) {
     typedef KvTile<HD> TL;
     typedef typename M32<T>::frag frag;
     constexpr int NDS = HD / 16, NDB = HD / 32, NT = 64 * NWV, NCH = 64 * TL::CPR / NT, ROWS = 32 * NWV;
-    // two stages of K | V, then per ring slot (tile & 3) two 64-bit key masks: pages the cache does not have, values taken out
-    unsigned long long* flags = reinterpret_cast<unsigned long long*>(smem + 4 * TL::BYTES);  // [slot][page | value]
+    // two stages of K | V, then per ring slot (tile & 3) a 64-bit mask of the keys in pages the cache does not have, and whether
+    // values that are not finite have been taken out of the products, and whether an output is not finite
+    unsigned long long* flags = reinterpret_cast<unsigned long long*>(smem + 4 * TL::BYTES);
+    int* taken = reinterpret_cast<int*>(flags + 4);
+    int* bad_out = taken + 1;
     const int tid = threadIdx.x, wave = (int)scalar(tid >> 6), lane = tid & 63, r = lane & 31, hh = lane >> 5;
     const int r0 = row_block * ROWS;
     const int R = s.n * a.group;
@@ -441,23 +480,25 @@ __device__ __forceinline__ void paged_attn_many(const PagedAttnArgs& a, char* sm
             vreg[i] = *reinterpret_cast<const u32x4*>(kp + k_to_v);
         }
     };
+    bool check_all = false;
     // registers -> LDS stage of tile j; where some row of the block does not see the whole tile, the values behind the end become
-    // zero and the non-finite ones are taken out and noted
+    // zero and the non-finite ones are taken out
     auto put = [&](char* ks, int j) __attribute__((always_inline)) {
         const int kv0 = c0 + j * 64;
-        unsigned long long* fl = flags + 2 * (j & 3);
-        if (kv0 + 63 > blk_first) {
+        if (check_all || kv0 + 63 > blk_first) {
+            bool any = false;
 #pragma unroll
             for (int i = 0; i < NCH; ++i) {
                 const int key = trow + RSTEP * i;
                 if (kv0 + key >= s.len) vreg[i] = u32x4{0, 0, 0, 0};
-                if (take_nonfinite<T>(vreg[i])) atomicOr(fl + 1, 1ull << key);
+                any |= take_nonfinite<T>(vreg[i]);
             }
+            if (any) *taken = 1;
         }
         if (__ballot(bad != 0)) {
 #pragma unroll
             for (int i = 0; i < NCH; ++i)
-                if ((bad >> i) & 1) atomicOr(fl, 1ull << (trow + RSTEP * i));
+                if ((bad >> i) & 1) atomicOr(flags + (j & 3), 1ull << (trow + RSTEP * i));
         }
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
@@ -467,26 +508,7 @@ __device__ __forceinline__ void paged_attn_many(const PagedAttnArgs& a, char* sm
     };
 
     f32x16 o[NDB];
-#pragma unroll
-    for (int i = 0; i < NDB; ++i)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
-    float m_run = -INFINITY, l_run = 0.f;
-
-    if (tid < 8) flags[tid] = 0;
-    __syncthreads();
-    if (ntiles > 0) {
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) pos[i].set((uint32_t)(c0 + trow + RSTEP * i), a.page, slot_bytes);
-        fetch_pid();
-        fetch();
-        fetch_pid();
-        put(smem, 0);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int ds = 0; ds < NDS; ++ds) pin(qf[ds]);
-
+    float m_run, l_run;
     // this lane's fragments: row reads of K (chunk 2 ds + hh of row r), transposed reads of V (as tr_frag in mfma32.h)
     const int ka0 = TL::off(r, hh);
     const int tg = lane >> 4, tq = (lane & 15) >> 2, tp = lane & 3;
@@ -510,9 +532,9 @@ __device__ __forceinline__ void paged_attn_many(const PagedAttnArgs& a, char* sm
             fetch();
             fetch_pid();
         }
-        if (tid < 2) flags[2 * ((j + 2) & 3) + tid] = 0;  // read in tile j - 2, written for tile j + 2 behind this tile's barrier
-        const u32x4 fl = *reinterpret_cast<const u32x4*>(flags + 2 * (j & 3));
-        const uint32_t badk[2] = {scalar(fl[0]), scalar(fl[1])}, nonf[2] = {scalar(fl[2]), scalar(fl[3])};
+        if (tid == 0) flags[(j + 2) & 3] = 0;  // read in tile j - 2, written for tile j + 2 behind this tile's barrier
+        const u32x2 fl = *reinterpret_cast<const u32x2*>(flags + (j & 3));
+        const uint32_t badk[2] = {scalar(fl[0]), scalar(fl[1])};
         if (kv0 <= wave_last) {
             f32x16 sacc[2];
             __builtin_amdgcn_s_setprio(1);
@@ -579,27 +601,55 @@ __device__ __forceinline__ void paged_attn_many(const PagedAttnArgs& a, char* sm
                         o[d] = M32<T>::run(v_frag(vs, 32 * t + 16 * s2, d), pf, o[d]);
                 }
             __builtin_amdgcn_s_setprio(0);
-            if (nonf[0] | nonf[1]) {
-                for (unsigned long long left = nonf[0] | (unsigned long long)nonf[1] << 32; left; left &= left - 1) {
-                    const int key = kv0 + __builtin_ctzll(left);
-                    const int pi = (int)fdiv((uint32_t)key, a.page), pg = bt[pi];
-                    if ((uint32_t)pg >= (uint32_t)a.kv.num_pages || key > limit) continue;
-                    const u16* vp = (const u16*)a.kv.v + (int64_t)pg * a.kv.page + (int64_t)kh * a.kv.head +
-                                    (int64_t)(key - pi * (int)a.page.d) * a.kv.slot;
-#pragma unroll
-                    for (int d = 0; d < NDB; ++d)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[d][i] += only_nonfinite<T>(vp + 32 * d + acc_row(i, hh));
-                }
-            }
         }
         if (j + 1 < ntiles) put(smem + (cur ^ 1) * 2 * TL::BYTES, j + 1);
         __syncthreads();
     };
-    for (int j = 0; j < ntiles; j += 2) {
-        tile_step(j, std::integral_constant<int, 0>{});
-        if (j + 1 < ntiles) tile_step(j + 1, std::integral_constant<int, 1>{});
+    for (;; check_all = true) {
+        int first = trow;
+        asm volatile("" : "+v"(first));  // computed anew for the second pass, not held in registers through the first
+#pragma unroll
+        for (int i = 0; i < NDB; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
+        m_run = -INFINITY, l_run = 0.f;
+        if (tid < 4) flags[tid] = 0;
+        if (tid < 2) taken[tid] = 0;
+        __syncthreads();
+        if (ntiles > 0) {
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) pos[i].set((uint32_t)(c0 + first + RSTEP * i), a.page, slot_bytes);
+            fetch_pid();
+            fetch();
+            fetch_pid();
+            put(smem, 0);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int ds = 0; ds < NDS; ++ds) pin(qf[ds]);
+        for (int j = 0; j < ntiles; j += 2) {
+            tile_step(j, std::integral_constant<int, 0>{});
+            if (j + 1 < ntiles) tile_step(j + 1, std::integral_constant<int, 1>{});
+        }
+        if (check_all) break;
+        float b = 0.f;  // NaN if an output is not finite
+#pragma unroll
+        for (int d = 0; d < NDB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) b = fmaf(o[d][i], 0.f, b);
+        if (b != b) *bad_out = 1;
+        __syncthreads();
+        if (!scalar((uint32_t)*bad_out)) break;
+        __syncthreads();  // everyone has read it
     }
+    if (scalar((uint32_t)*taken))
+        each_nonfinite<T, HD>(a, bt, kh, c0, min(c1, wave_last + 1), [&](int key, const u16* vp) {
+            if (key > limit) return;
+#pragma unroll
+            for (int d = 0; d < NDB; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] += only_nonfinite<T>(vp + 32 * d + acc_row(i, hh));
+        });
 
     const float l_tot = half_sum(l_run);
     if (row >= R) return;
@@ -698,9 +748,9 @@ template <typename T, int HD> __global__ __launch_bounds__(256) void paged_attn_
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 const float f = __shfl(w, min(i + u, 63), 64);
-                if (i + u < n && f != 0.f)
+                if (i + u < n)
 #pragma unroll
-                    for (int e = 0; e < E; ++e) acc[e] += f * v[u][e];
+                    for (int e = 0; e < E; ++e) acc[e] += weigh(f, v[u][e]);
             }
         }
     }
@@ -774,7 +824,7 @@ static int check_paged_attn(const char* fn, const mm_paged_kv* kv, const mm_page
     MM_CHECK_ARG(nq > 0 && nq % kv->heads == 0 && nq < 1 << 20, "%s: %d query heads are no multiple of %d key heads", fn, nq, kv->heads);
     MM_CHECK_ARG((int64_t)st->max_new * (nq / kv->heads) < (int64_t)1 << 30 && (int64_t)st->max_new * (nq / kv->heads) / 128 < 16000,
                  "%s: max_new=%d rows of %d heads exceed the grid limit", fn, st->max_new, nq);
-    MM_CHECK_ARG((int64_t)st->seqs * kv->heads < (int64_t)1 << 31 && (int64_t)rows * nq < (int64_t)1 << 31,
+    MM_CHECK_ARG((int64_t)st->seqs * kv->heads < (int64_t)1 << 23 && (int64_t)rows * nq < (int64_t)1 << 31,
                  "%s: %d sequences, %d rows exceed the grid limit", fn, st->seqs, rows);
     MM_CHECK_ARG(st->max_kv < 1 << 30, "%s: max_kv=%d exceeds 2^30", fn, st->max_kv);
     return MM_OK;
@@ -804,6 +854,7 @@ extern "C" int mm_paged_attn_fwd(const mm_paged_kv* kv, const mm_paged_step* ste
     const size_t need = p.splits() == 1 ? 0 : (size_t)p.splits() * rows * nq * (kv->hn + 2) * sizeof(float);
     MM_CHECK_ARG(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need),
                  "%s: workspace of %zu bytes needed (16-byte aligned), got %zu", fn, need, workspace ? workspace_bytes : (size_t)0);
+    MM_CHECK_ARG(need == 0 || (int64_t)rows * nq < (int64_t)1 << 26, "%s: %d rows of %d heads exceed the joining launch's grid", fn, rows, nq);
     PagedAttnArgs a{};
     a.kv = *kv;
     a.st = *step;

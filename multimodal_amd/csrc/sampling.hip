@@ -576,7 +576,7 @@ extern "C" int mm_sample_tokens(int64_t* tokens, const void* logits, int64_t row
                                 float temperature, const float* temperature_rows, int top_k, const int32_t* top_k_rows, float top_p,
                                 const float* top_p_rows, float min_p, const float* min_p_rows, int dtype, void* stream) {
     const char* fn = "mm_sample_tokens";
-    MM_CHECK_ARG(rows >= 0 && vocab > 0 && vocab < 1 << 30, "%s: rows=%d vocab=%d out of range", fn, rows, vocab);
+    MM_CHECK_ARG(rows >= 0 && rows < 1 << 22 && vocab > 0 && vocab < 1 << 30, "%s: rows=%d vocab=%d out of range", fn, rows, vocab);
     if (rows == 0) return MM_OK;
     MM_CHECK_ARG(tokens && logits && u, "%s: null pointer", fn);
     MM_CHECK_ARG(((uintptr_t)logits & 1) == 0, "%s: logits must be 2-byte aligned", fn);

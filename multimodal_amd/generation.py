@@ -39,15 +39,16 @@ def generate(stack, prompts, enc_out=None, maximum_tokens=64, eos_token_id=None,
     image); enc_out [b, P, enc_dim] the pooled encoder outputs, or None; temperature / top_k / top_p as the reference's arguments
     (0: the most likely token / off / off) and min_p, numbers or [b] tensors (ops.sample_tokens); generator: torch generator on
     the stack's device for the random numbers; vocab_size: the tokens to draw from (default: the padded vocabulary); cache: a
-    PagedKVCache with free pages for all of it (default: one is made).  graph=False: launch every token step eagerly.
-    Returns a list of int64 tensors on the CPU, each up to and with eos_token_id.  The stack must be in eval mode."""
+    PagedKVCache of the stack's layers with free pages for all of it (default: one is made).  graph=False: launch every token step
+    eagerly.  Returns a list of int64 tensors on the CPU, each up to and with eos_token_id, or with -1 where the logits held a NaN
+    (the sequence ends there).  The stack must be in eval mode."""
     if stack.training:
         raise RuntimeError("generate: put the stack in eval mode (dropout has no place here)")
     if mpu.get_model_parallel_world_size() > 1:
         raise NotImplementedError("generate: the sampled distribution is not vocabulary-parallel (tensor-parallel size 1 only)")
     w = stack.word_embeddings.weight
     dev, h = w.device, w.size(1)
-    prompts = [torch.as_tensor(p, dtype=torch.int64).reshape(-1) for p in prompts]
+    prompts = [torch.as_tensor(p, dtype=torch.int64).reshape(-1).cpu() for p in prompts]
     b = len(prompts)
     if b == 0 or maximum_tokens < 1:
         return [torch.empty(0, dtype=torch.int64) for _ in prompts]
@@ -61,15 +62,20 @@ def generate(stack, prompts, enc_out=None, maximum_tokens=64, eos_token_id=None,
     if min(lens) < 1:
         raise RuntimeError("generate: an empty prompt without an image has nothing to continue")
     total = [n + maximum_tokens - 1 for n in lens]  # the last token drawn enters no cache
+    if vocab_size is not None and not 0 < vocab_size <= w.size(0):
+        raise RuntimeError(f"generate: vocab_size {vocab_size} is not in (0, {w.size(0)}]")
     if cache is None:
         cache = make_cache(stack, b, max(total), page_size)
+    elif len(cache.layers) != len(stack.layers):
+        raise RuntimeError(f"generate: a cache of {len(cache.layers)} layers for a stack of {len(stack.layers)}")
     seqs = []
     try:
         for n in total:
             seqs.append(cache.add(n))
-        return _generate(stack, prompts, prefix, p_len, lens, max(total), cache, seqs, maximum_tokens, eos_token_id,
-                         dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p), generator,
-                         vocab_size or w.size(0), graph)
+        with torch.cuda.device(dev):  # the captured step's stream is the current device's
+            return _generate(stack, prompts, prefix, p_len, lens, max(total), cache, seqs, maximum_tokens, eos_token_id,
+                             dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p), generator,
+                             vocab_size or w.size(0), graph)
     finally:
         for s in seqs:
             cache.release(s)
@@ -118,14 +124,16 @@ def _generate(stack, prompts, prefix, p_len, lens, positions, cache, seqs, maxim
                 with torch.cuda.graph(replay):
                     token_step()
         out[t] = token
-        if eos is not None and t % 16 == 0 and bool((out[:t + 1] == eos).any(dim=0).all()):
+        if t % 16 == 0 and eos is not None and bool(_ends(out[:t + 1], eos).any(dim=0).all()):
             out = out[:t + 1]
             break
     return _trim(out, eos)
 
 
+def _ends(tokens, eos):
+    return tokens == -1 if eos is None else (tokens == eos) | (tokens == -1)
+
+
 def _trim(out, eos):
     rows = out.t().cpu()
-    if eos is None:
-        return list(rows)
-    return [r[:int((r == eos).nonzero()[0]) + 1] if bool((r == eos).any()) else r for r in rows]
+    return [r[:int(e.nonzero()[0]) + 1] if bool(e.any()) else r for r, e in zip(rows, _ends(rows, eos))]

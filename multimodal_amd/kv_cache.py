@@ -60,8 +60,8 @@ class PagedStep:
             max_new = int((cu_new[1:] - cu_new[:-1]).max()) if self.seqs else 0
         if max_kv is None:
             max_kv = int(kv_lens.max()) if self.seqs else 0
-        if max_new < 0 or max_kv < 0:
-            raise RuntimeError(f"PagedStep: max_new={max_new}, max_kv={max_kv} must not be negative")
+        if not (0 <= max_new < 1 << 31 and 0 <= max_kv < 1 << 31):
+            raise RuntimeError(f"PagedStep: max_new={max_new}, max_kv={max_kv} must be in [0, 2^31)")
         self.block_table, self.cu_new, self.kv_lens = block_table, cu_new, kv_lens
         self.max_new, self.max_kv, self.device = int(max_new), int(max_kv), cu_new.device
         self._c = MmPagedStep(block_table.data_ptr(), cu_new.data_ptr(), kv_lens.data_ptr(), block_table.stride(0), self.seqs,
@@ -90,6 +90,11 @@ class PagedKVCache:
         self._pages = {}   # sequence -> its pages, in order
         self._next = 0
 
+    def _of(self, seq):
+        if seq not in self._pages:
+            raise RuntimeError(f"PagedKVCache: no sequence {seq}")
+        return self._pages[seq]
+
     @property
     def free_pages(self):
         return len(self._free)
@@ -107,7 +112,7 @@ class PagedKVCache:
 
     def reserve(self, seq, tokens):
         """Room for `tokens` tokens in all; raises, and takes nothing, when the free pages do not suffice."""
-        pages = self._pages[seq]
+        pages = self._of(seq)
         need = -(-int(tokens) // self.page_size) - len(pages)
         if need > len(self._free):
             raise RuntimeError(f"PagedKVCache: {need} pages needed, {len(self._free)} free")
@@ -117,18 +122,24 @@ class PagedKVCache:
     def release(self, seq):
         """Give a sequence's pages back.  Work on the GPU that still reads them must have been enqueued on the stream of the work
         that will write them next."""
-        self._free.extend(reversed(self._pages.pop(seq)))
+        self._free.extend(reversed(self._of(seq)))
+        del self._pages[seq]
 
     def block_table(self, seqs):
         """int32 [len(seqs), pages of the longest] on the device; entries behind a sequence's last page are -1."""
-        width = max([len(self._pages[s]) for s in seqs] + [1])
+        width = max([len(self._of(s)) for s in seqs] + [1])
         rows = [self._pages[s] + [-1] * (width - len(self._pages[s])) for s in seqs]
         return torch.tensor(rows, dtype=torch.int32).view(len(seqs), width).to(self.device)
 
     def step(self, seqs, new, lens):
-        """The step that brings new[i] rows to sequence seqs[i], whose length is lens[i] afterwards (host numbers)."""
+        """The step that brings new[i] rows to sequence seqs[i], whose length is lens[i] afterwards (host numbers).  A sequence comes
+        once: two rows of a step must not share a slot."""
+        if not len(seqs) == len(new) == len(lens):
+            raise RuntimeError(f"PagedKVCache: {len(seqs)} sequences, but {len(new)} and {len(lens)} numbers for them")
+        if len(set(seqs)) != len(seqs):
+            raise RuntimeError(f"PagedKVCache: a sequence comes twice in {list(seqs)}")
         for s, n, l in zip(seqs, new, lens):
-            if not 0 <= n <= l or l > len(self._pages[s]) * self.page_size:
+            if not 0 <= n <= l or l > len(self._of(s)) * self.page_size:
                 raise RuntimeError(f"PagedKVCache: sequence {s} has room for {len(self._pages[s]) * self.page_size} tokens, not for "
                                    f"{n} new ones up to {l}")
         cu = [0]

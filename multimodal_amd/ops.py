@@ -733,6 +733,8 @@ def _out_rows(name, t, shape, dtype, device):
     if t.shape != shape or t.dtype != dtype or t.device != device or stride[-1] != 1:
         raise RuntimeError(f"{name} must be a {tuple(shape)} {dtype} tensor on {device} with a contiguous last dim, got {tuple(t.shape)} "
                            f"{t.dtype} on {t.device}, strides {stride}")
+    if 0 in stride and any(s == 0 and n > 1 for s, n in zip(stride, shape)):
+        raise RuntimeError(f"{name} must not overlap itself, strides {stride}")
     return stride
 
 

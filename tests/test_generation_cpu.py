@@ -118,3 +118,30 @@ def test_division_by_multiplication(d):
         if 0 <= n < 1 << 31:
             q = ((m * n) >> 32) + n
             assert q < 1 << 32 and q >> l == n // d, (n, d)
+
+
+def test_launches_beyond_the_grid_are_refused():
+    """A grid dimension times the workgroup's threads stays below 2^32."""
+    lib = _lib.get_lib()
+    rc, msg = append(rows=1 << 24)
+    assert rc == -1 and "grid" in msg
+    rc, msg = attend(step=dict(seqs=1 << 21))
+    assert rc == -1 and "grid" in msg
+    big = dict(max_kv=5000, max_pages=512, table_stride=512, seqs=1)
+    a, b, pa, pb = refs(step=big)
+    need = lib.mm_paged_attn_workspace_bytes(pa, pb, 4, 1 << 24)
+    rc, msg = attend(step=big, rows=1 << 24, ws=4096, ws_bytes=need)
+    assert need > 0 and rc == -1 and "grid" in msg
+    assert lib.mm_sample_tokens(4096, 4096, 128, 4096, 1 << 22, 100, 1.0, None, 0, None, 0.0, None, 0.0, None, 0, None) == -1
+
+
+def test_empty_arrays_may_be_null():
+    assert append(step=dict(seqs=0, block_table=0, cu_new=0, kv_lens=0))[0] == 0 and attend(step=dict(seqs=0, block_table=0, kv_lens=0))[0] == 0
+    assert append(rows=0, k=0, v=0, q=0, q_out=0)[0] == 0
+
+
+def test_generated_rows_end_with_the_end_token_or_a_failed_draw():
+    from multimodal_amd.generation import _trim
+    out = torch.tensor([[5, 7, 9, 1], [3, -1, 9, 2], [8, 4, 3, 3], [3, 3, -1, 4]])
+    assert [r.tolist() for r in _trim(out, 3)] == [[5, 3], [7, -1], [9, 9, 3], [1, 2, 3]]
+    assert [r.tolist() for r in _trim(out, None)] == [[5, 3, 8, 3], [7, -1], [9, 9, 3, -1], [1, 2, 3, 4]]

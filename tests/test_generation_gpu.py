@@ -149,3 +149,29 @@ def test_refusals_of_the_layer():
     stack.train()
     with pytest.raises(RuntimeError, match="eval"):
         stack.generate([[1, 2]], maximum_tokens=3)
+
+
+def test_arguments_of_generate():
+    """Prompts may live on the GPU; a cache of another depth and a vocabulary the head does not have are refused; a sequence whose
+    logits hold a NaN ends with -1, the others go on."""
+    from multimodal_amd.kv_cache import PagedKVCache
+    cfg, stack = build("tiny")
+    g = torch.Generator().manual_seed(7)
+    prompts = [torch.randint(0, 1000, (n,), generator=g) for n in (3, 9)]
+    ref = stack.generate(prompts, maximum_tokens=10)
+    got = stack.generate([p.cuda() for p in prompts], maximum_tokens=10)
+    assert all(torch.equal(x, y) for x, y in zip(ref, got))
+    heads = cfg["num_attention_heads"]
+    for layers in (len(stack.layers) - 1, len(stack.layers) + 1):
+        cache = PagedKVCache(layers, heads, cfg["hidden_size"] // heads, 40)
+        with pytest.raises(RuntimeError, match="layers"):
+            stack.generate(prompts, maximum_tokens=4, cache=cache)
+        assert cache.free_pages == 40
+    for v in (-1, 0, stack.word_embeddings.weight.size(0) + 1):
+        with pytest.raises(RuntimeError, match="vocab_size"):
+            stack.generate(prompts, maximum_tokens=4, vocab_size=v)
+    unused = next(t for t in range(1000) if all(t not in o.tolist() + p.tolist() for o, p in zip(ref, prompts)))
+    with torch.no_grad():
+        stack.word_embeddings.weight[unused] = float("nan")
+    got = stack.generate([prompts[0], torch.cat((prompts[1], torch.tensor([unused])))], maximum_tokens=10)
+    assert torch.equal(got[0], ref[0]) and got[1].tolist() == [-1]

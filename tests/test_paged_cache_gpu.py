@@ -296,3 +296,78 @@ def test_same_bits_twice_on_another_stream_and_in_a_replayed_graph(seqs):
             g.replay()
             torch.cuda.synchronize()
             assert all(torch.equal(x[:n], y) for x, y in zip(res, eager)), f"replay {rep}"
+
+
+# ------------------------------------------------------------------------- values that are not finite where every row sees them
+@pytest.mark.parametrize("hn,dtype", [(64, F16), (128, BF16), (128, F16)])
+@pytest.mark.parametrize("n,l", [(1, 90), (6, 300), (1, 5000), (40, 300), (150, 700), (40, 3000)])
+@pytest.mark.parametrize("spread", [1.0, 60.0])
+def test_attention_nonfinite_values_that_every_row_sees(hn, dtype, n, l, spread):
+    """p > 0 times an infinity is that infinity, also where p rounds to 0 (in 16 bits or, at the wide spread of scores, in 32) and
+    whichever split or wave it meets; infinities of both signs or a NaN in one dim make it NaN."""
+    c = Case([(n, l), (3, 200), (1, 33)], nq=2, nkv=1, hn=hn, ps=16, dtype=dtype)
+    c.q = (c.q.float() * spread).to(dtype)
+    inf = float("inf")
+    for p, d, x in ((2, 3, inf), (37, 3, inf), (41, 9, -inf), (70, 20, inf), (11, 20, -inf), (l - n, hn - 1, float("nan"))):
+        c.v_cache[c.block_table[0, p // 16], 0, p % 16, d] = x
+    check_attention(c, *run_attention(c))
+
+
+@pytest.mark.parametrize("n", [1, 40])
+def test_attention_lengths_below_zero(n):
+    """A length below the new rows, down to the smallest number: the rows see nothing."""
+    c = Case([(n, -3), (n, 100), (n, -2 ** 31)], nq=2, nkv=2, hn=64, ps=16, dtype=BF16, pad=1, garbage=float("nan"))
+    check_attention(c, *run_attention(c))
+    check_attention(c, *run_attention(c, max_kv=9000))
+
+
+def test_nothing_to_do():
+    """No rows, no sequences, sequences without rows: nothing is written and nothing fails."""
+    from multimodal_amd import ops
+    from multimodal_amd.kv_cache import PagedStep
+    c = Case([(0, 5), (0, 40)], nq=4, nkv=2, hn=64, ps=16, dtype=BF16)
+    for step in (c.step(), PagedStep(torch.empty(0, 4, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda"),
+                                     torch.empty(0, dtype=torch.int32, device="cuda"))):
+        kv = c.kv()
+        kv_rows = torch.empty(0, 2, 64, dtype=BF16, device="cuda")
+        q = torch.empty(0, 4, 64, dtype=BF16, device="cuda")
+        assert ops.paged_kv_append(kv, step, kv_rows, kv_rows.clone(), q=q).shape == (0, 4, 64)
+        assert ops.paged_kv_append(kv, step, kv_rows, kv_rows.clone()) is None
+        out, lse = ops.paged_attn_fwd(kv, step, q, c.scale)
+        assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+        torch.cuda.synchronize()
+        assert torch.equal(kv.k.cpu(), c.k_cache) and torch.equal(kv.v.cpu(), c.v_cache)
+
+
+def test_outputs_that_overlap_themselves_are_refused():
+    from multimodal_amd import ops
+    c = Case([(2, 9)], nq=2, nkv=2, hn=64, ps=16, dtype=BF16)
+    one = torch.zeros(1, 2, 64, dtype=BF16, device="cuda").expand(2, 2, 64)
+    with pytest.raises(RuntimeError, match="overlap"):
+        ops.paged_attn_fwd(c.kv(), c.step(), c.q.cuda(), c.scale, out=one)
+    with pytest.raises(RuntimeError, match="overlap"):
+        ops.paged_attn_fwd(c.kv(), c.step(), c.q.cuda(), c.scale, lse=torch.zeros(1, 2, device="cuda").expand(2, 2))
+    with pytest.raises(RuntimeError, match="overlap"):
+        ops.paged_kv_append(c.kv(), c.step(), c.k.cuda(), c.v.cuda(), q=c.q.cuda(), q_out=one)
+
+
+def test_cache_steps_that_make_no_sense_are_refused():
+    from multimodal_amd.kv_cache import PagedKVCache, PagedStep
+    cache = PagedKVCache(1, 2, 64, num_pages=8, page_size=4)
+    a, b = cache.add(8), cache.add(3)
+    with pytest.raises(RuntimeError, match="twice"):
+        cache.step([a, b, a], [1, 1, 1], [3, 2, 4])
+    with pytest.raises(RuntimeError, match="numbers"):
+        cache.step([a, b], [1], [3, 2])
+    with pytest.raises(RuntimeError, match="no sequence"):
+        cache.step([a, 99], [1, 1], [3, 2])
+    for bad in (lambda: cache.release(99), lambda: cache.reserve(99, 4), lambda: cache.block_table([99])):
+        with pytest.raises(RuntimeError, match="no sequence"):
+            bad()
+    cache.release(b)
+    with pytest.raises(RuntimeError, match="no sequence"):
+        cache.release(b)
+    assert cache.free_pages == 6
+    s = cache.step([a], [1], [3])
+    with pytest.raises(RuntimeError, match="max_kv"):
+        PagedStep(s.block_table, s.cu_new, s.kv_lens, max_new=1, max_kv=2 ** 32 + 3)
