@@ -418,6 +418,11 @@ __device__ __forceinline__ void paged_attn_many(const PagedAttnArgs& a, char* sm
     typedef KvTile<HD> TL;
     typedef typename M32<T>::frag frag;
     constexpr int NDS = HD / 16, NDB = HD / 32, NT = 64 * NWV, NCH = 64 * TL::CPR / NT, ROWS = 32 * NWV;
+    constexpr bool AHEAD = HD == 64 || NWV == 8;
+    constexpr int KG = HD == 128 ? 2 : 4;  // key fragments read ahead
+    auto fence = []() __attribute__((always_inline)) {
+        if constexpr (AHEAD) __builtin_amdgcn_sched_barrier(0);
+    };
     // two stages of K | V, then per ring slot (tile & 3) a 64-bit mask of the keys in pages the cache does not have, and whether
     // values that are not finite have been taken out of the products, and whether an output is not finite
     unsigned long long* flags = reinterpret_cast<unsigned long long*>(smem + 4 * TL::BYTES);
@@ -539,11 +544,33 @@ __device__ __forceinline__ void paged_attn_many(const PagedAttnArgs& a, char* sm
             f32x16 sacc[2];
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sacc[t][i] = 0.f;
+            frag kf[2][KG], vf[2][NDB];
+            auto load_k = [&](int grp, frag (&f)[KG]) __attribute__((always_inline)) {
 #pragma unroll
-                for (int ds = 0; ds < NDS; ++ds) sacc[t] = M32<T>::run(k_frag(ks, t, ds), qf[ds], sacc[t]);
+                for (int i = 0; i < KG; ++i) f[i] = k_frag(ks, (grp * KG + i) & 1, (grp * KG + i) >> 1);
+                fence();
+            };
+            auto load_v = [&](int grp, frag (&f)[NDB]) __attribute__((always_inline)) {
+#pragma unroll
+                for (int d = 0; d < NDB; ++d) f[d] = v_frag(vs, 16 * grp, d);
+                fence();
+            };
+            // Fragments are read from LDS a group ahead of the matrix instructions that take them (the fences keep the compiler from
+            // moving the reads back to their use, where each waits out the LDS latency), the first values' behind the softmax: 1024
+            // tokens over 17k, 32 / 8 heads of 128: 325 -> 300 us.  In 4 waves of 128 it takes registers that are not there (32 x 100 tokens
+            // over 1.8k, 16 heads: 115 -> 123): the compiler's order stays.
+            fence();
+            load_k(0, kf[0]);
+#pragma unroll
+            for (int grp = 0; grp < 2 * NDS / KG; ++grp) {
+                if (grp + 1 < 2 * NDS / KG) load_k(grp + 1, kf[(grp + 1) & 1]);
+                else load_v(0, vf[0]);
+#pragma unroll
+                for (int i = 0; i < KG; ++i) sacc[(grp * KG + i) & 1] = M32<T>::run(kf[grp & 1][i], qf[(grp * KG + i) >> 1], sacc[(grp * KG + i) & 1]);
+                fence();
             }
             __builtin_amdgcn_s_setprio(0);
             if (badk[0] | badk[1]) {
@@ -594,11 +621,12 @@ __device__ __forceinline__ void paged_attn_many(const PagedAttnArgs& a, char* sm
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int s2 = 0; s2 < 2; ++s2) {
+                    if (2 * t + s2 < 3) load_v(2 * t + s2 + 1, vf[(s2 + 1) & 1]);
                     const frag pf = M32<T>::cvt8(sacc[t][8 * s2], sacc[t][8 * s2 + 1], sacc[t][8 * s2 + 2], sacc[t][8 * s2 + 3],
                                                  sacc[t][8 * s2 + 4], sacc[t][8 * s2 + 5], sacc[t][8 * s2 + 6], sacc[t][8 * s2 + 7]);
 #pragma unroll
-                    for (int d = 0; d < NDB; ++d)
-                        o[d] = M32<T>::run(v_frag(vs, 32 * t + 16 * s2, d), pf, o[d]);
+                    for (int d = 0; d < NDB; ++d) o[d] = M32<T>::run(vf[s2][d], pf, o[d]);
+                    fence();
                 }
             __builtin_amdgcn_s_setprio(0);
         }
