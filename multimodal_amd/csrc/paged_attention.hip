@@ -32,7 +32,10 @@ struct PagedAttnArgs {
     float scale_log2e;
     FastDiv page, grp;
     int few_chunk, few_splits, many_chunk, many_splits;  // keys per split (a multiple of the tiles) and splits, by kind of sequence
-    float *ws_o, *ws_ml;  // more than one split: [splits, rows, nq, hn] unnormalised outputs, [splits, rows, nq, 2] (max, sum)
+    // More than one split: unnormalised outputs [splits, .., hn] and (max, sum) [splits, .., 2] of [seqs, heads, few_rows] in the few-row
+    // form and of [rows, nq] in the other, so that a long chunk beside single tokens is not kept once a split of theirs.
+    int few_rows;
+    float *few_o, *few_ml, *many_o, *many_ml;
 };
 
 // How far a score may exceed the running reference of a row's exponentials (in powers of two) before the row is rescaled
@@ -384,13 +387,13 @@ __device__ __forceinline__ void paged_attn_few(const PagedAttnArgs& a, char* sme
             *reinterpret_cast<u32x4*>(a.out + (int64_t)grow * a.o_row + (int64_t)h * a.o_head + d0) = pack8<T>(acc);
             if (d0 == 0) a.lse[(int64_t)grow * a.l_row + h] = (M + __log2f(L)) * kLn2;
         } else {
-            const int64_t at = ((int64_t)split * a.rows + grow) * a.nq + h;
-            f32x4* dst = reinterpret_cast<f32x4*>(a.ws_o + at * HD + d0);
+            const int64_t at = (((int64_t)split * a.st.seqs + seq) * a.kv.heads + kh) * a.few_rows + row;
+            f32x4* dst = reinterpret_cast<f32x4*>(a.few_o + at * HD + d0);
             dst[0] = f32x4{acc[0], acc[1], acc[2], acc[3]};
             dst[1] = f32x4{acc[4], acc[5], acc[6], acc[7]};
             if (d0 == 0) {
-                a.ws_ml[2 * at] = M;
-                a.ws_ml[2 * at + 1] = L;
+                a.few_ml[2 * at] = M;
+                a.few_ml[2 * at + 1] = L;
             }
         }
     }
@@ -694,15 +697,15 @@ __device__ __forceinline__ void paged_attn_many(const PagedAttnArgs& a, char* sm
         if (hh == 0) a.lse[(int64_t)grow * a.l_row + qh] = (m_run + __log2f(l_tot)) * kLn2;
     } else {
         const int64_t at = ((int64_t)split * a.rows + grow) * a.nq + qh;
-        float* orow = a.ws_o + at * HD;
+        float* orow = a.many_o + at * HD;
 #pragma unroll
         for (int d = 0; d < NDB; ++d)
 #pragma unroll
             for (int g4 = 0; g4 < 4; ++g4)
                 *reinterpret_cast<f32x4*>(orow + 32 * d + 8 * g4 + 4 * hh) = f32x4{o[d][4 * g4], o[d][4 * g4 + 1], o[d][4 * g4 + 2], o[d][4 * g4 + 3]};
         if (hh == 0) {
-            a.ws_ml[2 * at] = m_run;
-            a.ws_ml[2 * at + 1] = l_tot;
+            a.many_ml[2 * at] = m_run;
+            a.many_ml[2 * at + 1] = l_tot;
         }
     }
 }
@@ -752,18 +755,21 @@ template <typename T, int HD> __global__ __launch_bounds__(256) void paged_attn_
     const int chunk = few ? a.few_chunk : a.many_chunk, splits = few ? a.few_splits : a.many_splits;
     if (splits == 1) return;  // written by the main kernel
     const int ns = min(splits, max(1, (len + chunk - 1) / chunk));
-    const int64_t step = (int64_t)a.rows * a.nq;
+    const int kh = (int)fdiv((uint32_t)h, a.grp);
+    const int64_t at = few ? ((int64_t)seq * a.kv.heads + kh) * a.few_rows + (row - beg) * a.group + h - kh * a.group : id;
+    const int64_t step = few ? (int64_t)a.st.seqs * a.kv.heads * a.few_rows : (int64_t)a.rows * a.nq;
+    const float *ws_o = few ? a.few_o : a.many_o, *ws_ml = few ? a.few_ml : a.many_ml;
     float M = -INFINITY, L = 0.f, acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int i = lane; i < ns; i += 64) M = fmaxf(M, a.ws_ml[2 * (id + i * step)]);
+    for (int i = lane; i < ns; i += 64) M = fmaxf(M, ws_ml[2 * (at + i * step)]);
     M = wave_max(M);
     const float mu = M == -INFINITY ? 0.f : M;
     for (int i0 = 0; i0 < ns; i0 += 64) {  // a lane has the factor of one split; the outputs of 8 splits are in flight
         const int n = min(ns - i0, 64);
         float w = 0.f;
         if (lane < n) {
-            const float m = a.ws_ml[2 * (id + (i0 + lane) * step)], l = a.ws_ml[2 * (id + (i0 + lane) * step) + 1];
+            const float m = ws_ml[2 * (at + (i0 + lane) * step)], l = ws_ml[2 * (at + (i0 + lane) * step) + 1];
             w = m == -INFINITY && l == 0.f ? 0.f : fast_exp2(m - mu);
             L += w == 0.f && l == l ? 0.f : w * l;
         }
@@ -772,7 +778,7 @@ template <typename T, int HD> __global__ __launch_bounds__(256) void paged_attn_
 #pragma unroll
             for (int u = 0; u < 8; ++u)
 #pragma unroll
-                for (int e = 0; e < E; ++e) v[u][e] = a.ws_o[(id + min(i0 + i + u, ns - 1) * step) * HD + E * lane + e];
+                for (int e = 0; e < E; ++e) v[u][e] = ws_o[(at + min(i0 + i + u, ns - 1) * step) * HD + E * lane + e];
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 const float f = __shfl(w, min(i + u, 63), 64);
@@ -794,7 +800,13 @@ template <typename T, int HD> __global__ __launch_bounds__(256) void paged_attn_
 struct PagedPlan {
     bool few;
     int waves, row_blocks, few_chunk, few_splits, many_chunk, many_splits;
-    int splits() const { return few_splits > many_splits ? few_splits : many_splits; }
+    int few_rows;
+    // rows of partial results
+    int64_t few_partials(const mm_paged_kv& kv, const mm_paged_step& st) const { return few_splits > 1 ? (int64_t)few_splits * st.seqs * kv.heads * few_rows : 0; }
+    int64_t many_partials(int rows, int nq) const { return many_splits > 1 ? (int64_t)many_splits * rows * nq : 0; }
+    size_t bytes(const mm_paged_kv& kv, const mm_paged_step& st, int rows, int nq) const {
+        return (size_t)(few_partials(kv, st) + many_partials(rows, nq)) * (kv.hn + 2) * sizeof(float);
+    }
 };
 // Splits while a launch has too few workgroups: as many as keep one resident set (`target`), none shorter than `least` keys
 static void split_keys(int64_t wgs, int64_t target, int64_t least, int64_t gran, int max_kv, int& chunk, int& splits) {
@@ -813,6 +825,7 @@ static PagedPlan plan(const mm_paged_kv& kv, const mm_paged_step& st, int nq) {
     const int group = nq / kv.heads;
     const int64_t rows = (int64_t)st.max_new * group, pairs = (int64_t)st.seqs * kv.heads;
     p.few = rows <= kFewRows;
+    p.few_rows = p.few ? (int)rows : kFewRows;
     // Few rows: one workgroup of 8 waves a CU.  With more, smaller ones the same bytes are in flight in more places at once: 2 x 131071
     // keys of 4 heads of 128: 162 us with 1024 workgroups of 4 waves, 133 with 512, 112 with 256 of 8.
     // Many rows: 128 a workgroup.  At head size 128 the registers hold two waves a SIMD whatever the workgroup's size, and one of 8
@@ -840,7 +853,7 @@ template <typename T, int HD> static int launch_paged_attn(const PagedAttnArgs& 
         else paged_attn_any_k<T, 128, 4><<<grid, 256, 0, st>>>(a, p.row_blocks);
     } else paged_attn_any_k<T, 64, 4><<<grid, 256, 0, st>>>(a, p.row_blocks);
     MM_CHECK_LAUNCH();
-    if (p.splits() > 1) {
+    if (p.few_splits > 1 || p.many_splits > 1) {
         paged_attn_join_k<T, HD><<<(unsigned)(((int64_t)a.rows * a.nq + 3) / 4), 256, 0, st>>>(a);
         MM_CHECK_LAUNCH();
     }
@@ -865,7 +878,7 @@ using namespace mm;
 extern "C" size_t mm_paged_attn_workspace_bytes(const mm_paged_kv* kv, const mm_paged_step* step, int nq, int rows) {
     if (check_paged_attn("mm_paged_attn_workspace_bytes", kv, step, nq, rows) != MM_OK) return 0;
     const PagedPlan p = plan(*kv, *step, nq);
-    return p.splits() == 1 ? 0 : (size_t)p.splits() * rows * nq * (kv->hn + 2) * sizeof(float);
+    return p.bytes(*kv, *step, rows, nq);
 }
 
 extern "C" int mm_paged_attn_fwd(const mm_paged_kv* kv, const mm_paged_step* step, void* out, int64_t o_row, int64_t o_head, float* lse,
@@ -879,7 +892,7 @@ extern "C" int mm_paged_attn_fwd(const mm_paged_kv* kv, const mm_paged_step* ste
                  "%s: q / out must be 16-byte aligned with strides a multiple of 8", fn);
     MM_CHECK_ARG(softmax_scale > 0.f, "%s: softmax_scale %g must be positive", fn, (double)softmax_scale);
     const PagedPlan p = plan(*kv, *step, nq);
-    const size_t need = p.splits() == 1 ? 0 : (size_t)p.splits() * rows * nq * (kv->hn + 2) * sizeof(float);
+    const size_t need = p.bytes(*kv, *step, rows, nq);
     MM_CHECK_ARG(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need),
                  "%s: workspace of %zu bytes needed (16-byte aligned), got %zu", fn, need, workspace ? workspace_bytes : (size_t)0);
     MM_CHECK_ARG(need == 0 || (int64_t)rows * nq < (int64_t)1 << 26, "%s: %d rows of %d heads exceed the joining launch's grid", fn, rows, nq);
@@ -892,8 +905,13 @@ extern "C" int mm_paged_attn_fwd(const mm_paged_kv* kv, const mm_paged_step* ste
     a.scale_log2e = softmax_scale * kLog2e;
     a.page = make_fastdiv(kv->page_size), a.grp = make_fastdiv(a.group);
     a.few_chunk = p.few_chunk, a.few_splits = p.few_splits, a.many_chunk = p.many_chunk, a.many_splits = p.many_splits;
-    a.ws_o = (float*)workspace;
-    a.ws_ml = need ? a.ws_o + (size_t)p.splits() * rows * nq * kv->hn : nullptr;
+    a.few_rows = p.few_rows;
+    if (need) {
+        a.few_o = (float*)workspace;
+        a.many_o = a.few_o + p.few_partials(*kv, *step) * kv->hn;
+        a.few_ml = a.many_o + p.many_partials(rows, nq) * kv->hn;
+        a.many_ml = a.few_ml + p.few_partials(*kv, *step) * 2;
+    }
     hipStream_t st = (hipStream_t)stream;
     return dispatch_dtype(kv->dtype, [&](auto t) -> int {
         using T = decltype(t);

@@ -145,3 +145,12 @@ def test_generated_rows_end_with_the_end_token_or_a_failed_draw():
     out = torch.tensor([[5, 7, 9, 1], [3, -1, 9, 2], [8, 4, 3, 3], [3, 3, -1, 4]])
     assert [r.tolist() for r in _trim(out, 3)] == [[5, 3], [7, -1], [9, 9, 3], [1, 2, 3]]
     assert [r.tolist() for r in _trim(out, None)] == [[5, 3, 8, 3], [7, -1], [9, 9, 3, -1], [1, 2, 3, 4]]
+
+
+def test_workspace_of_a_long_chunk_is_not_multiplied_by_the_single_tokens_splits():
+    """The few-row form's partial results are kept for at most 16 rows a sequence and key head."""
+    lib = _lib.get_lib()
+    step = dict(seqs=1, max_new=8192, max_kv=131072, max_pages=8192, table_stride=8192)
+    a, b, pa, pb = refs(kv=dict(hn=128, heads=8, page=8 * 16 * 128, head=16 * 128, slot=128), step=step)
+    need = lib.mm_paged_attn_workspace_bytes(pa, pb, 32, 8192)
+    assert 0 < need <= 32 * 8 * 16 * 130 * 4
