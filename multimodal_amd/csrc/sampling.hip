@@ -11,14 +11,19 @@
 //
 // One workgroup of 16 waves per row.  Its histogram (a count of a non-negative value in the low half of a word, of a negative one
 // in the high half; 130 KB) fills most of a CU's LDS.  Steps: (1) the row into registers, each wave a contiguous 16th of it (the
-// search by index needs that), and its largest value; (2) one LDS atomic per logit; (3) count and weight of every 64 neighbouring
-// values ("chunk"), one thread a chunk: the values of a chunk share their exponent and are evenly spaced, so their weights are a
-// geometric sequence and the chunk's weight is a polynomial, sum n_i r^i, by Horner's rule - two exponentials a chunk instead of one
-// a value.  A chunk takes 65 words of LDS, so that 64 lanes walking 64 chunks in step meet 64 banks; (4) a scan over the 1024 chunks;
-// (5) one wave finds the borders: 64-way search for the chunk, a scan over its 64 values; (6) the j-th match of the value found.
-// With a top-k of at most 512, what can be among the first k is listed and ranked instead of (2) to (6).
+// search by index needs that), one LDS atomic per logit as it arrives, and its largest value; (2) count and weight of every 64
+// neighbouring values ("chunk"), one thread a chunk: the values of a chunk share their exponent and are evenly spaced, so their weights
+// are a geometric sequence and the chunk's weight is a polynomial, sum n_i r^i, by Horner's rule - two exponentials a chunk instead of
+// one a value.  A chunk takes 65 words of LDS, so that 64 lanes walking 64 chunks in step meet 64 banks; (3) a scan over the 1024
+// chunks; (4) one wave finds the borders: 64-way search for the chunk, a scan over its 64 values; (5) the j-th match of the value found.
+// With a top-k of at most 512, what can be among the first k is listed and ranked instead of counted.
 // Rows of more than 65528 logits (BIG) could overflow 16-bit counts: they count non-negative and negative values one after the
 // other in 32 bits, re-read the row instead of keeping it, and recount a chunk when a border falls into it.
+//
+// Bound by a row's chain of steps in one CU, not by HBM.  50304 fp16 logits, cycles: row and LDS atomics (1024 wave instructions) 11400,
+// chunk sums 5300 (vector instructions), scan 1600, borders 5600, match 4400; the list instead of all of that 12000.  Kernel times:
+// one row of bf16 with top-k 40: 9.2 us; 64 rows, top-p and min-p: 17 us; 512 rows with parameters of their own (two
+// rows a CU after each other): 35 us, 51.5 MB at 1.5 TB/s.
 #include "common.h"
 
 namespace mm {
@@ -194,11 +199,42 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
         u32x4* h = reinterpret_cast<u32x4*>(sm.hist);
         for (int i = tid; i < 512 * 65 / 4; i += kSampleThreads) h[i] = u32x4{0, 0, 0, 0};
     };
-    if (!greedy && (BIG || k <= 0 || k > kSampleThreads / 2)) clear_hist();
+    const bool try_list = !BIG && !greedy && k > 0 && k <= kSampleThreads / 2;
+    if (!greedy && !try_list) clear_hist();
+    us2 lo2 = {0xffff, 0xffff}, hi2 = {0, 0};
+    auto ends_of = [&](uint32_t o) {
+        lo2 = pk_min(lo2, __builtin_bit_cast(us2, o));
+        hi2 = __builtin_elementwise_max(hi2, __builtin_bit_cast(us2, o));
+    };
+    auto count2 = [&](uint32_t o) {  // hist_word of both halves at once
+        const uint32_t w = (o & 0x7fff7fffu) + ((o >> 6) & 0x01ff01ffu);
+        uint32_t s0 = __builtin_amdgcn_ubfe(o, 15, 1), s1 = o >> 31;
+        asm("" : "+v"(s0), "+v"(s1));  // keep the signs numbers: a compare and a select each cost more
+        atomicAdd(&sm.hist[w & 0xffffu], __umul24(s0, 0xffffu) + 1u);
+        atomicAdd(&sm.hist[w >> 16], __umul24(s1, 0xffffu) + 1u);
+    };
     if constexpr (!BIG) {
+        if (!greedy && !try_list) {  // counted as it arrives: the vector work hides behind the LDS atomics
+            __syncthreads();
 #pragma unroll
-        for (int s = 0; s < kSampleSteps; ++s)
-            if (s < steps && ch0 + 64 * s + lane < ch1) reg[s] = ordered(reg[s], ch0 + 64 * s + lane);
+            for (int s = 0; s < kSampleSteps; ++s)
+                if (s < steps && ch0 + 64 * s + lane < ch1) {
+                    reg[s] = ordered(reg[s], ch0 + 64 * s + lane);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        count2(reg[s][i]);
+                        ends_of(reg[s][i]);
+                    }
+                }
+        } else {
+#pragma unroll
+            for (int s = 0; s < kSampleSteps; ++s)
+                if (s < steps && ch0 + 64 * s + lane < ch1) {
+                    reg[s] = ordered(reg[s], ch0 + 64 * s + lane);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) ends_of(reg[s][i]);
+                }
+        }
     }
     // f(two places in the order) over this thread's logits
     auto each2 = [&](auto&& f) {
@@ -218,11 +254,7 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
         }
     };
 
-    us2 lo2 = {0xffff, 0xffff}, hi2 = {0, 0};
-    each2([&](uint32_t o) {
-        lo2 = pk_min(lo2, __builtin_bit_cast(us2, o));
-        hi2 = __builtin_elementwise_max(hi2, __builtin_bit_cast(us2, o));
-    });
+    if constexpr (BIG) each2(ends_of);
     hi2 = ~hi2;
     const us2 mine2 = pk_min(us2{lo2[0], hi2[0]}, us2{lo2[1], hi2[1]});  // {smallest, complement of the largest} place of this thread
     {
@@ -253,7 +285,7 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
         sm.count[tid] = 0;
         sm.mass[tid] = 0.0;
         bool listed = false;
-        if (!BIG && k > 0 && k <= kSampleThreads / 2) {
+        if (try_list) {
             // The k-th largest of the threads' largest logits bounds the k-th largest logit from below: what lies in a later chunk
             // is not among the first k (50304 logits, k = 64: some 0.3 % are left).
             __syncthreads();
@@ -376,18 +408,12 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
             }
         };
         if constexpr (!BIG) {
-            if (k > 0 && k <= kSampleThreads / 2) {  // the list has been where the counts go
+            if (try_list) {  // the list has been where the counts go
                 __syncthreads();
                 clear_hist();
                 __syncthreads();
+                each2(count2);
             }
-            each2([&](uint32_t o) {  // hist_word of both halves at once
-                const uint32_t w = (o & 0x7fff7fffu) + ((o >> 6) & 0x01ff01ffu);
-                uint32_t s0 = __builtin_amdgcn_ubfe(o, 15, 1), s1 = o >> 31;
-                asm("" : "+v"(s0), "+v"(s1));  // keep the signs numbers: a compare and a select each cost more
-                atomicAdd(&sm.hist[w & 0xffffu], __umul24(s0, 0xffffu) + 1u);
-                atomicAdd(&sm.hist[w >> 16], __umul24(s1, 0xffffu) + 1u);
-            });
             __syncthreads();
             if (tid == 0) {  // -0 is +0
                 const uint32_t z = sm.hist[hist_word(kMinusZero)] >> 16;
