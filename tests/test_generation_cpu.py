@@ -127,7 +127,7 @@ def test_launches_beyond_the_grid_are_refused():
     assert rc == -1 and "grid" in msg
     rc, msg = attend(step=dict(seqs=1 << 21))
     assert rc == -1 and "grid" in msg
-    big = dict(max_kv=5000, max_pages=512, table_stride=512, seqs=1)
+    big = dict(max_kv=5000, max_new=100, max_pages=512, table_stride=512, seqs=1)  # the long axis is split, and its rows joined
     a, b, pa, pb = refs(step=big)
     need = lib.mm_paged_attn_workspace_bytes(pa, pb, 4, 1 << 24)
     rc, msg = attend(step=big, rows=1 << 24, ws=4096, ws_bytes=need)
