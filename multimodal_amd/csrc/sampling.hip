@@ -21,9 +21,9 @@
 // other in 32 bits, re-read the row instead of keeping it, and recount a chunk when a border falls into it.
 //
 // Bound by a row's chain of steps in one CU, not by HBM.  50304 fp16 logits, cycles: row and LDS atomics (1024 wave instructions) 11400,
-// chunk sums 5300 (vector instructions), scan 1600, borders 5600, match 4400; the list instead of all of that 12000.  Kernel times:
-// one row of bf16 with top-k 40: 9.2 us; 64 rows, top-p and min-p: 17 us; 512 rows with parameters of their own (two
-// rows a CU after each other): 35 us, 51.5 MB at 1.5 TB/s.
+// chunk sums 5300 (vector instructions), scan 1600, borders 4300, match 2400; the list instead of all of that 12000.  Kernel times:
+// one row of bf16 with top-k 40: 9.2 us; 64 rows, top-p and min-p: 15 us; 512 rows with parameters of their own (two
+// rows a CU after each other): 30 us, 51.5 MB at 1.7 TB/s.
 #include "common.h"
 
 namespace mm {
@@ -136,6 +136,7 @@ struct SampleShared {
     double wave_mass[kSampleWaves];
     uint32_t wave_count[kSampleWaves];
     us2 wave_ends[kSampleWaves];
+    double min_p_mass;
     int dk, j;
     uint32_t one_chunk[64];
     uint32_t listed;
@@ -456,8 +457,9 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
             __syncthreads();
         }
 
-        // Borders.  One wave (BIG: every wave alike, because recounting a chunk takes the whole workgroup).
-        if (BIG || wave == 0) {
+        // Borders.  One wave, a second one for min-p beside it (BIG: every wave alike, because recounting a chunk takes the whole
+        // workgroup).
+        {
             auto counts = [&](int c) -> uint32_t {
                 if constexpr (!BIG) return (sm.hist[(c & 511) * 65 + lane] >> (c < 512 ? 0 : 16)) & 0xffffu;
                 __syncthreads();
@@ -495,20 +497,7 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
                 const double up = before + (jj + 1.0) * w;
                 return Found{64 * c + l, (int)lane_u((uint32_t)(int)jj, l), lane_d(up, l)};
             };
-            double z = sm.mass[kChunks - 1];
-            if (k > 0 && (uint32_t)k < sm.count[kChunks - 1]) {
-                const int c = first_of([&](int i) { return sm.count[i] >= (uint32_t)k; });
-                const uint32_t n = counts(c);
-                const double w = n ? wt.at(64 * c + lane) : 0.0;
-                const uint32_t ci = (c ? sm.count[c - 1] : 0u) + scan_u(n);
-                const double mi = (c ? sm.mass[c - 1] : 0.0) + scan_d((double)n * w);
-                const uint64_t over = __ballot(n != 0 && ci >= (uint32_t)k);
-                const int l = over ? __builtin_ctzll(over) : 63;
-                z = fmin(z, lane_d(mi - (double)(ci - (uint32_t)k) * w, l));
-            }
-            double zp = z;
-            if (p > 0.f && p < 1.f) zp = fmin(zp, find((double)p * z).upto);
-            if (mp > 0.f) {
+            auto min_p_mass = [&]() -> double {
                 // the first value whose weight is below min_p: 64-way search in the order
                 const double floor_w = fmin((double)mp, 1.0);
                 int from = lo, span = 65536 - lo;
@@ -525,15 +514,39 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
                 const uint32_t n = counts(c);
                 const double w = n ? wt.at(64 * c + lane) : 0.0;
                 const double mi = scan_d(64 * c + lane < from ? (double)n * w : 0.0);
-                zp = fmin(zp, (c ? sm.mass[c - 1] : 0.0) + lane_d(mi, 63));
+                return (c ? sm.mass[c - 1] : 0.0) + lane_d(mi, 63);
+            };
+            if (!BIG && wave == 1 && mp > 0.f) {
+                const double m = min_p_mass();
+                if (lane == 0) sm.min_p_mass = m;
             }
-            zp = fmax(zp, 1.0);
-            double t = (double)u * zp;
-            if (!(t < zp)) t = __longlong_as_double(__double_as_longlong(zp) - 1);  // u of 1 or more: the last token kept
-            const Found f = find(t);
-            if (BIG || lane == 0) {
-                sm.dk = f.dk;
-                sm.j = f.j;
+            double zp = 0.0;
+            if (BIG || wave == 0) {
+                double z = sm.mass[kChunks - 1];
+                if (k > 0 && (uint32_t)k < sm.count[kChunks - 1]) {
+                    const int c = first_of([&](int i) { return sm.count[i] >= (uint32_t)k; });
+                    const uint32_t n = counts(c);
+                    const double w = n ? wt.at(64 * c + lane) : 0.0;
+                    const uint32_t ci = (c ? sm.count[c - 1] : 0u) + scan_u(n);
+                    const double mi = (c ? sm.mass[c - 1] : 0.0) + scan_d((double)n * w);
+                    const uint64_t over = __ballot(n != 0 && ci >= (uint32_t)k);
+                    const int l = over ? __builtin_ctzll(over) : 63;
+                    z = fmin(z, lane_d(mi - (double)(ci - (uint32_t)k) * w, l));
+                }
+                zp = z;
+                if (p > 0.f && p < 1.f) zp = fmin(zp, find((double)p * z).upto);
+            }
+            if (!BIG) __syncthreads();
+            if (BIG || wave == 0) {
+                if (mp > 0.f) zp = fmin(zp, BIG ? min_p_mass() : sm.min_p_mass);
+                zp = fmax(zp, 1.0);
+                double t = (double)u * zp;
+                if (!(t < zp)) t = __longlong_as_double(__double_as_longlong(zp) - 1);  // u of 1 or more: the last token kept
+                const Found f = find(t);
+                if (BIG || lane == 0) {
+                    sm.dk = f.dk;
+                    sm.j = f.j;
+                }
             }
         }
         __syncthreads();
@@ -549,14 +562,15 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
         if (dk == kPlusZero) m |= ((o & 0xffffu) == kMinusZero ? 1u : 0u) | ((o >> 16) == kMinusZero ? 2u : 0u);
         return m;
     };
-    us2 some = {1, 1};  // 0 where a half has been equal
-    each2([&](uint32_t o) { some = pk_min(some, __builtin_bit_cast(us2, o ^ want)); });
-    uint32_t tot = 0;
-    if (dk == kPlusZero || __ballot(some[0] == 0 || some[1] == 0)) {
-        uint32_t mine = 0;
+    uint32_t mine = 0;
+    if (dk == kPlusZero || BIG) {
         each2([&](uint32_t o) { mine += __popc(matches(o)); });
-        tot = lane_u(scan_u(mine), 63);
+    } else {  // both halves of a word at once: 1 - 0 where they are equal, else 1 - 1 or more, saturated
+        us2 equal = {0, 0};
+        each2([&](uint32_t o) { equal += __builtin_elementwise_sub_sat(us2{1, 1}, __builtin_bit_cast(us2, o ^ want)); });
+        mine = (uint32_t)equal[0] + equal[1];
     }
+    const uint32_t tot = lane_u(scan_u(mine), 63);
     if (lane == 0) sm.wave_count[wave] = tot;  // its readers of the scan above have passed a barrier since
     __syncthreads();
     const uint32_t before = lane_u(row_sum_u((lane & 15) < wave ? sm.wave_count[lane & 15] : 0u), 15);
