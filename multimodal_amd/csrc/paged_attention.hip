@@ -98,6 +98,8 @@ template <typename T> __device__ __forceinline__ float only_nonfinite(const u16*
 __device__ __forceinline__ bool nonfinite(float x) { return !(x - x == 0.f); }
 // w * x where w stands for a positive weight that may have become 0
 __device__ __forceinline__ float weigh(float w, float x) { return w != 0.f ? w * x : nonfinite(x) ? x : 0.f; }
+// the same of a sum of weights: a NaN stays
+__device__ __forceinline__ float weigh_sum(float w, float l) { return w == 0.f && l == l ? 0.f : w * l; }
 // add(key, its value row) for the keys of [k0, k1) whose value rows hold infinities or NaN; a whole wave calls it
 template <typename T, int HD, typename F>
 __device__ __forceinline__ void each_nonfinite(const PagedAttnArgs& a, const int32_t* __restrict__ bt, int kh, int k0, int k1, F&& add) {
@@ -141,7 +143,7 @@ template <> struct M16<F16> {
 //   O^T[dim][row] += V^T P^T: P^T is S^T's registers as they stand - register j of sub-tile t in group g is key 16 t + 4 g + j,
 //   and the V^T operand takes its keys in that order - V through a wave-private LDS tile, read transposed (ds_read_b64_tr_b16).
 // Measured: 64 sequences of 5 .. 2047 keys, 32 heads of 128 in bf16: 198 us, 1.08 GB at 5.5 TB/s; 2 of 131k, 32 / 4 heads: 97 us with
-// the joining, 5.2 TB/s; one of 701, 16 heads of 64: 9.5 us, the latency of one workgroup's chain of loads.
+// the joining, 5.2 TB/s; one of 701, 16 heads of 64: 10 us, the latency of one workgroup's chain of loads.
 // The LDS rows are unpadded; the 32-byte units of a row are XOR-ed with the row so that the transposed reads (16 rows, one unit
 // each) and the writes (16 rows, two units each) spread evenly over the banks.
 template <int HD> __device__ __forceinline__ int v_off(int row, int byte) {
@@ -373,11 +375,9 @@ __device__ __forceinline__ void paged_attn_few(const PagedAttnArgs& a, char* sme
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc[e] = 0.f;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const float m = sm_m[w][row];
-            if (m == -INFINITY && sm_l[w][row] == 0.f) continue;  // a wave without a key
-            const float al = fast_exp2(m - mu);
-            L += al * sm_l[w][row];
+        for (int w = 0; w < NW; ++w) {  // a wave without a key has the maximum -inf and zeros
+            const float al = fast_exp2(sm_m[w][row] - mu);
+            L += weigh_sum(al, sm_l[w][row]);
             const float* src = red + (w * 16 + row) * RS + d0;
 #pragma unroll
             for (int e = 0; e < 8; ++e) acc[e] += weigh(al, src[e]);
@@ -788,8 +788,6 @@ template <typename T, int HD, bool few> __device__ __forceinline__ void join_row
         if (beg > row) return;
     }
     const int ns = len > chunk ? min(splits, (len - 1) / chunk + 1) : 1;
-    // w L where w stands for a positive weight that may have become 0: a NaN stays
-    auto weigh_sum = [](float w, float l) { return w == 0.f && l == l ? 0.f : w * l; };
     float M = -INFINITY, L = 0.f;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     for (int i0 = 0;;) {
@@ -872,11 +870,13 @@ static PagedPlan plan(const mm_paged_kv& kv, const mm_paged_step& st, int nq) {
     p.few = rows <= kFewRows;
     p.few_rows = p.few ? (int)rows : kFewRows;
     // Few rows: one workgroup of 8 waves a CU.  With more, smaller ones the same bytes are in flight in more places at once: 2 x 131071
-    // keys of 4 heads of 128: 162 us with 1024 workgroups of 4 waves, 133 with 512, 112 with 256 of 8.
+    // keys of 4 heads of 128: 162 us with 1024 workgroups of 4 waves, 133 with 512, 112 with 256 of 8.  Where the keys and values are
+    // few (64 MB), the chain of loads and the waves' exchange count, and 4 waves do it sooner: 100 keys of 16 heads of 64 6.45 -> 5.7 us,
+    // 1023 of 32 heads of 128 15.9 -> 15.3, 8191 of 16 heads of 64 13.6 -> 13.1; 65000 of 8 heads of 128, 266 MB, 52.4 -> 54.9.
     // Many rows: 128 a workgroup.  At head size 128 the registers hold two waves a SIMD whatever the workgroup's size, and one of 8
     // waves fetches each tile once for 256 rows: 1024 tokens over 17k, 32 / 8 heads: 337 -> 314 us.  At 64 three waves a SIMD fit,
     // which 8-wave workgroups cannot use: 59 us against 70 (4 x 2048 tokens, 16 heads).
-    p.waves = p.few || (kv.hn == 128 && rows > 128) ? 8 : 4;
+    p.waves = p.few ? (pairs * st.max_kv * kv.hn <= 1 << 24 ? 4 : 8) : kv.hn == 128 && rows > 128 ? 8 : 4;
     p.row_blocks = p.few ? 1 : (int)((rows + 32 * p.waves - 1) / (32 * p.waves));
     // A token step's split pays for its second launch (about 2 us) once a workgroup's keys and values exceed 256 KB (one CU takes in
     // some 130 GB/s): 700 keys of 64 in one piece 9.7 us, in two 11.2; 1023 of 128 in one 19, in two 15; 2047 of 64 in two 15, in
@@ -892,7 +892,8 @@ template <typename T, int HD> static int launch_paged_attn(const PagedAttnArgs& 
     const unsigned bx = (unsigned)(a.st.seqs * a.kv.heads);
     const int many = p.row_blocks * p.many_splits;
     const dim3 grid(bx, p.few ? p.few_splits : (p.few_splits > many ? p.few_splits : many));
-    if (p.few) paged_attn_few_k<T, HD, 8><<<grid, 512, 0, st>>>(a);
+    if (p.few && p.waves == 4) paged_attn_few_k<T, HD, 4><<<grid, 256, 0, st>>>(a);
+    else if (p.few) paged_attn_few_k<T, HD, 8><<<grid, 512, 0, st>>>(a);
     else if constexpr (HD == 128) {
         if (p.waves == 8) paged_attn_any_k<T, 128, 8><<<grid, 512, 0, st>>>(a, p.row_blocks);
         else paged_attn_any_k<T, 128, 4><<<grid, 256, 0, st>>>(a, p.row_blocks);

@@ -371,3 +371,12 @@ def test_cache_steps_that_make_no_sense_are_refused():
     s = cache.step([a], [1], [3])
     with pytest.raises(RuntimeError, match="max_kv"):
         PagedStep(s.block_table, s.cu_new, s.kv_lens, max_new=1, max_kv=2 ** 32 + 3)
+
+
+@pytest.mark.parametrize("hn,dtype", [(64, BF16), (128, F16)])
+@pytest.mark.parametrize("group,ps", [(1, 16), (16, 24), (3, 1)])
+@pytest.mark.parametrize("max_kv", [10000, 1000000])
+def test_attention_single_tokens_under_larger_bounds(hn, dtype, group, ps, max_kv):
+    """Bounds far above the lengths: larger workgroups and splits that hold no key, the same rows."""
+    c = Case(LENGTHS, nq=2 * group, nkv=2, hn=hn, ps=ps, dtype=dtype, pad=2, seed=group, garbage=float("inf"))
+    check_attention(c, *run_attention(c, max_kv=max_kv))
