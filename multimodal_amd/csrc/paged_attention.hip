@@ -408,9 +408,10 @@ __device__ __forceinline__ void paged_attn_few(const PagedAttnArgs& a, char* sme
 // double-buffered LDS, one barrier a tile; page ids are fetched a tile further ahead, so that no load waits for another.  Row
 // blocks with the most keys start first.
 // Measured: 1024 tokens over 17k, 32 / 8 heads of 128: 287 us with the joining, 960 TFLOP/s; 4 x 2048 tokens, 16 heads of 64: 58 us, 590
-// TFLOP/s of what the causal mask leaves.  A wave's 64-key tile at 128 takes 4460 cycles at 1.95 GHz beside a second wave on its
-// SIMD: 1024 of matrix instructions, about 900 of softmax, 350 .. 550 each for issuing the loads and writing LDS, the rest waiting
-// for the other wave, whose matrix instructions hold the vector unit up (8 cycles each) and the other way round.
+// TFLOP/s of what the causal mask leaves.  A wave's 64-key tile at 128 takes 4070 cycles beside a second wave on its SIMD: 1024 of
+// matrix instructions, about 900 of softmax, 350 .. 550 each for issuing the loads and writing LDS, the rest waiting for the other
+// wave, whose matrix instructions hold the vector unit up (8 cycles each) and the other way round.  The clock falls with the work
+// per cycle (1.88 GHz here, 1.73 at head size 64; a schedule of 4440 cycles a tile ran at 2.03).
 // LDS rows are unpadded; the 16-byte chunks of a row are XOR-ed with the row so that the row reads (16 rows, one chunk) and the
 // transposed reads (4 rows, 4 chunks) both meet all banks once.
 template <int HD> struct KvTile {
