@@ -407,8 +407,9 @@ int mm_paged_kv_append(const mm_paged_kv* kv, const mm_paged_step* step, const v
  *   out[row, h] = softmax(softmax_scale q k^T) v in the cache's dtype, lse[row, h] = ln sum exp(softmax_scale q k^T) in fp32
  * (ParallelSelfAttention.attention with layer_past, megatron/model/transformer.py:315-416).  A row that sees no key gets 0 and
  * -inf; rows of no sequence are left as they were.  What the cache holds behind a sequence's end, and infinities or NaN in keys
- * and values that a row does not see, do not reach it.  q, out [rows, nq, hn]: 16-byte aligned, strides a multiple of 8 elements;
- * lse [rows, nq] with row stride l_row.  workspace: mm_paged_attn_workspace_bytes bytes (0: none; it depends on the shapes and
+ * and values that a row does not see, do not reach it; an infinite value that it does see is infinite in its output, however small
+ * its weight.  q, out [rows, nq, hn]: 16-byte aligned, strides a multiple of 8 elements; lse [rows, nq] with row stride l_row; out
+ * and lse overlap neither the inputs nor themselves.  workspace: mm_paged_attn_workspace_bytes bytes (0: none; it depends on the shapes and
  * bounds alone), 16-byte aligned; calls that share one must not overlap.  Deterministic. */
 size_t mm_paged_attn_workspace_bytes(const mm_paged_kv* kv, const mm_paged_step* step, int nq, int rows);
 int mm_paged_attn_fwd(const mm_paged_kv* kv, const mm_paged_step* step, void* out, int64_t o_row, int64_t o_head, float* lse,

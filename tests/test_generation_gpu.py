@@ -175,3 +175,15 @@ def test_arguments_of_generate():
         stack.word_embeddings.weight[unused] = float("nan")
     got = stack.generate([prompts[0], torch.cat((prompts[1], torch.tensor([unused])))], maximum_tokens=10)
     assert torch.equal(got[0], ref[0]) and got[1].tolist() == [-1]
+
+
+def test_generation_on_another_stream():
+    cfg, stack = build("tiny_magma")
+    g = torch.Generator().manual_seed(6)
+    prompts = [torch.randint(0, 1000, (n,), generator=g) for n in (5, 17)]
+    ref = stack.generate(prompts, maximum_tokens=12)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = stack.generate(prompts, maximum_tokens=12)
+    assert all(torch.equal(a, b) for a, b in zip(got, ref))

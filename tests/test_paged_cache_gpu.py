@@ -380,3 +380,22 @@ def test_attention_single_tokens_under_larger_bounds(hn, dtype, group, ps, max_k
     """Bounds far above the lengths: larger workgroups and splits that hold no key, the same rows."""
     c = Case(LENGTHS, nq=2 * group, nkv=2, hn=hn, ps=ps, dtype=dtype, pad=2, seed=group, garbage=float("inf"))
     check_attention(c, *run_attention(c, max_kv=max_kv))
+
+
+def test_two_streams_at_once():
+    """Calls in flight together, each with a workspace of its own, over one cache: the bits of a call alone."""
+    from multimodal_amd import ops
+    cases = [Case([(1, 3000), (1, 70), (2, 900)], nq=4, nkv=2, hn=64, ps=16, dtype=BF16, seed=1),
+             Case([(40, 2000), (1, 1500)], nq=4, nkv=2, hn=64, ps=16, dtype=BF16, seed=2)]
+    ready = [(c.kv(), c.step(), c.q.cuda(), c.scale) for c in cases]
+    ref = [ops.paged_attn_fwd(*r) for r in ready]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(10):
+        for i, r in enumerate(ready):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(ops.paged_attn_fwd(*r))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, ref[i][0]) and torch.equal(l, ref[i][1]) for o, l in got[i])
