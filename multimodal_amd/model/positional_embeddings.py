@@ -17,6 +17,18 @@ class RotaryEmbedding(torch.nn.Module):
         self.sin_cached = None
         self.precision = precision
         self._stamp = None  # event behind the kernels that filled the cache (multimodal_amd/_streams.py)
+        self._kept = {}     # tables of generation: key -> (cos, sin, event)
+
+    def _build(self, x, seq_len):
+        t = torch.arange(seq_len, device=x.device).type_as(self.inv_freq)
+        freqs = torch.einsum("i,j->ij", t, self.inv_freq.to(x.device))
+        emb = torch.cat((freqs, freqs), dim=-1).to(x.device)
+        if self.precision == torch.bfloat16:
+            emb = emb.float()
+        cos, sin = emb.cos()[:, None, None, :], emb.sin()[:, None, None, :]
+        if self.precision == torch.bfloat16:
+            cos, sin = cos.bfloat16(), sin.bfloat16()
+        return cos, sin
 
     def forward(self, x, seq_dim=1, seq_len=None):
         """Returns (cos, sin) as [seq_len, 1, 1, dim] like the reference."""
@@ -24,20 +36,27 @@ class RotaryEmbedding(torch.nn.Module):
             seq_len = x.shape[seq_dim]
         if seq_len != self.seq_len_cached or self.cos_cached is None or self.cos_cached.device != x.device:
             self.seq_len_cached = seq_len
-            t = torch.arange(seq_len, device=x.device).type_as(self.inv_freq)
-            freqs = torch.einsum("i,j->ij", t, self.inv_freq.to(x.device))
-            emb = torch.cat((freqs, freqs), dim=-1).to(x.device)
-            if self.precision == torch.bfloat16:
-                emb = emb.float()
-            self.cos_cached = emb.cos()[:, None, None, :]
-            self.sin_cached = emb.sin()[:, None, None, :]
-            if self.precision == torch.bfloat16:
-                self.cos_cached = self.cos_cached.bfloat16()
-                self.sin_cached = self.sin_cached.bfloat16()
+            self.cos_cached, self.sin_cached = self._build(x, seq_len)
             self._stamp = _streams.stamp(x.device) if x.is_cuda else None
         elif self._stamp is not None:
             _streams.wait(self._stamp, x.device)
         return self.cos_cached, self.sin_cached
+
+    def kept_tables(self, x, positions):
+        """[positions, dim] contiguous tables in x.dtype that stay where they are: generation's lengths change from call to call, and
+        a captured step (of training with the tables of `forward`, of generation with these) goes on reading the ones it was
+        captured with.  One pair for each power of two."""
+        length = 1 << (positions - 1).bit_length() if positions > 1 else 1
+        key = (length, x.dtype, x.device, self.inv_freq.dtype, self.inv_freq._version)
+        entry = self._kept.get(key)
+        if entry is None:
+            cos, sin = (t.reshape(length, self.dim).to(x.dtype).contiguous() for t in self._build(x, length))
+            entry = (cos, sin, _streams.stamp(x.device) if x.is_cuda else None)
+            if not (x.is_cuda and torch.cuda.is_current_stream_capturing()):  # inside a capture nothing has been computed yet
+                self._kept[key] = entry
+        elif entry[2] is not None:
+            _streams.wait(entry[2], x.device)
+        return entry[0][:positions], entry[1][:positions]
 
     def tables(self, x, seq_len):
         """[seq_len, dim] contiguous tables in x.dtype for the kernel."""

@@ -169,7 +169,7 @@ class ParallelSelfAttention(nn.Module):
         q, k, v = mixed.view(rows, np_, 3, hn).unbind(2)
         cos = sin = None
         if exists(self.rotary_emb):
-            cos, sin = self.rotary_emb.tables(hidden_states, past.max_positions)
+            cos, sin = self.rotary_emb.kept_tables(hidden_states, past.max_positions)
         ops.paged_kv_append(past.kv, past.step, k, v, q=q, cos=cos, sin=sin, q_out=q)
         context, _ = ops.paged_attn_fwd(past.kv, past.step, q, 1.0 / self.norm_factor)
         return self.dense(context.view(rows, 1, np_ * hn))

@@ -154,3 +154,22 @@ def test_workspace_of_a_long_chunk_is_not_multiplied_by_the_single_tokens_splits
     a, b, pa, pb = refs(kv=dict(hn=128, heads=8, page=8 * 16 * 128, head=16 * 128, slot=128), step=step)
     need = lib.mm_paged_attn_workspace_bytes(pa, pb, 32, 8192)
     assert 0 < need <= 32 * 8 * 16 * 130 * 4
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_generation_leaves_the_rotary_tables_of_training_alone(dtype):
+    """A captured training step reads the tables it was captured with: generation's, of other lengths, are others, and stay too."""
+    from multimodal_amd.model.positional_embeddings import RotaryEmbedding
+    rot = RotaryEmbedding(16, precision=dtype).to(dtype)
+    x = torch.zeros(1, dtype=dtype)
+    cos, sin = rot.forward(x, seq_len=64)
+    seen = [rot.kept_tables(x, n) for n in (5, 64, 33, 200, 1, 300)]
+    assert rot.cos_cached is cos and rot.sin_cached is sin
+    for n, (c, s) in zip((5, 64, 33, 200, 1, 300), seen):
+        want_c, want_s = rot.tables(x, n)
+        assert c.shape == (n, 16) and c.is_contiguous() and torch.equal(c, want_c) and torch.equal(s, want_s)
+    assert seen[1][0].data_ptr() == seen[2][0].data_ptr() == rot.kept_tables(x, 40)[0].data_ptr()
+    before = rot.kept_tables(x, 40)[0].clone()
+    with torch.no_grad():
+        rot.inv_freq.mul_(0.5)  # e.g. a loaded checkpoint
+    assert not torch.equal(rot.kept_tables(x, 40)[0], before)

@@ -187,3 +187,27 @@ def test_generation_on_another_stream():
     with torch.cuda.stream(side):
         got = stack.generate(prompts, maximum_tokens=12)
     assert all(torch.equal(a, b) for a, b in zip(got, ref))
+
+
+def test_generation_between_replays_of_a_captured_layer():
+    """A captured forward keeps its rotary tables while generation of other lengths runs and memory is handed out anew."""
+    cfg, stack = build("tiny_magma")
+    layer, s = stack.layers[0], 96
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn(s, 2, cfg["hidden_size"], generator=g).bfloat16().cuda()
+    mask = stack.attention_mask(s, x.device)
+    with torch.no_grad():
+        layer(x, mask)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = layer(x, mask)
+    graph.replay()
+    want = y.clone()
+    for n in (1, 30, 150):
+        stack.generate([torch.randint(0, 1000, (n,), generator=g)], maximum_tokens=6)
+        held = [torch.full((1 << k,), 3.0, device="cuda", dtype=torch.bfloat16) for k in range(6, 16) for _ in range(4)]
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want), n
+        del held
