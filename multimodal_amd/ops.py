@@ -706,18 +706,19 @@ def embed_prefix(table, tokens, prefix=None):
 # A token step of one sequence is a few microseconds of GPU time a call: these wrappers read each tensor's shape and strides once.
 def _launch(device, fn, *args):
     """fn(*args, stream) with the current stream of `device`, which need not be the current device.  (The raw handle: the Stream
-    object around it costs 2.6 us a call.)"""
-    if device.index == torch.cuda.current_device():
-        return fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    object around it costs 2.6 us a call; the tensors at hand have initialised the GPU.)"""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
     with torch.cuda.device(device):
-        return fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _rows(name, t, kv, rows=None, heads=None):
     """(tensor, rows, heads, strides) of a [rows, heads, hn] operand in the cache's dtype, on its device, its head dim contiguous."""
     shape = t.shape
-    if (len(shape) != 3 or shape[2] != kv.hn or t.dtype != kv.dtype or t.device != kv.device
-            or (heads is not None and shape[1] != heads) or (rows is not None and shape[0] != rows)):
+    if (len(shape) != 3 or shape[2] != kv.hn or (heads is not None and shape[1] != heads) or (rows is not None and shape[0] != rows)
+            or t.dtype != kv.dtype or t.device != kv.device):
         raise RuntimeError(f"{name} must be a [{'rows' if rows is None else rows}, {'heads' if heads is None else heads}, {kv.hn}] "
                            f"{kv.dtype} tensor on {kv.device}, got {tuple(shape)} {t.dtype} on {t.device}")
     stride = t.stride()
