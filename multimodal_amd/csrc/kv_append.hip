@@ -8,8 +8,8 @@
 // rotated head the chunk and its partner half a rotation further, so that the rotation needs no exchange between lanes; the
 // lanes of a head's row are neighbours, so every access is a contiguous run of at least d bytes.  W = 8 (16-byte accesses) when
 // rows and rotation allow it, else W = 1.
-// Measured: 4 prompts of 2001 .. 2048 tokens, 32 + 2 x 32 heads of 128: 75.3 us, 399 MB at 5.3 TB/s, what a large copy reaches; 256 rows of one token 4.6 us, one row 2.7 us, the latency of
-// sequence -> length -> page -> row.
+// Measured: 4 prompts of 2001 .. 2048 tokens, 32 + 2 x 32 heads of 128: 75 us, 399 MB at 5.3 TB/s, what a large copy reaches; 16 of
+// 2048, 32 + 2 x 8 heads: 166 us, 4.9 TB/s; 256 rows of one token 4.6 us, one row 2.7 us, the latency of sequence -> length -> page.
 #include "common.h"
 #include "paged.h"
 
@@ -42,80 +42,151 @@ template <typename T, int W> __device__ __forceinline__ void store_chunk(u16* __
     else *p = from_f32<T>(f[0]);
 }
 
-// block b moves items [256 i, 256 i + 256) of row b / parts, i = b % parts (all of one row, so that the sequence search and the
-// page look-up are uniform over the block)
-template <typename T, typename TT, int W, int HN>
-__global__ __launch_bounds__(256) void paged_kv_append_k(const AppendArgs a, int parts) {
-    constexpr int IPH = HN / (2 * W);  // items per head
-    const int row = blockIdx.x / parts;
-    const int seq = find_seq(a.st.cu_new, a.st.seqs, row, threadIdx.x & 63);
-    if (seq >= a.st.seqs || a.st.cu_new[seq] > row) return;  // padding: belongs to no sequence
+// Where a row goes: its position, and the elements from the first page to its slot of head 0; -1: no such place, -2: padding, the
+// row belongs to no sequence.
+struct RowPlace {
+    int64_t slot;
+    int pos;
+};
+__device__ __forceinline__ bool is_padding(const AppendArgs& a, int row, int seq) { return seq >= a.st.seqs || a.st.cu_new[seq] > row; }
+__device__ __forceinline__ RowPlace place_of(const AppendArgs& a, int row, int seq) {
     const int64_t pos64 = (int64_t)a.st.kv_lens[seq] - a.st.cu_new[seq + 1] + row;
-    bool ok = pos64 >= 0 && pos64 < (int64_t)a.st.max_pages * a.kv.page_size && (a.rot_d == 0 || pos64 < a.table_rows);
+    const bool ok = pos64 >= 0 && pos64 < (int64_t)a.st.max_pages * a.kv.page_size && (a.rot_d == 0 || pos64 < a.table_rows);
     const int pos = ok ? (int)pos64 : 0;
     const int pi = (int)fdiv((uint32_t)pos, a.page);
     const int page = a.st.block_table[(int64_t)seq * a.st.table_stride + pi];
-    ok = ok && page >= 0 && page < a.kv.num_pages;
-
-    const int item = (blockIdx.x - row * parts) * 256 + threadIdx.x;
-    const int slot = item / IPH, c = item % IPH;
-    const int nkv = a.kv.heads;
-    if (slot >= a.nq + 2 * nkv) return;
-    const int hc = a.rot_d / (2 * W);  // chunks per half of the rotated dims
-    const u16* src;
-    u16* dst;
-    bool rot = hc > 0;
-    if (slot < a.nq) {
-        src = a.q + (int64_t)row * a.q_row + (int64_t)slot * a.q_head;
-        dst = a.q_out + (int64_t)row * a.qo_row + (int64_t)slot * a.qo_head;
-    } else {
-        if (!ok) return;  // no place for it
-        const bool is_k = slot < a.nq + nkv;
-        const int h = slot - a.nq - (is_k ? 0 : nkv);
-        const int off = pos - pi * a.kv.page_size;
-        rot = rot && is_k;
-        src = is_k ? a.k + (int64_t)row * a.k_row + (int64_t)h * a.k_head : a.v + (int64_t)row * a.v_row + (int64_t)h * a.v_head;
-        dst = (u16*)(is_k ? a.kv.k : a.kv.v) + (int64_t)page * a.kv.page + (int64_t)h * a.kv.head + (int64_t)off * a.kv.slot;
-    }
-    rot = rot && c < hc;
-    // the item's two chunks: partners in the rotated part; behind it (everywhere for an unrotated row) neighbours
-    const int c1 = rot ? c : 2 * c, c2 = rot ? c + hc : 2 * c + 1;
-    float x1[W], x2[W];
-    load_chunk<T, W>(src + c1 * W, x1);
-    load_chunk<T, W>(src + c2 * W, x2);
-    if (rot) {
-        float k1[W], k2[W], s1[W], s2[W];
-        const TT* ct = (const TT*)a.cos + (int64_t)pos * a.rot_d;
-        const TT* st = (const TT*)a.sin + (int64_t)pos * a.rot_d;
-        if constexpr (sizeof(TT) == 4) {
-            load_chunk_f32<W>(ct + c1 * W, k1), load_chunk_f32<W>(ct + c2 * W, k2);
-            load_chunk_f32<W>(st + c1 * W, s1), load_chunk_f32<W>(st + c2 * W, s2);
-        } else {
-            load_chunk<T, W>(ct + c1 * W, k1), load_chunk<T, W>(ct + c2 * W, k2);
-            load_chunk<T, W>(st + c1 * W, s1), load_chunk<T, W>(st + c2 * W, s2);
-        }
-#pragma unroll
-        for (int j = 0; j < W; ++j) {
-            const float y1 = x1[j] * k1[j] - x2[j] * s1[j], y2 = x2[j] * k2[j] + x1[j] * s2[j];
-            x1[j] = y1;
-            x2[j] = y2;
-        }
-    }
-    if (!ok)  // only queries come here: a row without a place must not pass for a number
-#pragma unroll
-        for (int j = 0; j < W; ++j) x1[j] = x2[j] = __builtin_nanf("");
-    store_chunk<T, W>(dst + c1 * W, x1);
-    store_chunk<T, W>(dst + c2 * W, x2);
+    if (!ok || page < 0 || page >= a.kv.num_pages) return RowPlace{-1, 0};
+    return RowPlace{(int64_t)page * a.kv.page + (int64_t)(pos - pi * a.kv.page_size) * a.kv.slot, pos};
 }
 
-template <typename T, typename TT, int W> static int launch_append(const AppendArgs& a, hipStream_t st) {
-    const int items = (a.nq + 2 * a.kv.heads) * (a.kv.hn / (2 * W));
-    const int parts = (items + 255) / 256;
-    MM_CHECK_ARG((int64_t)parts * a.rows < (int64_t)1 << 24, "mm_paged_kv_append: %d rows of %d items exceed the grid limit", a.rows, items);
-    if (a.kv.hn == 64) paged_kv_append_k<T, TT, W, 64><<<parts * a.rows, 256, 0, st>>>(a, parts);
-    else paged_kv_append_k<T, TT, W, 128><<<parts * a.rows, 256, 0, st>>>(a, parts);
+// one work item: its two chunks loaded (a row that is no padding can be read before it is known where it goes), then rotated and stored
+template <typename T, typename TT, int W, int HN> struct Item {
+    static constexpr int IPH = HN / (2 * W);  // items per head
+    int slot, c1, c2;
+    bool rot;
+    float x1[W], x2[W];
+    __device__ __forceinline__ bool load(const AppendArgs& a, int row, int item) {
+        slot = item / IPH;
+        const int c = item % IPH, nkv = a.kv.heads, hc = a.rot_d / (2 * W);  // chunks per half of the rotated dims
+        if (slot >= a.nq + 2 * nkv) return false;
+        const u16* src;
+        if (slot < a.nq) src = a.q + (int64_t)row * a.q_row + (int64_t)slot * a.q_head;
+        else if (slot < a.nq + nkv) src = a.k + (int64_t)row * a.k_row + (int64_t)(slot - a.nq) * a.k_head;
+        else src = a.v + (int64_t)row * a.v_row + (int64_t)(slot - a.nq - nkv) * a.v_head;
+        rot = slot < a.nq + nkv && c < hc;
+        // the item's two chunks: partners in the rotated part; behind it (everywhere for an unrotated row) neighbours
+        c1 = rot ? c : 2 * c, c2 = rot ? c + hc : 2 * c + 1;
+        load_chunk<T, W>(src + c1 * W, x1);
+        load_chunk<T, W>(src + c2 * W, x2);
+        return true;
+    }
+    __device__ __forceinline__ void store(const AppendArgs& a, int row, const RowPlace& to) {
+        u16* dst;
+        if (slot < a.nq) dst = a.q_out + (int64_t)row * a.qo_row + (int64_t)slot * a.qo_head;
+        else {
+            if (to.slot < 0) return;  // no place for it
+            const bool is_k = slot < a.nq + a.kv.heads;
+            dst = (u16*)(is_k ? a.kv.k : a.kv.v) + to.slot + (int64_t)(slot - a.nq - (is_k ? 0 : a.kv.heads)) * a.kv.head;
+        }
+        if (rot) {
+            float k1[W], k2[W], s1[W], s2[W];
+            const TT* ct = (const TT*)a.cos + (int64_t)to.pos * a.rot_d;
+            const TT* st = (const TT*)a.sin + (int64_t)to.pos * a.rot_d;
+            if constexpr (sizeof(TT) == 4) {
+                load_chunk_f32<W>(ct + c1 * W, k1), load_chunk_f32<W>(ct + c2 * W, k2);
+                load_chunk_f32<W>(st + c1 * W, s1), load_chunk_f32<W>(st + c2 * W, s2);
+            } else {
+                load_chunk<T, W>(ct + c1 * W, k1), load_chunk<T, W>(ct + c2 * W, k2);
+                load_chunk<T, W>(st + c1 * W, s1), load_chunk<T, W>(st + c2 * W, s2);
+            }
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const float y1 = fmaf(x1[j], k1[j], -(x2[j] * s1[j])), y2 = fmaf(x2[j], k2[j], x1[j] * s2[j]);
+                x1[j] = y1;
+                x2[j] = y2;
+            }
+        }
+        if (to.slot < 0)  // only queries come here: a row without a place must not pass for a number
+#pragma unroll
+            for (int j = 0; j < W; ++j) x1[j] = x2[j] = __builtin_nanf("");
+        store_chunk<T, W>(dst + c1 * W, x1);
+        store_chunk<T, W>(dst + c2 * W, x2);
+    }
+};
+
+// Few rows: block b moves items [256 i, 256 i + 256) of row b / parts, i = b % parts (all of one row, so that the sequence search
+// and the page look-up are uniform over the block)
+template <typename T, typename TT, int W, int HN>
+__global__ __launch_bounds__(256) void paged_kv_append_k(const AppendArgs a, int parts) {
+    const int row = blockIdx.x / parts;
+    const int seq = find_seq(a.st.cu_new, a.st.seqs, row, threadIdx.x & 63);
+    if (is_padding(a, row, seq)) return;
+    Item<T, TT, W, HN> it;
+    const bool live = it.load(a, row, (blockIdx.x - row * parts) * 256 + threadIdx.x);
+    const RowPlace to = place_of(a, row, seq);
+    if (live) it.store(a, row, to);
+}
+// Many rows: a block moves `per` rows, whose places are looked up side by side, one lane each
+template <typename T, typename TT, int W, int HN>
+__global__ __launch_bounds__(256) void paged_kv_append_rows_k(const AppendArgs a, int per, FastDiv items) {
+    __shared__ RowPlace places[64];
+    const int row0 = blockIdx.x * per, n = min(per, a.rows - row0), tid = threadIdx.x;
+    if (tid < 64) {
+        int seq = find_seq(a.st.cu_new, a.st.seqs, row0, tid);
+        if (tid < n) {
+            // the row's own sequence: rarely far behind the first row's; sequences without rows may lie between
+            int step = 0;
+            while (step < 4 && seq < a.st.seqs && a.st.cu_new[seq + 1] <= row0 + tid) ++seq, ++step;
+            for (int left = step == 4 ? a.st.seqs - seq : 0; left > 0;) {
+                const int half = left >> 1;
+                if (a.st.cu_new[seq + half + 1] <= row0 + tid) seq += half + 1, left -= half + 1;
+                else left = half;
+            }
+            places[tid] = is_padding(a, row0 + tid, seq) ? RowPlace{-2, 0} : place_of(a, row0 + tid, seq);
+        }
+    }
+    __syncthreads();
+    const int total = n * (int)items.d;
+    constexpr int U = 2;
+    for (int i0 = tid; i0 < total; i0 += 256 * U) {
+        Item<T, TT, W, HN> it[U];
+        RowPlace to[U];
+        int row[U];
+        bool live[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + 256 * u;
+            live[u] = i < total;
+            if (!live[u]) continue;
+            const int r = (int)fdiv((uint32_t)i, items);
+            row[u] = row0 + r;
+            to[u] = places[r];
+            live[u] = to[u].slot != -2 && it[u].load(a, row[u], i - r * (int)items.d);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (live[u]) it[u].store(a, row[u], to[u]);
+    }
+}
+
+template <typename T, typename TT, int W, int HN> static int launch_append_hn(const AppendArgs& a, hipStream_t st) {
+    const int items = (a.nq + 2 * a.kv.heads) * (HN / (2 * W));
+    // One row a block leaves lanes idle where its items are few, or a little over 256; then several rows share one, once that leaves
+    // 4 blocks a CU.  8 x 2048 tokens and more: 72 items (16 / 1 heads of 64) 43 -> 30.6 us, 288 (32 / 2 of 128) 92 -> 72, 320 with
+    // fp32 tables 98 -> 75, 384 183 -> 166; but 192 (16 / 16 of 64) 87 -> 96, 768 (32 / 32 of 128) 75 -> 89.  The narrow path is short of
+    // loads in flight: 1536 items of 64 with 20 rotated dims 61 -> 44.6.
+    const int per = items <= 96 ? 8 : W == 1 || (items > 256 && items <= 384) ? 2 : 1;
+    const bool shared = per > 1 && a.rows / per >= 1024;
+    const int parts = shared ? 1 : (items + 255) / 256;
+    const int64_t blocks = shared ? ((int64_t)a.rows + per - 1) / per : (int64_t)parts * a.rows;
+    MM_CHECK_ARG(blocks < (int64_t)1 << 24, "mm_paged_kv_append: %d rows of %d items exceed the grid limit", a.rows, items);
+    if (shared) paged_kv_append_rows_k<T, TT, W, HN><<<(unsigned)blocks, 256, 0, st>>>(a, per, make_fastdiv(items));
+    else paged_kv_append_k<T, TT, W, HN><<<(unsigned)blocks, 256, 0, st>>>(a, parts);
     MM_CHECK_LAUNCH();
     return MM_OK;
+}
+template <typename T, typename TT, int W> static int launch_append(const AppendArgs& a, hipStream_t st) {
+    return a.kv.hn == 64 ? launch_append_hn<T, TT, W, 64>(a, st) : launch_append_hn<T, TT, W, 128>(a, st);
 }
 
 }  // namespace mm

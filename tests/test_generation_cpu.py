@@ -123,7 +123,7 @@ def test_division_by_multiplication(d):
 def test_launches_beyond_the_grid_are_refused():
     """A grid dimension times the workgroup's threads stays below 2^32."""
     lib = _lib.get_lib()
-    rc, msg = append(rows=1 << 24)
+    rc, msg = append(rows=(1 << 31) - 1)
     assert rc == -1 and "grid" in msg
     rc, msg = attend(step=dict(seqs=1 << 21))
     assert rc == -1 and "grid" in msg

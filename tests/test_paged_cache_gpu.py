@@ -399,3 +399,33 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(o, ref[i][0]) and torch.equal(l, ref[i][1]) for o, l in got[i])
+
+
+@pytest.mark.parametrize("nq,nkv,hn,d", [(4, 1, 64, 16), (26, 4, 128, 128), (4, 2, 64, 20), (16, 16, 64, 16)])
+def test_append_many_rows_equals_few(nq, nkv, hn, d):
+    """Thousands of rows in one call - sequences without rows between them, padding, rows without a place - against the same rows a
+    few hundred at a time: the same bits."""
+    from multimodal_amd import ops
+    from multimodal_amd.kv_cache import PagedStep
+    g = torch.Generator().manual_seed(nq)
+    n = torch.randint(0, 90, (240,), generator=g)
+    n[20:32] = 0   # a run of sequences without rows
+    n[100:103] = 0
+    seqs = [(int(x), int(x) + int(p)) for x, p in zip(n, torch.randint(0, 40, (240,), generator=g))]
+    c = Case(seqs, nq=nq, nkv=nkv, hn=hn, ps=16, dtype=BF16, pad=5, seed=d)
+    assert c.rows > 8 * 1024 + 64
+    c.block_table[50, 0] = c.num_pages
+    c.block_table[51, 1:] = -1
+    cos, sin = (t.cuda() for t in tables(110, d, BF16))  # some positions lie behind them
+    k, v, q = c.k.cuda(), c.v.cuda(), c.q.cuda()
+    many, few = c.kv(), c.kv()
+    out = torch.full((c.rows, nq, hn), 7.0, dtype=BF16, device="cuda")
+    ref = out.clone()
+    ops.paged_kv_append(many, c.step(), k, v, q=q, cos=cos, sin=sin, q_out=out)
+    for a in range(0, 240, 8):
+        r0, r1 = int(c.cu[a]), int(c.cu[a + 8])
+        step = PagedStep(c.block_table[a:a + 8].cuda(), (c.cu[a:a + 9] - r0).cuda(), c.lens[a:a + 8].cuda(), c.max_new, c.max_kv)
+        ops.paged_kv_append(few, step, k[r0:r1], v[r0:r1], q=q[r0:r1], cos=cos, sin=sin, q_out=ref[r0:r1])
+    assert torch.equal(torch.isnan(out), torch.isnan(ref)) and torch.equal(out.nan_to_num(), ref.nan_to_num())
+    assert bool(torch.isnan(out).any()) and bool((out[int(c.cu[-1]):] == 7).all())
+    assert torch.equal(many.k, few.k) and torch.equal(many.v, few.v)
