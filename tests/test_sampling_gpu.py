@@ -193,3 +193,71 @@ def test_replayed_graph_and_other_stream():
         other = ops.sample_tokens(x, u, top_p=0.9)
     torch.cuda.synchronize()
     assert torch.equal(other, want)
+
+
+def odd_rows(rows, vocab, dtype, seed, sigma=2.5):
+    """Rows that start at any alignment, with values behind them that must not count."""
+    g = torch.Generator().manual_seed(seed)
+    flat = torch.full((rows * (vocab + 3) + 16,), 60.0, dtype=dtype)
+    x = flat[5:5 + rows * (vocab + 3)].view(rows, vocab + 3)[:, :vocab]
+    x.copy_((torch.randn(rows, vocab, generator=g) * sigma).to(dtype))
+    return flat.cuda()[5:5 + rows * (vocab + 3)].view(rows, vocab + 3)[:, :vocab], torch.rand(rows, generator=g), g
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows,vocab", [(1, 500), (257, 504), (257, 505), (257, 506), (300, 1016), (300, 1017), (300, 1018), (1025, 2040),
+                                        (1025, 2041), (1025, 2042), (1030, 3), (1030, 64)])
+def test_small_vocabularies(dtype, rows, vocab):
+    """Every number of rows, at the borders of the vocabularies that are sorted; every filter, parameters of each row."""
+    x, u, g = odd_rows(rows, vocab, dtype, rows + vocab)
+    check(x, u)
+    check(x, u, top_k=20, top_p=0.9)
+    check(x, u, temperature=torch.rand(rows, generator=g) * 2 * (torch.arange(rows) % 5 != 0),
+          top_k=torch.randint(-2, vocab + 5, (rows,), generator=g, dtype=torch.int32),
+          top_p=torch.rand(rows, generator=g) * 1.2 - 0.1, min_p=torch.rand(rows, generator=g) * 0.2 - 0.05)
+
+
+@pytest.mark.parametrize("par", PAR, ids=[str(p) for p in PAR])
+def test_parameters_of_small_vocabularies(par):
+    for vocab, rows in ((500, 40), (1010, 270), (2030, 1030)):
+        x, u, _ = odd_rows(rows, vocab, BF16, 7)
+        check(x, u, **par)
+
+
+@pytest.mark.parametrize("rows,vocab", [(6, 400), (260, 1000), (1026, 2000)])
+def test_ties_infinities_and_nan_of_small_vocabularies(rows, vocab):
+    inf = float("inf")
+    x, u, _ = odd_rows(rows, vocab, F16, 9)
+    x[0, :] = -inf
+    x[1, vocab // 2] = float("nan")
+    x[2, 50:] = -inf
+    x[3, [9, 20, 300]] = inf
+    x[4, :] = 0.0
+    x[4, ::2] = -0.0
+    x[5, :] = 1.5
+    for par in (dict(), dict(temperature=0.0), dict(top_k=5, top_p=0.9, min_p=0.01), dict(temperature=inf), dict(top_p=0.5)):
+        got = check(x, u, **par)
+        assert got[0] == -1 and got[1] == -1 and 0 <= got[2] < 50 and int(got[3]) in (9, 20, 300)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("vocab", [1, 9, 500, 16384, 16385, 50277, 70001])
+def test_greedy_rows(dtype, vocab):
+    """Ties to the lowest index, zeros of both signs, infinities, NaN; at any alignment."""
+    inf = float("inf")
+    x, u, g = odd_rows(12, vocab, dtype, vocab)
+    at = torch.randint(0, vocab, (12, 3), generator=g)
+    for r, v in ((0, 50.0), (1, 50.0), (2, inf), (3, -inf), (4, float("nan")), (5, -float("nan"))):
+        if r == 3:
+            x[r, :] = -inf
+        else:
+            x[r, at[r].cuda()] = v
+    x[6, :] = -0.0
+    x[6, int(at[6, 0])] = 0.0
+    x[7, :] = -inf
+    x[7, int(at[7, 0])] = -3.0
+    x[8, :] = torch.finfo(dtype).min
+    got = check(x, u, temperature=0.0)
+    assert got[3] == -1 and got[4] == -1 and got[5] == -1 and got[6] == 0 and got[8] == 0 and got[7] == at[7, 0]
+    per_row = torch.zeros(12)  # the same through each row's own temperature
+    assert torch.equal(check(x, u, temperature=per_row), got)
