@@ -421,7 +421,8 @@ int mm_paged_attn_fwd(const mm_paged_kv* kv, const mm_paged_step* step, void* ou
  * ordered by descending logit, ties by ascending index, and weigh w = exp((logit - max) / temperature):
  *   top_k > 0 keeps the first top_k; 0 < top_p < 1 keeps a token while the weight ahead of it is at most top_p times the weight of
  *   what top_k kept; min_p > 0 keeps w >= min_p; the first token always stays; other values of the three switch them off;
- *   tokens[row] = the first token in that order whose running weight exceeds u times the kept weight (u >= 1: the last one kept).
+ *   tokens[row] = the first token in that order whose running weight exceeds u times the kept weight (u >= 1 or NaN: the last one kept
+ *   whose weight is not 0 in 64 bits).
  * temperature <= 0 takes the first token (the lowest index of the largest logit).  -inf is never drawn, +inf always wins; a row
  * with a NaN, or of nothing but -inf, gives -1.  Each parameter is the scalar, or per row where its array is not NULL.  Weights and
  * their sums are in 64 bits and the order of summation is fixed. */

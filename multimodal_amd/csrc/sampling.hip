@@ -7,7 +7,9 @@
 // weight exceeds u min(Z_k, Z_p, Z_m).  No sort is needed: a 16-bit logit has 65536 values at most, so a histogram over the
 // values, in order, holds the whole distribution exactly - counts are integers, one weight per value in 64 bits - and the token is
 // the j-th by index of one value.  Sums run in a fixed order: the result does not depend on scheduling, and a border of two tokens
-// is off by about 1e-15 of the weight.
+// is off by about 1e-15 of the weight.  The running sums of neighbours are added up in different orders and so may differ either way
+// by that much; a random number below 1 stays 2^-24 of the weight away from the end, but the last token kept, which one of 1 or
+// more asks for, is found by counting tokens instead.
 //
 // One workgroup of 16 waves per row.  Its histogram (a count of a non-negative value in the low half of a word, of a negative one
 // in the high half; 130 KB) fills most of a CU's LDS.  Steps: (1) the row into registers, each wave a contiguous 16th of it (the
@@ -196,6 +198,9 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
     const float p = a.top_p_v ? a.top_p_v[row] : a.top_p, mp = a.min_p_v ? a.min_p_v[row] : a.min_p;
     const int k = a.top_k_v ? a.top_k_v[row] : a.top_k;
     const bool greedy = !(temp > 0.f);
+    const bool last = !(u < 1.f);  // (or NaN) the last token kept
+    // a token is kept whose weight is at least this, and not 0
+    const double floor_w = mp > 0.f ? fmin((double)mp, 1.0) : 0.0;
     auto clear_hist = [&]() {
         u32x4* h = reinterpret_cast<u32x4*>(sm.hist);
         for (int i = tid; i < 512 * 65 / 4; i += kSampleThreads) h[i] = u32x4{0, 0, 0, 0};
@@ -275,10 +280,11 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
     int dk = lo, j = 0;  // the token: the j-th by index of the value with this place
     if (!greedy) {
         const Weights<T> wt{lo, (double)order_value<T>(lo), 1.0 / (double)temp};
-        // values below max - 50 T weigh less than 2^-72 each: nothing of them reaches a 64-bit sum that holds the largest's 1
+        // values below max - 50 T weigh less than 2^-72 each: nothing of them reaches a 64-bit sum that holds the largest's 1 (but
+        // the last token kept may be one of them)
         const float xlow = (float)(wt.xmax - 50.0 * (double)temp);
         int dlow = minus_inf<T>();
-        if (xlow > -INFINITY) {
+        if (xlow > -INFINITY && !last) {
             const u16 b = from_f32<T>(xlow);
             dlow = min(dlow, ((b & 0x8000) ? (int)b : 0x7fff - (int)b) + 1);
         }
@@ -348,7 +354,7 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
                 double wgt = 0.0;
                 if (tid < m && tid < k) wgt = wt.at((int)(sm.sorted()[tid] >> 32));
                 const double c2 = scan_d(wgt);
-                const uint64_t heavy = __ballot(wgt >= fmin((double)mp, 1.0));
+                const uint64_t heavy = __ballot(wgt >= floor_w && wgt > 0.0);
                 if (lane == 63) {
                     sm.wave_mass[wave] = c2;
                     sm.wave_count[wave] = __popcll(heavy);
@@ -358,12 +364,16 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
                 __syncthreads();
                 if (wave == 0) {
                     double z = sm.mass[kChunks - 1], zp = z;
-                    if (p > 0.f && p < 1.f) zp = fmin(zp, sm.mass[first_of([&](int i) { return sm.mass[i] > (double)p * z; })]);
-                    if (mp > 0.f) zp = fmin(zp, sm.mass[max((int)lane_u(row_sum_u(sm.wave_count[lane & 15]), 15), 1) - 1]);
+                    int end = max((int)lane_u(row_sum_u(sm.wave_count[lane & 15]), 15), 1) - 1;  // the last one kept
+                    if (mp > 0.f) zp = fmin(zp, sm.mass[end]);
+                    if (p > 0.f && p < 1.f) {
+                        const int at = first_of([&](int i) { return sm.mass[i] > (double)p * z; });
+                        zp = fmin(zp, sm.mass[at]);
+                        end = min(end, at);
+                    }
                     zp = fmax(zp, 1.0);
-                    double t = (double)u * zp;
-                    if (!(t < zp)) t = __longlong_as_double(__double_as_longlong(zp) - 1);  // u of 1 or more: the last token kept
-                    const int f = first_of([&](int i) { return sm.mass[i] > t; });
+                    const double t = (double)u * zp;
+                    const int f = last ? end : min(first_of([&](int i) { return sm.mass[i] > t; }), end);
                     if (lane == 0) a.out[row] = (int64_t)(uint32_t)sm.sorted()[f];
                 }
                 return;
@@ -483,13 +493,19 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
                 double upto;
             };
             auto find = [&](double t) -> Found {
-                const int c = first_of([&](int i) { return sm.mass[i] > t; });
+                int c = first_of([&](int i) { return sm.mass[i] > t; });
+                uint32_t n = counts(c);
+                if (__ballot(n != 0) == 0) {
+                    // an empty chunk: rounding put t between the sums of chunks without a token between them, or t is below 0.  The
+                    // chunk that holds the last token up to here, or the first of all
+                    const uint32_t upto = max(sm.count[c], 1u);
+                    c = first_of([&](int i) { return sm.count[i] >= upto; });
+                    n = counts(c);
+                }
                 const double ahead = c ? sm.mass[c - 1] : 0.0;
-                const uint32_t n = counts(c);
                 const double w = n ? wt.at(64 * c + lane) : 0.0;
                 const double incl = ahead + scan_d((double)n * w);
                 const uint64_t any = __ballot(n != 0);
-                if (!any) return Found{lo, 0, 1.0};  // rounding put t between two chunks' sums
                 const uint64_t over = __ballot(n != 0 && incl > t);
                 const int l = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any);
                 const double before = incl - (double)n * w, last = (double)(n ? n - 1 : 0);
@@ -497,19 +513,23 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
                 const double up = before + (jj + 1.0) * w;
                 return Found{64 * c + l, (int)lane_u((uint32_t)(int)jj, l), lane_d(up, l)};
             };
-            auto min_p_mass = [&]() -> double {
-                // the first value whose weight is below min_p: 64-way search in the order
-                const double floor_w = fmin((double)mp, 1.0);
+            // the first value that weighs too little to be kept: 64-way search in the order
+            auto first_below = [&]() -> int {
                 int from = lo, span = 65536 - lo;
                 while (span > 0) {
                     const int st = (span + 63) >> 6, at = from + lane * st + st - 1;
-                    const bool kept = lane * st + st - 1 < span && wt.at(min(at, minus_inf<T>())) >= floor_w;
+                    const double w = wt.at(min(at, minus_inf<T>()));
+                    const bool kept = lane * st + st - 1 < span && w >= floor_w && w > 0.0;
                     const int g = __popcll(__ballot(kept));
                     from += g * st;
                     span -= g * st;
                     if (st == 1) break;
                     span = min(span, st);
                 }
+                return from;
+            };
+            auto min_p_mass = [&]() -> double {
+                const int from = first_below();
                 const int c = min(from, 65535) >> 6;
                 const uint32_t n = counts(c);
                 const double w = n ? wt.at(64 * c + lane) : 0.0;
@@ -520,10 +540,18 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
                 const double m = min_p_mass();
                 if (lane == 0) sm.min_p_mass = m;
             }
+            // the number of tokens of the values ahead of this one
+            auto tokens_ahead = [&](int d) -> uint32_t {
+                const int c = min(d, 65535) >> 6;
+                const uint32_t n = counts(c);
+                return (c ? sm.count[c - 1] : 0u) + lane_u(scan_u(64 * c + lane < d ? n : 0u), 63);
+            };
             double zp = 0.0;
+            uint32_t kept = sm.count[kChunks - 1];  // how many tokens (`last` alone needs it)
             if (BIG || wave == 0) {
                 double z = sm.mass[kChunks - 1];
-                if (k > 0 && (uint32_t)k < sm.count[kChunks - 1]) {
+                if (k > 0 && (uint32_t)k < kept) {
+                    kept = (uint32_t)k;
                     const int c = first_of([&](int i) { return sm.count[i] >= (uint32_t)k; });
                     const uint32_t n = counts(c);
                     const double w = n ? wt.at(64 * c + lane) : 0.0;
@@ -534,18 +562,31 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
                     z = fmin(z, lane_d(mi - (double)(ci - (uint32_t)k) * w, l));
                 }
                 zp = z;
-                if (p > 0.f && p < 1.f) zp = fmin(zp, find((double)p * z).upto);
+                if (p > 0.f && p < 1.f) {
+                    const Found f = find((double)p * z);
+                    zp = fmin(zp, f.upto);
+                    if (last) kept = min(kept, tokens_ahead(f.dk) + (uint32_t)f.j + 1);
+                }
+                if (last) kept = min(kept, tokens_ahead(first_below()));
             }
             if (!BIG) __syncthreads();
             if (BIG || wave == 0) {
-                if (mp > 0.f) zp = fmin(zp, BIG ? min_p_mass() : sm.min_p_mass);
-                zp = fmax(zp, 1.0);
-                double t = (double)u * zp;
-                if (!(t < zp)) t = __longlong_as_double(__double_as_longlong(zp) - 1);  // u of 1 or more: the last token kept
-                const Found f = find(t);
+                int fdk, fj;
+                if (last) {
+                    const int c = first_of([&](int i) { return sm.count[i] >= kept; });
+                    const uint32_t n = counts(c), upto = (c ? sm.count[c - 1] : 0u) + scan_u(n);
+                    const int l = __builtin_ctzll(__ballot(upto >= kept));
+                    fdk = 64 * c + l;
+                    fj = (int)(kept - 1 - lane_u(upto - n, l));
+                } else {
+                    if (mp > 0.f) zp = fmin(zp, BIG ? min_p_mass() : sm.min_p_mass);
+                    const Found f = find((double)u * fmax(zp, 1.0));
+                    fdk = f.dk;
+                    fj = f.j;
+                }
                 if (BIG || lane == 0) {
-                    sm.dk = f.dk;
-                    sm.j = f.j;
+                    sm.dk = fdk;
+                    sm.j = fj;
                 }
             }
         }
@@ -756,7 +797,7 @@ template <typename T, int EPL> __global__ __launch_bounds__(256) void sample_sma
     else if (temp > 0.f) {
         const Weights<T> wt{lo, (double)order_value<T>(lo), 1.0 / (double)temp};
         const int kept = k > 0 && k < a.vocab ? k : a.vocab;
-        const double floor_w = fmin((double)mp, 1.0);
+        const double floor_w = mp > 0.f ? fmin((double)mp, 1.0) : 0.0;
         double run[EPL], z = 0.0;  // running weights of keys 64 j + lane
         int heavy = 0;
 #pragma unroll
@@ -764,7 +805,7 @@ template <typename T, int EPL> __global__ __launch_bounds__(256) void sample_sma
             run[j] = z;
             if (64 * j >= kept) continue;
             const double w = 64 * j + lane < kept ? wt.at((int)(sorted[64 * j + lane] >> 16)) : 0.0;
-            heavy += __popcll(__ballot(w >= floor_w));
+            heavy += __popcll(__ballot(w >= floor_w && w > 0.0));
             run[j] = z + scan_d(w);
             z = lane_d(run[j], 63);
         }
@@ -784,20 +825,19 @@ template <typename T, int EPL> __global__ __launch_bounds__(256) void sample_sma
             return at;
         };
         double zp = z, upto;
-        if (p > 0.f && p < 1.f) {
-            find((double)p * z, upto);
-            zp = fmin(zp, upto);
-        }
+        int end = max(heavy, 1) - 1;  // the last one kept
         if (mp > 0.f) {
-            const int last = max(heavy, 1) - 1;
 #pragma unroll
             for (int j = 0; j < EPL; ++j)
-                if (last >> 6 == j) zp = fmin(zp, lane_d(run[j], last & 63));
+                if (end >> 6 == j) zp = fmin(zp, lane_d(run[j], end & 63));
         }
-        zp = fmax(zp, 1.0);
-        double t = (double)u * zp;
-        if (!(t < zp)) t = __longlong_as_double(__double_as_longlong(zp) - 1);  // u of 1 or more: the last token kept
-        token = (int64_t)(sorted[find(t, upto)] & 0xffffu);
+        if (p > 0.f && p < 1.f) {
+            end = min(end, find((double)p * z, upto));
+            zp = fmin(zp, upto);
+        }
+        // a random number of 1 or more, or NaN: the last one kept
+        if (u < 1.f) end = min(end, find((double)u * fmax(zp, 1.0), upto));
+        token = (int64_t)(sorted[end] & 0xffffu);
     }
     if (live && lane == 0) a.out[row] = token;
 }

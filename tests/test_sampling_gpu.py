@@ -261,3 +261,44 @@ def test_greedy_rows(dtype, vocab):
     assert got[3] == -1 and got[4] == -1 and got[5] == -1 and got[6] == 0 and got[8] == 0 and got[7] == at[7, 0]
     per_row = torch.zeros(12)  # the same through each row's own temperature
     assert torch.equal(check(x, u, temperature=per_row), got)
+
+
+def ends(rows):
+    """Random numbers of 1 and beyond, and NaN (the last token kept), beside the largest below 1 and 0."""
+    v = torch.tensor([1.0, float("nan"), 2.0, float("inf"), 1.0, 1 - 2.0 ** -24, 0.0])
+    return v.repeat(-(-rows // 7))[:rows]
+
+
+# at the last one the weights fall below 2^-72 of the largest, which no sum of 64 bits shows
+ENDS = [dict(), dict(top_k=3), dict(top_k=5), dict(top_k=11), dict(top_k=200), dict(top_k=500), dict(top_k=700), dict(top_p=0.9),
+        dict(min_p=0.01), dict(top_k=11, top_p=0.95, min_p=1e-3), dict(top_k=700, top_p=0.95, min_p=1e-3),
+        dict(temperature=0.2, top_k=300), dict(temperature=0.2)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows,vocab", [(63, 500), (260, 1010), (1030, 2030), (63, 3001), (28, 50277), (28, 65528), (14, 70001)])
+def test_the_last_token_kept_is_drawn_at_one_and_beyond(dtype, rows, vocab):
+    """In every kernel: sorted rows, a top-k's list, the histogram, the histogram of long rows."""
+    x, _, g = odd_rows(rows, vocab, dtype, vocab + 1)
+    for par in ENDS:
+        check(x, ends(rows), **par)
+    check(x, ends(rows), temperature=0.5 + torch.rand(rows, generator=g), top_k=torch.randint(0, 600, (rows,), generator=g, dtype=torch.int32),
+          top_p=0.5 + torch.rand(rows, generator=g), min_p=torch.rand(rows, generator=g) * 0.02)
+
+
+@pytest.mark.parametrize("rows,vocab", [(28, 500), (260, 1010), (1030, 2030), (28, 3001), (14, 50277), (14, 70001)])
+def test_the_last_token_kept_is_never_a_banned_one(rows, vocab):
+    """Tokens of -inf have no weight: not drawn at 1 either, also where fewer are left than a top-k would keep."""
+    inf = float("inf")
+    x, _, g = odd_rows(rows, vocab, F16, vocab + 2)
+    some = torch.rand(rows, vocab, generator=g) < 0.5
+    x[some.cuda()] = -inf
+    x[1, 7:] = -inf
+    x[2, :] = -inf
+    x[2, vocab // 3] = 0.5
+    x[3, [2, vocab // 2, vocab - 1]] = inf   # they share everything
+    x[4, :] = torch.finfo(F16).min
+    x[8, :] = -0.0
+    x[8, 1::2] = 0.0
+    for par in ENDS:
+        check(x, ends(rows), **par)
