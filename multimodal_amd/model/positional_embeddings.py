@@ -17,7 +17,8 @@ class RotaryEmbedding(torch.nn.Module):
         self.sin_cached = None
         self.precision = precision
         self._stamp = None  # event behind the kernels that filled the cache (multimodal_amd/_streams.py)
-        self._kept = {}     # tables of generation: key -> (cos, sin, event)
+        self._kept = {}     # tables of generation: key -> (inv_freq, its version, cos, sin, event)
+        self._replaced = []  # those of frequencies the module no longer holds
 
     def _build(self, x, seq_len):
         t = torch.arange(seq_len, device=x.device).type_as(self.inv_freq)
@@ -45,18 +46,24 @@ class RotaryEmbedding(torch.nn.Module):
     def kept_tables(self, x, positions):
         """[positions, dim] contiguous tables in x.dtype that stay where they are: generation's lengths change from call to call, and
         a captured step (of training with the tables of `forward`, of generation with these) goes on reading the ones it was
-        captured with.  One pair for each power of two."""
+        captured with.  One pair for each power of two; new ones once the module holds other frequencies (another tensor, or a
+        version counted on: whatever a load or a cast does), the old ones kept for the steps captured with them."""
         length = 1 << (positions - 1).bit_length() if positions > 1 else 1
-        key = (length, x.dtype, x.device, self.inv_freq.dtype, self.inv_freq._version)
+        inv = self.inv_freq
+        key = (length, x.dtype, x.device, self.precision)
+        version = None if inv.is_inference() else inv._version  # None: changes are not counted, so nothing is kept
         entry = self._kept.get(key)
-        if entry is None:
-            cos, sin = (t.reshape(length, self.dim).to(x.dtype).contiguous() for t in self._build(x, length))
-            entry = (cos, sin, _streams.stamp(x.device) if x.is_cuda else None)
-            if not (x.is_cuda and torch.cuda.is_current_stream_capturing()):  # inside a capture nothing has been computed yet
-                self._kept[key] = entry
-        elif entry[2] is not None:
-            _streams.wait(entry[2], x.device)
-        return entry[0][:positions], entry[1][:positions]
+        if entry is not None and entry[0] is inv and entry[1] == version and version is not None:
+            if entry[4] is not None:
+                _streams.wait(entry[4], x.device)
+            return entry[2][:positions], entry[3][:positions]
+        cos, sin = (t.reshape(length, self.dim).to(x.dtype).contiguous() for t in self._build(x, length))
+        # inside a capture nothing has been computed yet
+        if version is not None and not (x.is_cuda and torch.cuda.is_current_stream_capturing()):
+            if entry is not None:
+                self._replaced.append(entry)
+            self._kept[key] = (inv, version, cos, sin, _streams.stamp(x.device) if x.is_cuda else None)
+        return cos[:positions], sin[:positions]
 
     def tables(self, x, seq_len):
         """[seq_len, dim] contiguous tables in x.dtype for the kernel."""

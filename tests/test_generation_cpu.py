@@ -173,3 +173,33 @@ def test_generation_leaves_the_rotary_tables_of_training_alone(dtype):
     with torch.no_grad():
         rot.inv_freq.mul_(0.5)  # e.g. a loaded checkpoint
     assert not torch.equal(rot.kept_tables(x, 40)[0], before)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_tables_of_generation_follow_the_frequencies_the_module_holds(dtype):
+    """A buffer that takes the place of inv_freq starts counting its versions anew: the tables are still those of what it holds."""
+    from multimodal_amd.model.positional_embeddings import RotaryEmbedding
+    x = torch.zeros(1, dtype=dtype)
+
+    def agree(rot):
+        for got, want in zip(rot.kept_tables(x, 40), rot.tables(x, 40)):
+            assert torch.equal(got, want)
+        rot.seq_len_cached = None  # `tables` keeps the last length's
+
+    rot = RotaryEmbedding(16, precision=dtype)
+    agree(rot)
+    first = rot.kept_tables(x, 40)[0]
+    copy = first.clone()
+    rot.load_state_dict({"inv_freq": 0.5 * rot.inv_freq}, assign=True)
+    agree(rot)
+    rot.to(torch.bfloat16).float()  # the frequencies have been rounded
+    agree(rot)
+    rot.precision = torch.float32
+    agree(rot)
+    rot.precision = dtype
+    with torch.inference_mode():
+        rot.inv_freq = 0.25 * rot.inv_freq  # no versions are counted in here
+        agree(rot)
+        rot.inv_freq.mul_(2.0)
+        agree(rot)
+    assert torch.equal(first, copy)  # a step captured with them goes on reading them
