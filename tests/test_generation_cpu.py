@@ -203,3 +203,24 @@ def test_tables_of_generation_follow_the_frequencies_the_module_holds(dtype):
         rot.inv_freq.mul_(2.0)
         agree(rot)
     assert torch.equal(first, copy)  # a step captured with them goes on reading them
+
+
+def test_a_wrong_rotation_position_or_scale_exceeds_the_bounds_of_the_wiring_tests():
+    """The mistakes are planted in the oracle: more than twice the attention test's bound (2 spreads) and twice the model test's,
+    over the rows of the tokens that came singly and over all of them."""
+    import generation_harness as G
+    for h, heads, part in G.ATTENTION:
+        p, d = G.layer_params(h, heads), int(h // heads * part)
+        x = torch.randn(119, h, generator=torch.Generator().manual_seed(1)).bfloat16()
+        want, spread = G.attention_by_hand(p, heads, d, x)
+        for mistake in G.MISTAKES:
+            got = G.attention_by_hand(p, heads, d, x, mistake, new=49)[0]
+            for rows in (slice(0, 119), slice(70, 119)):
+                assert (got - want)[rows].norm() > 2 * 2.0 * spread[rows].norm(), (h, mistake)
+    p = G.model_params()
+    for s in (21, 27, 50):
+        tokens = torch.randint(0, G.MODEL["V"], (s,), generator=torch.Generator().manual_seed(s))
+        want = G.model_logits(p, tokens, torch.float32)[-20:]
+        bound = 2 * G.off(G.model_logits(p, tokens, torch.bfloat16)[-20:], want) + G.U
+        for mistake in G.MISTAKES:
+            assert G.off(G.model_logits(p, tokens, torch.float32, mistake, 20)[-20:], want) > 2 * bound, (s, mistake)

@@ -211,3 +211,68 @@ def test_generation_between_replays_of_a_captured_layer():
         torch.cuda.synchronize()
         assert torch.equal(y, want), n
         del held
+
+
+@pytest.mark.parametrize("h,heads,part", [(256, 4, 0.25), (256, 2, 1.0), (512, 8, 0.25)])
+def test_attention_over_the_cache_rotates_places_and_scales(h, heads, part):
+    """The layer's attention against the definition by hand, on scores that spread by several units: two sequences that grow by chunks
+    and single tokens of their own.  Roundings are independent, so the difference over all elements stays within 2 of the spreads
+    that the harness bounds; the CPU test shows that mistakes of the wiring do not."""
+    import generation_harness as G
+    import layer_harness as LH
+    from multimodal_amd import mpu
+    from multimodal_amd.kv_cache import PagedKVCache, PagedPast
+    mpu.destroy_model_parallel()
+    mpu.initialize_model_parallel(1)
+    p, d = G.layer_params(h, heads), int(h // heads * part)
+    layer = LH.build_hip_layer(LH.make_neox_args(h, heads, torch.bfloat16, part, True, True), p, "cuda").eval()
+    layer.attention.rotary_emb.to(torch.bfloat16)
+    lens = (119, 60)
+    x = [torch.randn(n, h, generator=torch.Generator().manual_seed(i + 1)).bfloat16() for i, n in enumerate(lens)]
+    cache = PagedKVCache(1, heads, h // heads, 40, page_size=16)
+    seqs = [cache.add(n) for n in lens]
+    done, got = [0, 0], [[], []]
+    with torch.no_grad():
+        for new in [(70, 1), (1, 33), (0, 1), (20, 0), (1, 1), (1, 1), (26, 23)]:
+            rows = torch.cat([x[i][done[i]:done[i] + n] for i, n in enumerate(new)]).cuda()
+            done = [a + n for a, n in zip(done, new)]
+            past = PagedPast(cache.layers[0], cache.step(seqs, list(new), done), 130)
+            y = layer.attention(rows[:, None], None, layer_past=past)[0][:, 0].double().cpu()
+            for i, part_ in enumerate(y.split(list(new))):
+                got[i].append(part_)
+    assert done == list(lens)
+    for i in range(2):
+        want, spread = G.attention_by_hand(p, heads, d, x[i])
+        diff = torch.cat(got[i]) - want
+        assert diff.norm() <= 2 * spread.norm(), float(diff.norm() / spread.norm())
+
+
+def test_generated_logits_are_those_of_the_oracle(monkeypatch):
+    """Every step's logits against the fp32 oracle's over the whole sequence, on sharp attention: within twice what the oracle's own
+    bf16 evaluation is off, and a rounding.  The replayed run draws the same tokens."""
+    import generation_harness as G
+    import golden_params
+    from multimodal_amd import generation
+    cfg, stack = build("tiny")
+    assert (cfg["padded_vocab_size"], cfg["hidden_size"], cfg["num_attention_heads"], cfg["num_layers"], cfg["rotary_pct"]) == tuple(G.MODEL.values())
+    p = G.model_params()
+    names = {"word_embeddings.weight": "emb", "final_norm.weight": "fln.w", "final_norm.bias": "fln.b", "final_linear.weight": "head"}
+    names.update({f"layers.{i}.{k}": f"l{i}.{k}" for i in range(cfg["num_layers"]) for k in golden_params.PARAM_ORDER})
+    with torch.no_grad():
+        own = dict(stack.named_parameters())
+        for mine, theirs in names.items():
+            own[mine].copy_(p[theirs])
+    prompts = [torch.randint(0, 1024, (n,), generator=torch.Generator().manual_seed(n)) for n in (7, 1, 30)]
+    seen, head = [], generation._head
+    monkeypatch.setattr(generation, "_head", lambda *a: seen.append(head(*a)) or seen[-1])
+    out = stack.generate(prompts, maximum_tokens=20, graph=False)
+    assert len(seen) == 20
+    for i, (t, o) in enumerate(zip(prompts, out)):
+        got = torch.stack([s[i] for s in seen]).float().cpu()
+        tokens = torch.cat((t, o[:-1]))
+        want = G.model_logits(p, tokens, torch.float32)[-20:]
+        bound = 2 * G.off(G.model_logits(p, tokens, torch.bfloat16)[-20:], want) + G.U
+        assert G.off(got, want) <= bound, (i, G.off(got, want), bound)
+        assert torch.equal(got.argmax(1), o)
+    monkeypatch.undo()
+    assert all(torch.equal(a, b) for a, b in zip(out, stack.generate(prompts, maximum_tokens=20)))
