@@ -393,10 +393,10 @@ typedef struct mm_paged_step {
 /* Append: key / value rows [rows, kv->heads, hn] go to their slots; with cos / sin the first rot_d dims of the keys, and of the
  * queries on their way to q_out, are rotated by their position: x cos[p] + rotate_half(x) sin[p]
  * (megatron/model/positional_embeddings.py:69-92), products and sum in fp32, rounded once.  q / q_out [rows, nq, hn] (NULL: keys
- * and values only); q_out may be q.  cos / sin [table_rows, rot_d] contiguous, fp32 (table_fp32 != 0) or in the cache's dtype;
- * NULL with rot_d = 0: no rotation.  rot_d even.  Strides in elements, any alignment of the rows (16-byte aligned rows with
- * strides a multiple of 8 and rot_d a multiple of 16 take the wide path).  Two rows of one call must not share a slot, and
- * rows must not overlap the cache. */
+ * and values only); q_out may be q (the same strides), and else overlaps neither q, k, v nor itself (refused).  cos / sin
+ * [table_rows, rot_d] contiguous, fp32 (table_fp32 != 0) or in the cache's dtype; NULL with rot_d = 0: no rotation.  rot_d even.
+ * Strides in elements, any alignment of the rows (16-byte aligned rows with strides a multiple of 8 and rot_d a multiple of 16
+ * take the wide path).  Two rows of one call must not share a slot, and rows must not overlap the cache. */
 int mm_paged_kv_append(const mm_paged_kv* kv, const mm_paged_step* step, const void* k, int64_t k_row, int64_t k_head,
                        const void* v, int64_t v_row, int64_t v_head, const void* q, int64_t q_row, int64_t q_head, void* q_out,
                        int64_t qo_row, int64_t qo_head, int nq, int rows, const void* cos, const void* sin, int rot_d,
@@ -409,8 +409,9 @@ int mm_paged_kv_append(const mm_paged_kv* kv, const mm_paged_step* step, const v
  * -inf; rows of no sequence are left as they were.  What the cache holds behind a sequence's end, and infinities or NaN in keys
  * and values that a row does not see, do not reach it; an infinite value that it does see is infinite in its output, however small
  * its weight.  q, out [rows, nq, hn]: 16-byte aligned, strides a multiple of 8 elements; lse [rows, nq] with row stride l_row; out
- * and lse overlap neither the inputs nor themselves.  workspace: mm_paged_attn_workspace_bytes bytes (0: none; it depends on the shapes and
- * bounds alone), 16-byte aligned; calls that share one must not overlap.  Deterministic. */
+ * may be q (the same strides), else out and lse overlap neither the inputs nor each other nor themselves (refused where it is q
+ * or they).  workspace: mm_paged_attn_workspace_bytes bytes (0: none; it depends on the shapes and bounds alone), 16-byte
+ * aligned; calls that share one must not overlap.  Deterministic. */
 size_t mm_paged_attn_workspace_bytes(const mm_paged_kv* kv, const mm_paged_step* step, int nq, int rows);
 int mm_paged_attn_fwd(const mm_paged_kv* kv, const mm_paged_step* step, void* out, int64_t o_row, int64_t o_head, float* lse,
                       int64_t l_row, const void* q, int64_t q_row, int64_t q_head, int nq, int rows, float softmax_scale,

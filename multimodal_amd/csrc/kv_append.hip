@@ -180,6 +180,14 @@ template <typename T, typename TT, int W, int HN> static int launch_append_hn(co
     const int parts = shared ? 1 : (items + 255) / 256;
     const int64_t blocks = shared ? ((int64_t)a.rows + per - 1) / per : (int64_t)parts * a.rows;
     MM_CHECK_ARG(blocks < (int64_t)1 << 24, "mm_paged_kv_append: %d rows of %d items exceed the grid limit", a.rows, items);
+    if (a.nq) {  // items of a row are moved by different lanes, rows by different workgroups: in place, or apart
+        const auto runs = [&](const void* p, int64_t row, int64_t head, int heads) { return Runs{p, 2 * row, 2 * head, 2 * HN, a.rows, heads}; };
+        const Runs out = runs(a.q_out, a.qo_row, a.qo_head, a.nq), q = runs(a.q, a.q_row, a.q_head, a.nq);
+        MM_CHECK_ARG(!overlaps_itself(out), "mm_paged_kv_append: q_out overlaps itself");
+        MM_CHECK_ARG(out.same(q) || !overlap(out, q), "mm_paged_kv_append: q_out overlaps q in part");
+        MM_CHECK_ARG(!overlap(out, runs(a.k, a.k_row, a.k_head, a.kv.heads)) && !overlap(out, runs(a.v, a.v_row, a.v_head, a.kv.heads)),
+                     "mm_paged_kv_append: q_out overlaps k or v");
+    }
     if (shared) paged_kv_append_rows_k<T, TT, W, HN><<<(unsigned)blocks, 256, 0, st>>>(a, per, make_fastdiv(items));
     else paged_kv_append_k<T, TT, W, HN><<<(unsigned)blocks, 256, 0, st>>>(a, parts);
     MM_CHECK_LAUNCH();

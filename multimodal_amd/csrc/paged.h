@@ -63,6 +63,50 @@ __device__ __forceinline__ int find_seq(const int32_t* __restrict__ cu, int n, i
     }
 }
 
+// Host side: do operands share memory?  An operand is rows x heads runs of `width` bytes, strides in bytes.
+struct Runs {
+    const void* p;
+    int64_t row, head, width;
+    int rows, heads;
+    int64_t first() const { return (int64_t)(uintptr_t)p + (row < 0 ? (rows - 1) * row : 0) + (head < 0 ? (heads - 1) * head : 0); }
+    int64_t end() const { return (int64_t)(uintptr_t)p + (row > 0 ? (rows - 1) * row : 0) + (head > 0 ? (heads - 1) * head : 0) + width; }
+    bool same(const Runs& o) const { return p == o.p && heads == o.heads && (rows == 1 || row == o.row) && (heads == 1 || head == o.head); }
+};
+// |d + n row| < width for some |n| < rows: two runs d apart, or some rows further on
+inline bool meets(int64_t d, int64_t row, int rows, int64_t width) {
+    int64_t near = row == 0 ? 0 : -d / row;
+    near = near < 1 - rows ? 1 - rows : near > rows - 1 ? rows - 1 : near;
+    for (int64_t n = near - 1; n <= near + 1; ++n)
+        if (n > -rows && n < rows && d + n * row < width && d + n * row > -width) return true;
+    return false;
+}
+inline bool overlaps_itself(const Runs& a) {
+    const int64_t row = a.row < 0 ? -a.row : a.row, head = a.head < 0 ? -a.head : a.head;
+    if (a.rows > 1 && row < a.width) return true;
+    if (a.heads > 1 && head < a.width) return true;
+    if (a.rows == 1 || a.heads == 1 || row >= (a.heads - 1) * head + a.width || head >= (a.rows - 1) * row + a.width) return false;
+    for (int i = 1; i < a.heads; ++i)
+        if (meets(i * a.head, a.row, a.rows, a.width)) return true;
+    return false;
+}
+// Exact for operands of the same rows and row stride (slices of one tensor); others count as overlapping if the stretches of memory they span do.
+inline bool overlap(const Runs& a, const Runs& b) {
+    if (a.end() <= b.first() || b.end() <= a.first()) return false;
+    if (a.rows != b.rows || a.width != b.width || (a.rows > 1 && a.row != b.row)) return true;
+    const int64_t d = (int64_t)(uintptr_t)a.p - (int64_t)(uintptr_t)b.p;
+    if (a.head == b.head && a.head >= 2 * a.width && a.row % a.head == 0) {  // e.g. [rows, heads, 3, hn]: places within a head
+        const int64_t at = (d % a.head + a.head) % a.head;
+        if (at >= a.width && at <= a.head - a.width) return false;
+    }
+    if (a.head != b.head && (int64_t)a.heads * b.heads > 1 << 16) return true;  // not worth the search
+    for (int i = 0; i < a.heads; ++i)
+        for (int j = 0; j < b.heads; ++j) {
+            if (a.head == b.head && i > 0 && j > 0) break;  // the difference i - j has been seen
+            if (meets(d + i * a.head - j * b.head, a.row, a.rows, a.width)) return true;
+        }
+    return false;
+}
+
 inline int check_paged(const char* fn, const mm_paged_kv* kv, const mm_paged_step* st, int rows) {
     MM_CHECK_ARG(kv && st, "%s: null cache or step", fn);
     MM_CHECK_ARG(kv->k && kv->v && (st->seqs == 0 || (st->block_table && st->cu_new && st->kv_lens)), "%s: null pointer", fn);

@@ -890,6 +890,12 @@ static PagedPlan plan(const mm_paged_kv& kv, const mm_paged_step& st, int nq) {
 }
 
 template <typename T, int HD> static int launch_paged_attn(const PagedAttnArgs& a, const PagedPlan& p, hipStream_t st) {
+    const Runs out = {a.out, 2 * a.o_row, 2 * a.o_head, 2 * HD, a.rows, a.nq}, q = {a.q, 2 * a.q_row, 2 * a.q_head, 2 * HD, a.rows, a.nq};
+    const Runs lse = {a.lse, 4 * a.l_row, 0, 4 * (int64_t)a.nq, a.rows, 1};
+    MM_CHECK_ARG(!overlaps_itself(out) && !overlaps_itself(lse), "mm_paged_attn_fwd: out or lse overlaps itself");
+    // a workgroup has read its rows' queries before it, or the joining launch, writes their outputs
+    MM_CHECK_ARG(out.same(q) || !overlap(out, q), "mm_paged_attn_fwd: out overlaps q in part");
+    MM_CHECK_ARG(!overlap(lse, q) && !overlap(lse, out), "mm_paged_attn_fwd: lse overlaps q or out");
     const unsigned bx = (unsigned)(a.st.seqs * a.kv.heads);
     const int many = p.row_blocks * p.many_splits;
     const dim3 grid(bx, p.few ? p.few_splits : (p.few_splits > many ? p.few_splits : many));

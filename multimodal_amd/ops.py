@@ -742,8 +742,8 @@ def _out_rows(name, t, shape, dtype, device):
 def paged_kv_append(kv, step, k, v, q=None, cos=None, sin=None, q_out=None):
     """The step's key / value rows [rows, kv.heads, hn] into their slots of the cache; with cos / sin tables [positions, d] (fp32
     or the cache's dtype) the first d dims of the keys, and of the queries q [rows, nq, hn] on their way to q_out, are rotated by
-    each row's position.  kv: kv_cache.PagedKV, step: kv_cache.PagedStep.  Returns q_out (allocated unless given; it may be q;
-    rows of no sequence are left as they were), or None without q.  k, v and q may be strided views, e.g. the slices of the
+    each row's position.  kv: kv_cache.PagedKV, step: kv_cache.PagedStep.  Returns q_out (allocated unless given; it may be q, and
+    overlaps nothing else; rows of no sequence are left as they were), or None without q.  k, v and q may be strided views, e.g. the slices of the
     layer's fused [rows, heads, 3, hn] projection.  No backward: generation only."""
     dev = kv.device
     if dev != step.device:
@@ -780,8 +780,8 @@ def paged_kv_append(kv, step, k, v, q=None, cos=None, sin=None, q_out=None):
 def paged_attn_fwd(kv, step, q, softmax_scale, out=None, lse=None):
     """Attention of the step's new rows q [rows, nq, hn] over the cache (append their keys and values first): a row at position p
     sees keys 0 .. p of its sequence, query head h reads key head h // (nq // kv.heads).  Returns (out [rows, nq, hn], lse [rows,
-    nq] fp32), allocated unless given; rows of no sequence are left as they were, a row that sees no key gets 0 and -inf.  No
-    backward: generation only."""
+    nq] fp32), allocated unless given (out may be q, and they overlap nothing else); rows of no sequence are left as they were, a row
+    that sees no key gets 0 and -inf.  No backward: generation only."""
     dev = kv.device
     if dev != step.device:
         raise RuntimeError(f"paged_attn_fwd: cache on {dev}, step on {step.device}")

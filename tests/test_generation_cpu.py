@@ -224,3 +224,42 @@ def test_a_wrong_rotation_position_or_scale_exceeds_the_bounds_of_the_wiring_tes
         bound = 2 * G.off(G.model_logits(p, tokens, torch.bfloat16)[-20:], want) + G.U
         for mistake in G.MISTAKES:
             assert G.off(G.model_logits(p, tokens, torch.float32, mistake, 20)[-20:], want) > 2 * bound, (s, mistake)
+
+
+def test_outputs_that_overlap_are_refused():
+    """Rows 256 elements apart, heads 64 (4 heads of 64), from address 1 << 20; every call here is refused before any launch."""
+    lib = _lib.get_lib()
+    at = 1 << 20
+    far = at + (1 << 16)
+
+    def append(q_out, qo=(256, 64), q=at, qs=(256, 64), k=far, v=2 * far, rows=8):
+        a, b, pa, pb = refs()
+        return lib.mm_paged_kv_append(pa, pb, k, 256, 64, v, 256, 64, q, *qs, q_out, *qo, 4, rows, 0, 0, 0, 0, 0, None), lib.mm_last_error().decode()
+
+    def attend(out, os=(256, 64), q=at, qs=(256, 64), lse=far, l_row=4, rows=8):
+        a, b, pa, pb = refs()
+        return lib.mm_paged_attn_fwd(pa, pb, out, *os, lse, l_row, q, *qs, 4, rows, 0.125, 0, 0, None), lib.mm_last_error().decode()
+
+    three = (768, 192)  # a slice of [rows, heads, 3, 64]
+    for call in (append, attend):
+        for bad, text in [(dict(), "in part"),                                   # q moved by 8 elements
+                          (dict(shift=512), "in part"),                          # by a row
+                          (dict(shift=-128), "in part"),                         # by a head
+                          (dict(strides=three, other=three), "in part"),
+                          (dict(shift=2 * 192, strides=three, other=three), "in part"),   # by a head of the fused projection
+                          (dict(shift=0, strides=(512, 64)), "in part"),
+                          (dict(shift=0, strides=(256, 72)), "itself"),          # the rows reach into each other
+                          (dict(shift=0, strides=(0, 64)), "itself"),
+                          (dict(shift=0, strides=(256, 56)), "itself"),
+                          (dict(shift=0, strides=(64, 64)), "itself")]:
+            bad = {"shift": 16, "strides": (256, 64), "other": (256, 64), **bad}
+            rc, msg = call(at + bad["shift"], bad["strides"], qs=bad["other"])
+            assert rc == -1 and text in msg, (bad, rc, msg)
+    for other in ("k", "v"):
+        for where in (at, at + 2 * 63, at + 2 * 256 * 7):
+            rc, msg = append(at, **{other: where})
+            assert rc == -1 and "k or v" in msg, (other, where, msg)
+    for lse in (at, at + 2 * 256 * 7 + 2 * 192, far):
+        rc, msg = attend(far, lse=lse)
+        assert rc == -1 and "lse overlaps" in msg, (lse, msg)
+    assert attend(far, lse=2 * far, l_row=3)[0] == -1

@@ -429,3 +429,32 @@ def test_append_many_rows_equals_few(nq, nkv, hn, d):
     assert torch.equal(torch.isnan(out), torch.isnan(ref)) and torch.equal(out.nan_to_num(), ref.nan_to_num())
     assert bool(torch.isnan(out).any()) and bool((out[int(c.cu[-1]):] == 7).all())
     assert torch.equal(many.k, few.k) and torch.equal(many.v, few.v)
+
+
+def test_outputs_beside_their_inputs():
+    """q_out in a slot of its own in the fused projection, out in the queries' place: the bits of outputs apart; outputs that meet their
+    inputs otherwise are refused."""
+    from multimodal_amd import ops
+    for seqs in ([(4, 20), (1, 3)], [(1, 3000), (3, 500)], [(40, 60), (70, 3000)]):
+        c = Case(seqs, nq=4, nkv=4, hn=64, ps=16, dtype=BF16)
+        cos, sin = (t.cuda() for t in tables(3000, 16, BF16))
+        kv, step = c.kv(), c.step()
+        ref_q = ops.paged_kv_append(kv, step, c.k.cuda(), c.v.cuda(), q=c.q.cuda(), cos=cos, sin=sin)
+        ref = ops.paged_attn_fwd(kv, step, ref_q, c.scale)
+        four = torch.stack((c.q, c.k, c.v, torch.zeros_like(c.q)), dim=2).cuda()
+        q, k, v, out = four.unbind(2)
+        assert torch.equal(ops.paged_kv_append(kv, step, k, v, q=q, cos=cos, sin=sin, q_out=out), ref_q)
+        assert torch.equal(q.cpu(), c.q) and torch.equal(k.cpu(), c.k) and torch.equal(v.cpu(), c.v)
+        got = ops.paged_attn_fwd(kv, step, out, c.scale, out=q)
+        assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+        got = ops.paged_attn_fwd(kv, step, out, c.scale, out=out)
+        assert torch.equal(out, ref[0]) and torch.equal(got[1], ref[1])
+        wide = torch.zeros(c.rows + 1, 4, 64, dtype=BF16, device="cuda")
+        with pytest.raises(RuntimeError, match="in part"):
+            ops.paged_attn_fwd(kv, step, wide[:-1], c.scale, out=wide[1:])
+        with pytest.raises(RuntimeError, match="in part"):
+            ops.paged_kv_append(kv, step, k, v, q=wide[:-1], q_out=wide[1:])
+        with pytest.raises(RuntimeError, match="k or v"):
+            ops.paged_kv_append(kv, step, k, v, q=c.q.cuda(), q_out=v)
+        with pytest.raises(RuntimeError, match="lse overlaps"):
+            ops.paged_attn_fwd(kv, step, wide[:-1], c.scale, lse=wide.view(-1).view(torch.float32)[:c.rows * 4].view(c.rows, 4))
