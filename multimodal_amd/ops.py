@@ -721,6 +721,8 @@ def _rows(name, t, kv, rows=None, heads=None):
             or t.dtype != kv.dtype or t.device != kv.device):
         raise RuntimeError(f"{name} must be a [{'rows' if rows is None else rows}, {'heads' if heads is None else heads}, {kv.hn}] "
                            f"{kv.dtype} tensor on {kv.device}, got {tuple(shape)} {t.dtype} on {t.device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} requires a gradient, but there is no backward: call it under torch.no_grad()")
     stride = t.stride()
     if stride[2] != 1:
         t = t.contiguous()

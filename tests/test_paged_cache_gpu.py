@@ -458,3 +458,22 @@ def test_outputs_beside_their_inputs():
             ops.paged_kv_append(kv, step, k, v, q=c.q.cuda(), q_out=v)
         with pytest.raises(RuntimeError, match="lse overlaps"):
             ops.paged_attn_fwd(kv, step, wide[:-1], c.scale, lse=wide.view(-1).view(torch.float32)[:c.rows * 4].view(c.rows, 4))
+
+
+def test_operands_that_want_a_gradient_are_refused():
+    """There is no backward: a gradient would stop here without a word."""
+    from multimodal_amd import ops
+    c = Case([(2, 9)], nq=2, nkv=2, hn=64, ps=16, dtype=BF16)
+    kv, step = c.kv(), c.step()
+    k, v, q = c.k.cuda(), c.v.cuda(), c.q.cuda()
+    for which in range(3):
+        t = [k, v, q]
+        t[which] = t[which].clone().requires_grad_(True)
+        with pytest.raises(RuntimeError, match="no backward"):
+            ops.paged_kv_append(kv, step, t[0], t[1], q=t[2])
+        with torch.no_grad():
+            ops.paged_kv_append(kv, step, t[0], t[1], q=t[2])
+    with pytest.raises(RuntimeError, match="no backward"):
+        ops.paged_attn_fwd(kv, step, q.clone().requires_grad_(True), c.scale)
+    with torch.no_grad():
+        ops.paged_attn_fwd(kv, step, q.clone().requires_grad_(True), c.scale)
