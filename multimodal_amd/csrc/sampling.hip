@@ -470,7 +470,7 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
         // Borders.  One wave, a second one for min-p beside it (BIG: every wave alike, because recounting a chunk takes the whole
         // workgroup).
         {
-            auto counts = [&](int c) -> uint32_t {
+            auto counts = [&](int c) __attribute__((always_inline)) -> uint32_t {
                 if constexpr (!BIG) return (sm.hist[(c & 511) * 65 + lane] >> (c < 512 ? 0 : 16)) & 0xffffu;
                 __syncthreads();
                 if (tid < 64) sm.one_chunk[tid] = 0;
@@ -492,7 +492,7 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
                 int dk, j;
                 double upto;
             };
-            auto find = [&](double t) -> Found {
+            auto find = [&](double t) __attribute__((always_inline)) -> Found {
                 int c = first_of([&](int i) { return sm.mass[i] > t; });
                 uint32_t n = counts(c);
                 if (__ballot(n != 0) == 0) {
@@ -514,7 +514,7 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
                 return Found{64 * c + l, (int)lane_u((uint32_t)(int)jj, l), lane_d(up, l)};
             };
             // the first value that weighs too little to be kept: 64-way search in the order
-            auto first_below = [&]() -> int {
+            auto first_below = [&]() __attribute__((always_inline)) -> int {
                 int from = lo, span = 65536 - lo;
                 while (span > 0) {
                     const int st = (span + 63) >> 6, at = from + lane * st + st - 1;
@@ -541,7 +541,7 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
                 if (lane == 0) sm.min_p_mass = m;
             }
             // the number of tokens of the values ahead of this one
-            auto tokens_ahead = [&](int d) -> uint32_t {
+            auto tokens_ahead = [&](int d) __attribute__((always_inline)) -> uint32_t {
                 const int c = min(d, 65535) >> 6;
                 const uint32_t n = counts(c);
                 return (c ? sm.count[c - 1] : 0u) + lane_u(scan_u(64 * c + lane < d ? n : 0u), 63);
