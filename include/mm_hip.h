@@ -382,7 +382,9 @@ typedef struct mm_paged_kv {
  *   - a row whose position is negative, behind block_table's last page, behind the cos / sin tables, or in a page outside
  *     [0, num_pages) leaves the cache alone, and its q_out row is NaN;
  *   - attention: a key in a page outside [0, num_pages) makes every row that sees it NaN, and a sequence that exceeds max_new,
- *     max_kv, its block_table row or the packed rows has all its rows NaN (a wrong step never gives a wrong number). */
+ *     max_kv, its block_table row or the packed rows has all its rows NaN, so that these give no wrong number; a row whose
+ *     position is negative (a length below the new rows, or below 0) sees no key, and has the result of such a row, 0 and -inf;
+ *   - max_new = 0 says that no sequence brings a row: attention does nothing then, whatever the arrays hold. */
 typedef struct mm_paged_step {
     const int32_t* block_table;
     const int32_t* cu_new;

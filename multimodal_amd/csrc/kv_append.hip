@@ -8,8 +8,9 @@
 // rotated head the chunk and its partner half a rotation further, so that the rotation needs no exchange between lanes; the
 // lanes of a head's row are neighbours, so every access is a contiguous run of at least d bytes.  W = 8 (16-byte accesses) when
 // rows and rotation allow it, else W = 1.
-// Measured: 4 prompts of 2001 .. 2048 tokens, 32 + 2 x 32 heads of 128: 75 us, 399 MB at 5.3 TB/s, what a large copy reaches; 16 of
-// 2048, 32 + 2 x 8 heads: 166 us, 4.9 TB/s; 256 rows of one token 4.6 us, one row 2.7 us, the latency of sequence -> length -> page.
+// Measured: 4 prompts of 2001 .. 2048 tokens, 32 + 2 x 32 heads of 128: 76 us, 399 MB at 5.3 TB/s, what a large copy reaches; 16 of
+// 2048, 32 + 2 x 8 heads: 159 us, 806 MB at 5.1 TB/s; 256 rows of one token 4.6 us, one row 2.6 us, the latency of sequence ->
+// length -> page.
 #include "common.h"
 #include "paged.h"
 
@@ -172,9 +173,22 @@ __global__ __launch_bounds__(256) void paged_kv_append_rows_k(const AppendArgs a
 template <typename T, typename TT, int W, int HN> static int launch_append_hn(const AppendArgs& a, hipStream_t st) {
     const int items = (a.nq + 2 * a.kv.heads) * (HN / (2 * W));
     // One row a block leaves lanes idle where its items are few, or a little over 256; then several rows share one, once that leaves
-    // 4 blocks a CU.  8 x 2048 tokens and more: 72 items (16 / 1 heads of 64) 43 -> 30.6 us, 288 (32 / 2 of 128) 92 -> 72, 320 with
-    // fp32 tables 98 -> 75, 384 183 -> 166; but 192 (16 / 16 of 64) 87 -> 96, 768 (32 / 32 of 128) 75 -> 89.  The narrow path is short of
-    // loads in flight: 1536 items of 64 with 20 rotated dims 61 -> 44.6.
+    // 4 blocks a CU.  bf16, us with 1 / 2 / 8 rows a block (the kept one in brackets; 8 from 8192 rows on), at 4096, 8192 and
+    // 32768 rows:
+    //   72 items (16 / 1 of 64; 38 MB at 8192 rows): [8.5] / 7.9 / 8.5, 13.9 / 13.4 / [10.6], 42.4 / 40.8 / [29.0]
+    //   96 items (16 / 4 of 64; 51 MB at 8192 rows): [8.7] / 8.4 / 8.7, 14.5 / 14.6 / [12.5], 43.1 / 42.4 / [35.5]
+    //   112 items (24 / 2 of 64; 59 MB at 8192 rows): [9.1] / 9.0 / 9.1, [15.0] / 16.3 / 14.7, [44.6] / 45.6 / 40.2
+    //   144 items (32 / 2 of 64; 76 MB at 8192 rows): [10.2] / 10.9 / 10.2, [16.7] / 19.0 / 17.4, [72.8] / 82.1 / 68.6
+    //   160 items (32 / 4 of 64; 84 MB at 8192 rows): [10.6] / 11.5 / 10.7, [17.2] / 19.6 / 18.3, [75.5] / 85.1 / 76.4
+    //   192 items (16 / 16 of 64; 101 MB at 8192 rows): [11.4] / 13.0 / 11.5, [18.4] / 21.0 / 19.8, [86.7] / 96.0 / 91.3
+    //   224 items (24 / 2 of 128; 118 MB at 8192 rows): [13.3] / 14.9 / 13.3, [22.2] / 24.8 / 23.1, [91.2] / 101.9 / 104.1
+    //   256 items (24 / 4 of 128; 135 MB at 8192 rows): [15.0] / 16.9 / 14.8, [24.8] / 28.6 / 26.1, [100.9] / 113.0 / 117.9
+    //   288 items (32 / 2 of 128; 152 MB at 8192 rows): 21.1 / [18.2] / 21.1, 37.0 / [29.2] / 28.2, 159.5 / [131.3] / 130.9
+    //   384 items (32 / 8 of 128; 202 MB at 8192 rows): 22.1 / [21.0] / 22.0, 39.0 / [35.6] / 35.4, 170.2 / [159.5] / 171.4
+    //   768 items (32 / 32 of 128; 404 MB at 8192 rows): [33.0] / 36.0 / 33.2, [75.9] / 88.3 / 89.5
+    // (Data below 256 MB may come from the Infinity Cache: the calls timed repeat on the same rows.)  Between 97 and 256 items 8 rows a
+    // block win by up to 10 % at 32768 rows of 112 and 144 items and lose as much from 192 on or at 8192 rows.  The narrow path is
+    // short of loads in flight: 1536 items of 64 with 20 rotated dims 61 -> 44.6.
     const int per = items <= 96 ? 8 : W == 1 || (items > 256 && items <= 384) ? 2 : 1;
     const bool shared = per > 1 && a.rows / per >= 1024;
     const int parts = shared ? 1 : (items + 255) / 256;

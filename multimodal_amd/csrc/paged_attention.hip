@@ -7,8 +7,13 @@
 // key or value tile is read once for all of them.
 //
 // Softmax runs in the exp2 domain with fp32 statistics in one pass over the keys; products accumulate in fp32; the
-// probabilities (at most 2^kLag, see there) are rounded to the cache's dtype for the matrix instruction of P V - few rows: in two
-// parts, so that nothing is lost - and the row sum takes them unrounded.
+// probabilities (at most 2^kLag, see there) are rounded to the cache's dtype for the matrix instruction of P V and the row sum takes
+// them unrounded.  The few-row form, whose matrix unit is idle, takes what that rounding leaves over in a second instruction, so
+// that nothing is lost: bf16 outputs are 0.0017 (relative, over all elements) from the definition, which is their own rounding.  The
+// many-row form does not, as the training forward does not: 0.0021 (prompts at head size 64) and 0.0023 (a chunk at 128), fp16 0.00029
+// against 0.00021.  With the second instruction its outputs were as near as the few-row form's, at a fifth to a third more time (4 x
+// 2048 tokens, 16 heads of 64: 64.7 -> 78.5 us; 1024 over 17k, 32 / 8 heads of 128: 301 -> 401; 12 sequences, 18 heads of 128: 60.9 ->
+// 77.1).  Which form a sequence takes follows from its rows per key head (kFewRows) alone, never from what else is in the step.
 //
 // Masked places never matter: a score behind a row's position is replaced by -inf (not added to), value rows behind the
 // sequence's end are zeroed on their way into LDS, and where a tile holds keys that some of its rows do not see, infinities and
@@ -142,8 +147,9 @@ template <> struct M16<F16> {
 //   softmax over the keys of a column: 8 registers and the four 16-lane groups;
 //   O^T[dim][row] += V^T P^T: P^T is S^T's registers as they stand - register j of sub-tile t in group g is key 16 t + 4 g + j,
 //   and the V^T operand takes its keys in that order - V through a wave-private LDS tile, read transposed (ds_read_b64_tr_b16).
-// Measured: 64 sequences of 5 .. 2047 keys, 32 heads of 128 in bf16: 198 us, 1.08 GB at 5.5 TB/s; 2 of 131k, 32 / 4 heads: 97 us with
-// the joining, 5.2 TB/s; one of 701, 16 heads of 64: 10 us, the latency of one workgroup's chain of loads.
+// Measured: 64 sequences of 5 .. 2047 keys, 32 heads of 128 in bf16: 198 us, 1.08 GB at 5.5 TB/s; 2 of 99k and 131k, 32 / 4 heads: 97 us
+// with the joining, 5.2 TB/s (90 without, 0.51 GB at 5.7); one of 701, 16 heads of 64: 9.5 us, the latency of one workgroup's chain
+// of loads.
 // The LDS rows are unpadded; the 32-byte units of a row are XOR-ed with the row so that the transposed reads (16 rows, one unit
 // each) and the writes (16 rows, two units each) spread evenly over the banks.
 template <int HD> __device__ __forceinline__ int v_off(int row, int byte) {
@@ -407,11 +413,13 @@ __device__ __forceinline__ void paged_attn_few(const PagedAttnArgs& a, char* sme
 // wave owns 32 rows on the lane index of mfma 32x32x16 score tiles; keys and values come in 64-key tiles, global -> registers ->
 // double-buffered LDS, one barrier a tile; page ids are fetched a tile further ahead, so that no load waits for another.  Row
 // blocks with the most keys start first.
-// Measured: 1024 tokens over 17k, 32 / 8 heads of 128: 287 us with the joining, 960 TFLOP/s; 4 x 2048 tokens, 16 heads of 64: 58 us, 590
-// TFLOP/s of what the causal mask leaves.  A wave's 64-key tile at 128 takes 4070 cycles beside a second wave on its SIMD: 1024 of
-// matrix instructions, about 900 of softmax, 350 .. 550 each for issuing the loads and writing LDS, the rest waiting for the other
-// wave, whose matrix instructions hold the vector unit up (8 cycles each) and the other way round.  The clock falls with the work
-// per cycle (1.88 GHz here, 1.73 at head size 64; a schedule of 4440 cycles a tile ran at 2.03).
+// Measured: 1024 tokens over 17k, 32 / 8 heads of 128: 282 us with the joining, 980 TFLOP/s; 4 x 2048 tokens, 16 heads of 64: 57
+// us, 600 TFLOP/s of what the causal mask leaves (on other boards, or after many calls without a pause, up to 301 and 65).  The
+// occupancy bounds leave 7 registers spilled, written ahead of the tile loops and read behind them or once a pass, never inside.  A
+// wave's 64-key tile at 128 takes 4070 cycles beside a second wave on its SIMD: 1024 of matrix instructions, about 900 of softmax,
+// 350 .. 550 each for issuing the loads and writing LDS, the rest waiting for the other wave, whose matrix instructions hold the
+// vector unit up (8 cycles each) and the other way round.  The clock falls with the work per cycle (1.88 GHz here, 1.73 at head
+// size 64; a schedule of 4440 cycles a tile ran at 2.03).
 // LDS rows are unpadded; the 16-byte chunks of a row are XOR-ed with the row so that the row reads (16 rows, one chunk) and the
 // transposed reads (4 rows, 4 chunks) both meet all banks once.
 template <int HD> struct KvTile {

@@ -24,8 +24,9 @@
 //
 // Bound by a row's chain of steps in one CU, not by HBM.  50304 fp16 logits, cycles: row and LDS atomics (1024 wave instructions) 11400,
 // chunk sums 5300 (vector instructions), scan 1600, borders 4300, match 2400; the list instead of all of that 12000.  Kernel times:
-// one row of bf16 with top-k 40: 9.2 us; 64 rows, top-p and min-p: 15 us; 512 rows with parameters of their own (two
-// rows a CU after each other): 30 us, 51.5 MB at 1.7 TB/s.
+// one row of bf16 with top-k 40: 8.4 us; 64 rows, top-p and min-p: 15 us; 512 rows with parameters of their own (two
+// rows a CU after each other): 30 us, 51.5 MB at 1.7 TB/s.  BIG rows, read again for every recount: 64 of 65529 47 us (65528: 16), 64 of
+// 128256 78 us, 190 of them 95.
 #include "common.h"
 
 namespace mm {
@@ -650,8 +651,9 @@ template <typename T, bool BIG> __global__ __launch_bounds__(kSampleThreads) voi
 }
 
 // =====================================================================================  every row greedy
-// One workgroup a row: the largest value and the first 16-byte chunk that holds it, then the index inside that chunk.  Rows of 8000
-// logits, 3125 of them: 16 us, 50 MB at 3.2 TB/s.
+// One workgroup a row: the largest value and the first 16-byte chunk that holds it, then the index inside that chunk.  3125 rows of
+// 8000 logits: 11 us, 50 MB at 4.4 TB/s (from the Infinity Cache as well as from HBM); 50000 of 500: 57 us - three quarters of the
+// lanes have no chunk, and a row's join and second look at its chunk wait for each other.
 template <typename T, int THREADS> __global__ __launch_bounds__(THREADS) void sample_greedy_k(const SampleArgs a) {
     constexpr int WAVES = THREADS / 64;
     __shared__ unsigned long long best_of[WAVES];
@@ -859,11 +861,15 @@ extern "C" int mm_sample_tokens(int64_t* tokens, const void* logits, int64_t row
     hipStream_t st = (hipStream_t)stream;
     return dispatch_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        // Where the scalar temperature says that every row is greedy, nothing needs the histogram (50000 rows of 500 484 -> 60 us,
-        // 3125 of 8000 38 -> 16).  Its workgroups cost the same however small the vocabulary; a wave's sort of a small row takes
-        // longer the more keys a lane has, but 16 and more rows share a CU: 505 logits always (50000 rows of 500, top-p 1641 -> 145 us,
-        // 64 rows 10.4 -> 9.5), 1017 from two rows a CU on (64 rows 10.4 against 16.6, 300 rows 19.0 -> 16.8), 2041 from five on (300 rows
-        // of 2000 18.9 against 31, 2000 rows 73 -> 47).  16-bit counts and kSampleSteps 16-byte chunks per thread hold 65535 logits.
+        // Where the scalar temperature says that every row is greedy, nothing needs the histogram (50000 rows of 500 484 -> 57 us,
+        // 3125 of 8000 38 -> 12).  Workgroups of 256 or 1024 threads, us: 1 row of 8000 4.4 / 4.4, of 16384 5.2 / 4.6, of 32000 6.8
+        // / 5.1, 512 rows of 8000 5.3 / 5.8, of 16384 6.1 / 6.4, of 20000 8.0 / 6.3, of 50304 14.8 / 11.6, 1525 rows of 16384 11.6
+        // / 15.6; only beyond some 800 rows of 20000 .. 32000 are the smaller ones ahead again (1250 of 20000 10.9 / 14.0, 781 of
+        // 32000 11.5 / 13.1). The histogram's workgroups cost the same however small the vocabulary; a wave's sort of a small row
+        // takes longer the more keys a lane has, but 16 and more rows share a CU: 505 logits always (50000 rows of 500, top-p 1641
+        // -> 145 us, 64 rows 10.4 -> 9.5), 1017 from two rows a CU on (64 rows 10.4 against 16.6, 300 rows 19.0 -> 16.8), 2041 from
+        // five on (300 rows of 2000 18.9 against 31, 2000 rows 73 -> 47).  16-bit counts and kSampleSteps 16-byte chunks per thread
+        // hold 65535 logits.
         if (!temperature_rows && !(temperature > 0.f)) {
             if (vocab <= 16384) sample_greedy_k<T, 256><<<rows, 256, 0, st>>>(a);
             else sample_greedy_k<T, 1024><<<rows, 1024, 0, st>>>(a);

@@ -42,7 +42,7 @@ class PagedStep:
     [seqs]: its length including them.  max_new, max_kv: upper bounds of a sequence's new rows and length (defaults: read from
     the arrays, which waits for the GPU).  The kernels read the arrays when they run, so their contents may be rewritten between
     the replays of a captured step; a step that breaks the bounds, or names pages the cache does not have, gives NaN rows and
-    leaves the cache alone (include/mm_hip.h, mm_paged_step)."""
+    leaves the cache alone, and a row at a negative position attends to nothing: 0 (include/mm_hip.h, mm_paged_step)."""
 
     def __init__(self, block_table, cu_new, kv_lens, max_new=None, max_kv=None):
         if block_table.dim() != 2 or cu_new.dim() != 1 or kv_lens.dim() != 1:
