@@ -477,3 +477,101 @@ def test_operands_that_want_a_gradient_are_refused():
         ops.paged_attn_fwd(kv, step, q.clone().requires_grad_(True), c.scale)
     with torch.no_grad():
         ops.paged_attn_fwd(kv, step, q.clone().requires_grad_(True), c.scale)
+
+
+# --------------------------------------------------------------------------- calls that the documentation allows, less usual ones
+@pytest.mark.parametrize("hn,dtype", [(64, BF16), (128, F16)])
+@pytest.mark.parametrize("group,nkv", [(17, 1), (32, 2), (71, 1)])
+def test_attention_single_tokens_of_many_heads_a_key(hn, dtype, group, nkv):
+    """More than 16 query heads on a key head: single tokens in the form of chunks, in one piece and split."""
+    c = Case([(1, 1), (1, 40), (0, 7), (1, 200), (2, 65)], nq=group * nkv, nkv=nkv, hn=hn, ps=16, dtype=dtype, pad=1, garbage=float("nan"))
+    check_attention(c, *run_attention(c))
+    check_attention(c, *run_attention(c, max_kv=6000))
+
+
+@pytest.mark.parametrize("hn", [64, 128])
+@pytest.mark.parametrize("ps", [1, 7, 300])
+def test_attention_chunks_over_pages_of_any_size(hn, ps):
+    c = Case([(40, 130), (17, 17), (1, 90), (70, 71), (20, 300)], nq=4, nkv=2, hn=hn, ps=ps, dtype=BF16, pad=1, garbage=float("inf"))
+    check_attention(c, *run_attention(c))
+
+
+@pytest.mark.parametrize("seqs,max_kv", [([(1, 70), (2, 9), (1, 400)], 0), ([(1, 3000), (1, 70)], 0), ([(40, 300), (2, 9)], 0),
+                                         ([(40, 1500), (1, 700)], 9000)])
+def test_attention_outputs_in_wider_tensors(seqs, max_kv):
+    """Outputs as slices of wider tensors, whose other elements stay; rows ahead of the first sequence stay too."""
+    from multimodal_amd import ops
+    from multimodal_amd.kv_cache import PagedStep
+    c = Case(seqs, nq=4, nkv=2, hn=64, ps=16, dtype=BF16, pad=2, garbage=float("nan"))
+    ref = run_attention(c, **(dict(max_kv=max_kv) if max_kv else {}))
+    n, ahead = int(c.cu[-1]), 3
+    step = PagedStep(c.block_table.cuda(), (c.cu + ahead).cuda(), c.lens.cuda(), c.max_new, max_kv or c.max_kv)
+    q = torch.cat((torch.full((ahead, 4, 64), float("nan"), dtype=BF16), c.q)).cuda()
+    wide = torch.full((ahead + c.rows, 4, 3, 72), 7.0, dtype=BF16, device="cuda")
+    lse = torch.full((ahead + c.rows, 9), 7.0, device="cuda")
+    ops.paged_attn_fwd(c.kv(), step, q, c.scale, out=wide[:, :, 1, 8:], lse=lse[:, 2:6])
+    assert torch.equal(wide[ahead:ahead + n, :, 1, 8:], ref[0][:n]) and torch.equal(lse[ahead:ahead + n, 2:6], ref[1][:n])
+    wide[ahead:ahead + n, :, 1, 8:] = 7.0
+    lse[ahead:ahead + n, 2:6] = 7.0
+    assert bool((wide == 7).all()) and bool((lse == 7).all())
+    # the append leaves them alone as well
+    kv, kv2 = c.kv(), c.kv()
+    cos, sin = (t.cuda() for t in tables(3000, 16, BF16))
+    k, v = (torch.cat((t[:ahead], t)).cuda() for t in (c.k, c.v))
+    qo = torch.full((ahead + c.rows, 4, 64), 7.0, dtype=BF16, device="cuda")
+    ops.paged_kv_append(kv, step, k, v, q=q, cos=cos, sin=sin, q_out=qo)
+    want = ops.paged_kv_append(kv2, c.step(), c.k.cuda(), c.v.cuda(), q=c.q.cuda(), cos=cos, sin=sin)
+    assert torch.equal(kv.k.nan_to_num(), kv2.k.nan_to_num()) and torch.equal(kv.v.nan_to_num(), kv2.v.nan_to_num())
+    assert torch.equal(qo[ahead:ahead + n], want[:n]) and bool((qo[:ahead] == 7).all()) and bool((qo[ahead + n:] == 7).all())
+
+
+def test_thousands_of_sequences():
+    """More sequences than two steps of the search for a row's sequence cover, some without rows; and many that are split and joined."""
+    c = Case([(1 + (i % 7 == 3) if i % 5 else 0, 3 + (i * 7) % 50) for i in range(4500)], nq=1, nkv=1, hn=64, ps=16, dtype=BF16, pad=1, seed=3)
+    cos, sin = tables(64, 16, BF16)
+    check_append(c, *run_append(c, cos, sin), cos, sin)
+    check_attention(c, *run_attention(c))
+    c = Case([(17 + i % 3 if i % 4 else 1, 20 + (i * 37) % 1100) for i in range(100)], nq=1, nkv=1, hn=64, ps=16, dtype=BF16, pad=1, seed=4)
+    from multimodal_amd._lib import get_lib
+    step, kv = c.step(), c.kv()
+    assert get_lib().mm_paged_attn_workspace_bytes(kv._ref, step._ref, c.nq, c.rows) > 0
+    check_attention(c, *run_attention(c))
+
+
+def test_a_replayed_step_follows_its_arrays():
+    """Pages, rows and lengths of a captured step are rewritten between the replays, a broken step among them."""
+    from multimodal_amd import ops
+    steps = [[(1, 300), (3, 700), (0, 20)], [(2, 40), (1, 1500), (1, 1)], [(0, 9), (4, 1499), (0, 0)], [(3, 2000), (1, 5), (0, 3)], [(1, 1), (1, 2), (2, 3)]]
+    cases = [Case(s, nq=4, nkv=2, hn=64, ps=16, dtype=BF16, seed=i) for i, s in enumerate(steps)]
+    pages, width = max(c.num_pages for c in cases), 94  # 1504 positions: the fourth step's 2000 are behind the table
+    table = torch.zeros(3, width, dtype=torch.int32, device="cuda")
+    cu, lens = torch.zeros(4, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    from multimodal_amd.kv_cache import PagedKV, PagedStep
+    kv = PagedKV(torch.zeros(pages, 2, 16, 64, dtype=BF16, device="cuda"), torch.zeros(pages, 2, 16, 64, dtype=BF16, device="cuda"))
+    step = PagedStep(table, cu, lens, max_new=4, max_kv=1504)
+    q = torch.zeros(4, 4, 64, dtype=BF16, device="cuda")
+    out, lse = torch.zeros(4, 4, 64, dtype=BF16, device="cuda"), torch.zeros(4, 4, device="cuda")
+    ops.paged_attn_fwd(kv, step, q, 0.125, out=out, lse=lse)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.paged_attn_fwd(kv, step, q, 0.125, out=out, lse=lse)
+    for c in cases + cases[::-1]:
+        bt = torch.full((3, width), -1, dtype=torch.int32)
+        w = min(width, c.block_table.size(1))
+        bt[:, :w] = c.block_table[:, :w]
+        table.copy_(bt)
+        cu.copy_(c.cu)
+        lens.copy_(c.lens)
+        kv.k[:c.num_pages].copy_(c.k_cache)
+        kv.v[:c.num_pages].copy_(c.v_cache)
+        n = int(c.cu[-1])
+        q[:n].copy_(c.q[:n])
+        out.fill_(7.0)
+        lse.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert bool((out[n:] == 7).all()) and bool((lse[n:] == 7).all())
+        if int(c.lens.max()) > 1504:
+            assert bool(torch.isnan(out[:3]).all()) and bool(torch.isnan(lse[:3]).all()) and not bool(torch.isnan(out[3]).any())
+        else:
+            check_attention(c, out, lse)
