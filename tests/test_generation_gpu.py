@@ -276,3 +276,16 @@ def test_generated_logits_are_those_of_the_oracle(monkeypatch):
         assert torch.equal(got.argmax(1), o)
     monkeypatch.undo()
     assert all(torch.equal(a, b) for a, b in zip(out, stack.generate(prompts, maximum_tokens=20)))
+
+
+def test_generation_under_inference_mode():
+    """With an ordinary stack, and with one made there, whose tensors count no versions: the same tokens."""
+    g = torch.Generator().manual_seed(6)
+    prompts = [torch.randint(0, 1000, (n,), generator=g) for n in (5, 17)]
+    _, stack = build("tiny")
+    ref = stack.generate(prompts, maximum_tokens=12)
+    with torch.inference_mode():
+        assert all(torch.equal(a, b) for a, b in zip(stack.generate(prompts, maximum_tokens=12), ref))
+        _, own = build("tiny")
+        assert all(torch.equal(a, b) for a, b in zip(own.generate(prompts, maximum_tokens=12), ref))
+    assert all(torch.equal(a, b) for a, b in zip(own.generate(prompts, maximum_tokens=12), ref))
