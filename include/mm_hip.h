@@ -411,8 +411,8 @@ int mm_paged_kv_append(const mm_paged_kv* kv, const mm_paged_step* step, const v
  * -inf; rows of no sequence are left as they were.  What the cache holds behind a sequence's end, and infinities or NaN in keys
  * and values that a row does not see, do not reach it; an infinite value that it does see is infinite in its output, however small
  * its weight.  q, out [rows, nq, hn]: 16-byte aligned, strides a multiple of 8 elements; lse [rows, nq] with row stride l_row; out
- * may be q (the same strides), else out and lse overlap neither the inputs nor each other nor themselves (refused where it is q
- * or they).  workspace: mm_paged_attn_workspace_bytes bytes (0: none; it depends on the shapes and bounds alone), 16-byte
+ * may be q (the same strides); else out and lse overlap neither the inputs nor each other nor themselves (refused among q, out
+ * and lse).  workspace: mm_paged_attn_workspace_bytes bytes (0: none; it depends on the shapes and bounds alone), 16-byte
  * aligned; calls that share one must not overlap.  Deterministic. */
 size_t mm_paged_attn_workspace_bytes(const mm_paged_kv* kv, const mm_paged_step* step, int nq, int rows);
 int mm_paged_attn_fwd(const mm_paged_kv* kv, const mm_paged_step* step, void* out, int64_t o_row, int64_t o_head, float* lse,

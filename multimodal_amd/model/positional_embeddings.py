@@ -20,6 +20,10 @@ class RotaryEmbedding(torch.nn.Module):
         self._kept = {}     # tables of generation: key -> (inv_freq, its version, cos, sin, event)
         self._replaced = []  # those of frequencies the module no longer holds
 
+    def __getstate__(self):
+        """A copy (copy.deepcopy, pickle) makes its own tables: the events behind these can be neither copied nor saved."""
+        return {**self.__dict__, "seq_len_cached": None, "cos_cached": None, "sin_cached": None, "_stamp": None, "_kept": {}, "_replaced": []}
+
     def _build(self, x, seq_len):
         t = torch.arange(seq_len, device=x.device).type_as(self.inv_freq)
         freqs = torch.einsum("i,j->ij", t, self.inv_freq.to(x.device))

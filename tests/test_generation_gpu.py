@@ -289,3 +289,18 @@ def test_generation_under_inference_mode():
         _, own = build("tiny")
         assert all(torch.equal(a, b) for a, b in zip(own.generate(prompts, maximum_tokens=12), ref))
     assert all(torch.equal(a, b) for a, b in zip(own.generate(prompts, maximum_tokens=12), ref))
+
+
+def test_a_stack_is_copied_after_it_has_generated_and_run():
+    import copy
+    g = torch.Generator().manual_seed(6)
+    prompts = [torch.randint(0, 1000, (n,), generator=g) for n in (5, 17)]
+    cfg, stack = build("tiny")
+    ref = stack.generate(prompts, maximum_tokens=8)
+    with torch.no_grad():
+        stack.layers[0](torch.zeros(8, 2, cfg["hidden_size"], dtype=torch.bfloat16, device="cuda"), stack.attention_mask(8, "cuda"))
+    twin = copy.deepcopy(stack)
+    with torch.no_grad():
+        for layer in stack.layers:  # the copy's frequencies and tables are its own
+            layer.attention.rotary_emb.inv_freq.zero_()
+    assert all(torch.equal(a, b) for a, b in zip(twin.generate(prompts, maximum_tokens=8), ref))
